@@ -60,6 +60,18 @@ EXPORTED_SYMBOLS = (
     "cppmega_mi355_mask_sparse_indices",
 )
 
+# include/cppmega_mi355_layer.h
+LAYER_SYMBOLS = (
+    "cppmega_mi355_rms_norm",
+    "cppmega_mi355_rms_norm_bwd_workspace_bytes",
+    "cppmega_mi355_rms_norm_bwd",
+    "cppmega_mi355_grouped_gemm",
+)
+NORM_MAX_WIDTH = 32768                # CPPMEGA_MI355_NORM_MAX_WIDTH
+GROUPED_MAX_EXPERTS = 1024            # CPPMEGA_MI355_GROUPED_MAX_EXPERTS
+# operations of the grouped products
+GROUPED_ROWS, GROUPED_ROWS_GRAD, GROUPED_WEIGHTS_GRAD = range(3)
+
 
 class NativeLibraryError(RuntimeError):
     """The HIP library is missing, stale or unusable."""
@@ -368,6 +380,80 @@ class MaskIndicesArgs(C.Structure):
         ("indices", C.c_void_p),
     ]
 
+
+class RmsNormArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("x_dtype", C.c_int32),
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("weight_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("out", C.c_void_p),
+        ("residual_out", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("rows", C.c_int64),
+        ("x_pitch", C.c_int64),
+        ("residual_pitch", C.c_int64),
+        ("out_pitch", C.c_int64),
+        ("residual_out_pitch", C.c_int64),
+        ("width", C.c_int32),
+        ("eps", C.c_float),
+        ("scale_block", C.c_int32),
+        ("pow2_scales", C.c_int32),
+    ]
+
+
+class RmsNormBwdArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("dy", C.c_void_p),
+        ("h", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("dh", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dweight", C.c_void_p),
+        ("weight_dtype", C.c_int32),
+        ("width", C.c_int32),
+        ("rows", C.c_int64),
+        ("dy_pitch", C.c_int64),
+        ("h_pitch", C.c_int64),
+        ("dh_pitch", C.c_int64),
+        ("dx_pitch", C.c_int64),
+        ("eps", C.c_float),
+        ("reserved", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class GroupedGemmArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("op", C.c_int32),
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("y", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("x_scale", C.c_void_p),
+        ("w_scale", C.c_void_p),
+        ("x_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("offsets_dtype", C.c_int32),
+        ("x_scale_block", C.c_int32),
+        ("rows", C.c_int64),
+        ("x_pitch", C.c_int64),
+        ("w_pitch", C.c_int64),
+        ("y_pitch", C.c_int64),
+        ("experts", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("zero_tail", C.c_int32),
+    ]
+
+
 _lock = threading.RLock()
 _lib: C.CDLL | None = None
 
@@ -391,7 +477,7 @@ def load() -> C.CDLL:
             lib = C.CDLL(str(LIB_PATH))
         except OSError as exc:
             raise NativeLibraryError(f"cannot load {LIB_PATH}: {exc}") from exc
-        missing = [name for name in EXPORTED_SYMBOLS if not hasattr(lib, name)]
+        missing = [name for name in EXPORTED_SYMBOLS + LAYER_SYMBOLS if not hasattr(lib, name)]
         if missing:
             raise NativeLibraryError(f"{LIB_PATH} does not export {missing}; rebuild it")
         lib.cppmega_mi355_status.argtypes = [C.POINTER(StatusStruct), C.c_size_t]
@@ -439,6 +525,12 @@ def load() -> C.CDLL:
                            (lib.cppmega_mi355_mask_sparse_indices, MaskIndicesArgs)):
             fn.argtypes = [C.POINTER(struct), C.c_size_t, C.c_void_p]
             fn.restype = C.c_int
+        for fn, struct in ((lib.cppmega_mi355_rms_norm, RmsNormArgs), (lib.cppmega_mi355_rms_norm_bwd, RmsNormBwdArgs),
+                           (lib.cppmega_mi355_grouped_gemm, GroupedGemmArgs)):
+            fn.argtypes = [C.POINTER(struct), C.c_size_t, C.c_void_p]
+            fn.restype = C.c_int
+        lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.argtypes = [C.POINTER(RmsNormBwdArgs), C.c_size_t, C.POINTER(C.c_size_t)]
+        lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.restype = C.c_int
         lib.cppmega_mi355_fp8_vecmat_workspace_bytes.argtypes = [
             C.POINTER(VecmatArgs), C.c_size_t, C.POINTER(C.c_size_t)]
         lib.cppmega_mi355_fp8_vecmat_workspace_bytes.restype = C.c_int
@@ -553,6 +645,38 @@ def require_device_tensor(t: torch.Tensor, name: str, ref: torch.Tensor | None =
         raise ValueError(f"{name} must be contiguous (the boundary does not copy); got strides {t.stride()}")
     if ref is not None and t.device != ref.device:
         raise ValueError(f"{name} is on {t.device} but other operands are on {ref.device}")
+
+
+def row_pitch(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """(rows, elements between rows) of ``t[..., n]``: the last axis contiguous, the others one evenly spaced run of rows."""
+    if t.ndim < 1:
+        raise ValueError(f"{name} must have at least one axis")
+    n = t.shape[-1]
+    if n > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last axis of {name} must be contiguous (the boundary does not copy); got strides {t.stride()}")
+    rows, pitch = 1, None
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size != 1:
+            if pitch is None:
+                pitch = stride
+            elif stride != pitch * rows and 0 not in t.shape:
+                raise ValueError(f"the rows of {name} must be evenly spaced (the boundary does not copy); got strides {t.stride()}")
+        rows *= size
+    return rows, n if pitch is None else pitch
+
+
+def require_rows(t: torch.Tensor, name: str, ref: torch.Tensor | None = None) -> tuple[int, int]:
+    """A device tensor of rows with a pitch of their own; (rows, pitch)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor; got {type(t).__name__}")
+    if not t.is_cuda:
+        raise NativeCallError(
+            ERR_UNSUPPORTED,
+            f"{name} lives on {t.device}; the MI355X kernels take device tensors only and there is no CPU path",
+        )
+    if ref is not None and t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device} but other operands are on {ref.device}")
+    return row_pitch(t, name)
 
 
 def current_stream(device: torch.device) -> int:

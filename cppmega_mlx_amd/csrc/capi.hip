@@ -42,6 +42,10 @@ int dsa_indexer_loss_launch(const cppmega_mi355_dsa_loss_args_t& a, hipStream_t 
 int dsa_indexer_loss_workspace_bytes(const cppmega_mi355_dsa_loss_args_t& a, size_t* bytes);
 int head_gemm_launch(const cppmega_mi355_head_gemm_args_t& a, hipStream_t stream);
 int dequant_block_fp8_launch(const cppmega_mi355_dequant_block_args_t& a, hipStream_t stream);
+int rms_norm_launch(const cppmega_mi355_rms_norm_args_t& a, hipStream_t stream);
+int rms_norm_bwd_launch(const cppmega_mi355_rms_norm_bwd_args_t& a, hipStream_t stream);
+int rms_norm_bwd_workspace_bytes(const cppmega_mi355_rms_norm_bwd_args_t& a, size_t* bytes);
+int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream);
 int indexer_topk_launch(const cppmega_mi355_indexer_args_t& a, hipStream_t stream);
 int indexer_topk_workspace_bytes(const cppmega_mi355_indexer_args_t& a, size_t* bytes);
 
@@ -393,6 +397,27 @@ int cppmega_mi355_fp8_vecmat_workspace_bytes(const cppmega_mi355_vecmat_args_t* 
 int cppmega_mi355_fp8_vecmat(const cppmega_mi355_vecmat_args_t* args, size_t args_size, void* stream) {
   CM_CHECK_ARGS(args, args_size, cppmega_mi355_vecmat_args_t);
   return fp8_vecmat_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_rms_norm(const cppmega_mi355_rms_norm_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_rms_norm_args_t);
+  return rms_norm_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_rms_norm_bwd_workspace_bytes(const cppmega_mi355_rms_norm_bwd_args_t* args, size_t args_size, size_t* bytes) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_rms_norm_bwd_args_t);
+  if (!bytes) return fail(CPPMEGA_MI355_ERR_NULL, "bytes is NULL");
+  return rms_norm_bwd_workspace_bytes(*args, bytes);
+}
+
+int cppmega_mi355_rms_norm_bwd(const cppmega_mi355_rms_norm_bwd_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_rms_norm_bwd_args_t);
+  return rms_norm_bwd_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_grouped_gemm(const cppmega_mi355_grouped_gemm_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_grouped_gemm_args_t);
+  return grouped_gemm_launch(*args, (hipStream_t)stream);
 }
 
 }  // extern "C"

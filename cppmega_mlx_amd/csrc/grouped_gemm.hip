@@ -1,0 +1,34 @@
+// Products grouped by expert: checks and the choice of a kernel (gfx950).
+
+#include "grouped_gemm.h"
+
+namespace cm {
+
+int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
+  if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: unknown op %d", a.op);
+  if (a.rows < 0 || a.rows > 0x7fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
+  if (a.experts > kMaxExperts) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %d experts, at most %d are served", a.experts, kMaxExperts);
+  const bool fp8 = a.x_dtype == CPPMEGA_MI355_E4M3;
+  if (!fp8 && a.x_dtype != CPPMEGA_MI355_F16 && a.x_dtype != CPPMEGA_MI355_BF16)
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: operands of dtype %d are not float16 / bfloat16 / e4m3", a.x_dtype);
+  if (fp8 && a.op != kRows) return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: gradients of e4m3 operands are not served");
+  if (fp8 ? a.y_dtype != CPPMEGA_MI355_F32 && a.y_dtype != CPPMEGA_MI355_F16 && a.y_dtype != CPPMEGA_MI355_BF16
+          : a.y_dtype != CPPMEGA_MI355_F32 && a.y_dtype != a.x_dtype)
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: a result of dtype %d from operands of dtype %d", a.y_dtype, a.x_dtype);
+  if (a.offsets_dtype != CPPMEGA_MI355_I32 && a.offsets_dtype != CPPMEGA_MI355_I64)
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: offsets must be int32 or int64");
+  if (fp8 && a.x_scale_block != 0 && a.x_scale_block != 128)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: x_scale_block must be 0 (per row) or 128, got %d", a.x_scale_block);
+  if (a.rows == 0 && a.op != kWeightsGrad) return 0;
+  if (!a.y || !a.offsets || (a.rows > 0 && (!a.x || !a.w)) || (fp8 && (!a.x_scale || !a.w_scale)))
+    return fail(CPPMEGA_MI355_ERR_NULL, "grouped_gemm: x / w / y / offsets / scales is NULL");
+  GroupedParams p;
+  p.x = a.x; p.w = a.w; p.y = a.y; p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale;
+  p.rows = a.rows; p.x_pitch = a.x_pitch; p.w_pitch = a.w_pitch; p.y_pitch = a.y_pitch;
+  p.experts = a.experts; p.n = a.n; p.k = a.k;
+  p.y_dtype = a.y_dtype; p.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; p.x_scale_block = a.x_scale_block; p.zero_tail = a.zero_tail;
+  return grouped_general_launch(p, a.op, a.x_dtype, stream);
+}
+
+}  // namespace cm

@@ -882,3 +882,223 @@ def mask_sparse_indices(mask: torch.Tensor, out: torch.Tensor, *, topk: int) -> 
         rc = _lib.load().cppmega_mi355_mask_sparse_indices(C.byref(a), C.sizeof(a), _lib.current_stream(out.device))
     _lib.check(rc, "mask_sparse_indices")
     return out
+
+
+# ---------------------------------------------------------------------------
+# RMS norm of the residual stream
+# ---------------------------------------------------------------------------
+def _norm_weight(weight: torch.Tensor, x: torch.Tensor) -> None:
+    _lib.require_device_tensor(weight, "weight", x)
+    if tuple(weight.shape) != (x.shape[-1],):
+        raise ValueError(f"weight must have shape {(x.shape[-1],)}; got {tuple(weight.shape)}")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"weight must be float32 or of the rows' type {x.dtype}; got {weight.dtype}")
+
+
+def _like_rows(t: torch.Tensor, name: str, x: torch.Tensor, dtype: torch.dtype) -> int:
+    """Pitch of a tensor of x's shape."""
+    _, pitch = _lib.require_rows(t, name, x)
+    if tuple(t.shape) != tuple(x.shape) or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} with shape {tuple(x.shape)}; got {t.dtype} {tuple(t.shape)}")
+    return pitch
+
+
+def _own_rows(t: torch.Tensor, name: str, rows: int, pitch: int) -> None:
+    """Outputs must not write one place twice."""
+    if rows > 1 and abs(pitch) < t.shape[-1]:
+        raise ValueError(f"the rows of {name} overlap: strides {t.stride()}")
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float, out: torch.Tensor, residual: torch.Tensor | None = None,
+             residual_out: torch.Tensor | None = None, scale: torch.Tensor | None = None, scale_block: int = 0,
+             pow2_scales: bool = False) -> None:
+    """``out`` = norm(round(x + residual)) * weight into caller-owned buffers; uint8 ``out`` takes e4m3 codes with float32
+    ``scale`` ``x.shape[:-1]`` (scale_block 0) or ``[..., ceil(n / 128)]`` (128).  ``residual_out`` takes the sum."""
+    rows, x_pitch = _lib.require_rows(x, "x")
+    n = int(x.shape[-1])
+    a = _lib.RmsNormArgs()
+    a.struct_size = C.sizeof(a)
+    a.x_dtype = _dtype_or_raise(x, "x", (_lib.F32, _lib.F16, _lib.BF16))
+    _norm_weight(weight, x)
+    a.weight_dtype = _lib.dtype_code(weight)
+    fp8 = out.dtype == torch.uint8
+    if not fp8 and out.dtype != x.dtype:
+        raise TypeError(f"out must be {x.dtype} or uint8 (e4m3 codes); got {out.dtype}")
+    a.out_dtype = _lib.dtype_code(out)
+    a.out_pitch = _like_rows(out, "out", x, out.dtype)
+    _own_rows(out, "out", rows, a.out_pitch)
+    if fp8:
+        if scale_block not in (0, 128):
+            raise ValueError(f"scale_block must be 0 (per row) or 128, got {scale_block}")
+        want = tuple(x.shape[:-1]) + (((n + 127) // 128,) if scale_block else ())
+        if scale is None:
+            raise ValueError("e4m3 codes need a float32 scale")
+        _lib.require_device_tensor(scale, "scale", x)
+        if scale.dtype != torch.float32 or tuple(scale.shape) != want:
+            raise ValueError(f"scale must be float32 with shape {want}; got {scale.dtype} {tuple(scale.shape)}")
+    elif scale is not None:
+        raise ValueError("scale goes with e4m3 codes only")
+    if residual is not None:
+        a.residual_pitch = _like_rows(residual, "residual", x, x.dtype)
+    if residual_out is not None:
+        if residual is None:
+            raise ValueError("residual_out without a residual")
+        a.residual_out_pitch = _like_rows(residual_out, "residual_out", x, x.dtype)
+        _own_rows(residual_out, "residual_out", rows, a.residual_out_pitch)
+    a.x, a.residual, a.weight, a.out = x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), out.data_ptr()
+    a.residual_out, a.scale = _lib.ptr(residual_out), _lib.ptr(scale)
+    a.rows, a.width, a.x_pitch, a.eps = rows, n, x_pitch, float(eps)
+    a.scale_block, a.pow2_scales = int(scale_block), int(bool(pow2_scales))
+    with torch.cuda.device(x.device):
+        rc = _lib.load().cppmega_mi355_rms_norm(C.byref(a), C.sizeof(a), _lib.current_stream(x.device))
+    _lib.check(rc, "rms_norm")
+
+
+def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *, eps: float, dx: torch.Tensor, dweight: torch.Tensor,
+                      dh: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> None:
+    """Gradients of :func:`rms_norm` for the rows ``h`` that were normalised, into caller-owned ``dx`` (like h) and float32
+    ``dweight``; ``dh`` is the gradient that reaches the stream past the norm."""
+    rows, h_pitch = _lib.require_rows(h, "h")
+    n = int(h.shape[-1])
+    a = _lib.RmsNormBwdArgs()
+    a.struct_size = C.sizeof(a)
+    a.dtype = _dtype_or_raise(h, "h", (_lib.F32, _lib.F16, _lib.BF16))
+    _norm_weight(weight, h)
+    a.weight_dtype = _lib.dtype_code(weight)
+    a.h_pitch, a.dy_pitch, a.dx_pitch = h_pitch, _like_rows(dy, "dy", h, h.dtype), _like_rows(dx, "dx", h, h.dtype)
+    _own_rows(dx, "dx", rows, a.dx_pitch)
+    if dh is not None:
+        a.dh_pitch = _like_rows(dh, "dh", h, h.dtype)
+    _lib.require_device_tensor(dweight, "dweight", h)
+    if dweight.dtype != torch.float32 or tuple(dweight.shape) != (n,):
+        raise ValueError(f"dweight must be float32 with shape {(n,)}; got {dweight.dtype} {tuple(dweight.shape)}")
+    a.dy, a.h, a.weight, a.dh = dy.data_ptr(), h.data_ptr(), weight.data_ptr(), _lib.ptr(dh)
+    a.dx, a.dweight = dx.data_ptr(), dweight.data_ptr()
+    a.rows, a.width, a.eps = rows, n, float(eps)
+    lib = _lib.load()
+    stream = _lib.current_stream(h.device)
+    need = C.c_size_t(0)
+    _lib.check(lib.cppmega_mi355_rms_norm_bwd_workspace_bytes(C.byref(a), C.sizeof(a), C.byref(need)), "rms_norm_bwd")
+    if need.value:
+        if workspace is None:
+            workspace = _workspace(h.device, need.value, stream)
+        else:
+            _lib.require_device_tensor(workspace, "workspace", h)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    with torch.cuda.device(h.device):
+        rc = lib.cppmega_mi355_rms_norm_bwd(C.byref(a), C.sizeof(a), stream)
+    _lib.check(rc, "rms_norm_bwd")
+
+
+# ---------------------------------------------------------------------------
+# products grouped by expert
+# ---------------------------------------------------------------------------
+def _grouped_args(op: int, x: torch.Tensor, offsets: torch.Tensor, experts: int, n: int, k: int) -> _lib.GroupedGemmArgs:
+    a = _lib.GroupedGemmArgs()
+    a.struct_size = C.sizeof(a)
+    a.op = op
+    _lib.require_device_tensor(offsets, "offsets", x)
+    a.offsets_dtype = _dtype_or_raise(offsets, "offsets", (_lib.I32, _lib.I64))
+    if tuple(offsets.shape) != (experts + 1,):
+        raise ValueError(f"offsets must have shape {(experts + 1,)} for {experts} experts; got {tuple(offsets.shape)}")
+    a.offsets = offsets.data_ptr()
+    a.x_dtype = _lib.dtype_code(x)
+    a.rows, a.experts, a.n, a.k = x.shape[0], experts, n, k
+    return a
+
+
+def _rows2d(t: torch.Tensor, name: str, shape: tuple[int, int], ref: torch.Tensor | None = None) -> int:
+    _, pitch = _lib.require_rows(t, name, ref)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}; got {tuple(t.shape)}")
+    return pitch
+
+
+def _expert_weights(w: torch.Tensor, name: str, ref: torch.Tensor) -> tuple[int, int, int]:
+    _lib.require_device_tensor(w, name, ref)
+    if w.ndim != 3:
+        raise ValueError(f"{name} must be [E, N, K]; got {tuple(w.shape)}")
+    return tuple(int(d) for d in w.shape)
+
+
+def _grouped_call(a: _lib.GroupedGemmArgs, device: torch.device) -> None:
+    with torch.cuda.device(device):
+        rc = _lib.load().cppmega_mi355_grouped_gemm(C.byref(a), C.sizeof(a), _lib.current_stream(device))
+    _lib.check(rc, "grouped_gemm")
+
+
+_HALF = (torch.float16, torch.bfloat16)
+
+
+def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor, zero_tail: bool = False,
+                 transposed: bool = False) -> torch.Tensor:
+    """out[t, n] = sum_k x[t, k] w[e(t), n, k] into caller-owned ``out``; ``transposed``: out[t, k] = sum_n x[t, n] w[e(t), n, k].
+
+    Rows ``offsets[e] .. offsets[e + 1]`` belong to expert e; rows behind the last expert are left as they are, or zeroed."""
+    _lib.require_rows(x, "x")
+    if x.ndim != 2 or x.dtype not in _HALF:
+        raise TypeError(f"x must be a 2D float16 or bfloat16 tensor of rows; got {x.dtype} {tuple(x.shape)}")
+    E, N, K = _expert_weights(w, "w", x)
+    if w.dtype != x.dtype:
+        raise TypeError(f"w must be {x.dtype} like x; got {w.dtype}")
+    T = int(x.shape[0])
+    inner, outer = (N, K) if transposed else (K, N)
+    a = _grouped_args(_lib.GROUPED_ROWS_GRAD if transposed else _lib.GROUPED_ROWS, x, offsets, E, N, K)
+    a.x_pitch = _rows2d(x, "x", (T, inner))
+    a.y_pitch = _rows2d(out, "out", (T, outer), x)
+    _own_rows(out, "out", T, a.y_pitch)
+    a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, a.x_dtype))
+    a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
+    _grouped_call(a, x.device)
+    return out
+
+
+def grouped_weights_grad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor) -> torch.Tensor:
+    """out[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k] (zeros for an expert without rows)."""
+    _lib.require_rows(x, "x")
+    if x.ndim != 2 or x.dtype not in _HALF:
+        raise TypeError(f"x must be a 2D float16 or bfloat16 tensor of rows; got {x.dtype} {tuple(x.shape)}")
+    E, N, K = _expert_weights(out, "out", x)
+    T = int(x.shape[0])
+    if dy.dtype != x.dtype:
+        raise TypeError(f"dy must be {x.dtype} like x; got {dy.dtype}")
+    a = _grouped_args(_lib.GROUPED_WEIGHTS_GRAD, x, offsets, E, N, K)
+    a.w_pitch = _rows2d(x, "x", (T, K))
+    a.x_pitch = _rows2d(dy, "dy", (T, N), x)
+    a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, a.x_dtype))
+    a.x, a.w, a.y = dy.data_ptr(), x.data_ptr(), out.data_ptr()
+    _grouped_call(a, x.device)
+    return out
+
+
+def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor, *,
+                     out: torch.Tensor, zero_tail: bool = False) -> torch.Tensor:
+    """The product of e4m3 rows (uint8, float32 ``x_scale`` [T] or [T, ceil(K / 128)]) and their expert's e4m3 weight (uint8
+    [E, N, K], float32 ``w_scale`` [E, ceil(N / 128), ceil(K / 128)]) into caller-owned ``out`` [T, N]."""
+    _lib.require_rows(x, "x")
+    if x.ndim != 2 or x.dtype != torch.uint8:
+        raise TypeError(f"x must be 2D uint8 (fp8 storage); got {x.dtype} {tuple(x.shape)}")
+    E, N, K = _expert_weights(w, "w", x)
+    if w.dtype != torch.uint8:
+        raise TypeError(f"w must be uint8 (fp8 storage); got {w.dtype}")
+    T = int(x.shape[0])
+    a = _grouped_args(_lib.GROUPED_ROWS, x, offsets, E, N, K)
+    a.x_pitch = _rows2d(x, "x", (T, K))
+    a.y_pitch = _rows2d(out, "out", (T, N), x)
+    _own_rows(out, "out", T, a.y_pitch)
+    a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, _lib.F16, _lib.BF16))
+    blocks_n, blocks_k = (N + 127) // 128, (K + 127) // 128
+    for name, t in (("x_scale", x_scale), ("w_scale", w_scale)):
+        _lib.require_device_tensor(t, name, x)
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32; got {t.dtype}")
+    if tuple(x_scale.shape) == (T, blocks_k):
+        a.x_scale_block = 128
+    elif tuple(x_scale.shape) != (T,):
+        raise ValueError(f"x_scale must have shape {(T,)} or {(T, blocks_k)}; got {tuple(x_scale.shape)}")
+    if tuple(w_scale.shape) != (E, blocks_n, blocks_k):
+        raise ValueError(f"w_scale must have shape {(E, blocks_n, blocks_k)}; got {tuple(w_scale.shape)}")
+    a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
+    a.x_scale, a.w_scale = x_scale.data_ptr(), w_scale.data_ptr()
+    _grouped_call(a, x.device)
+    return out
