@@ -68,7 +68,7 @@ LAYER_SYMBOLS = (
     "cppmega_mi355_grouped_gemm",
 )
 NORM_MAX_WIDTH = 32768                # CPPMEGA_MI355_NORM_MAX_WIDTH
-GROUPED_MAX_EXPERTS = 1024            # CPPMEGA_MI355_GROUPED_MAX_EXPERTS
+GROUPED_MAX_EXPERTS = 512             # CPPMEGA_MI355_GROUPED_MAX_EXPERTS
 # operations of the grouped products
 GROUPED_ROWS, GROUPED_ROWS_GRAD, GROUPED_WEIGHTS_GRAD = range(3)
 

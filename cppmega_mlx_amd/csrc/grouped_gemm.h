@@ -34,9 +34,9 @@ __device__ __forceinline__ long long offset_of(const GroupedParams& p, int e) {
   return o < 0 ? 0 : (o > p.rows ? p.rows : o);
 }
 
-// Row tiles of all experts in a row: which expert tile t belongs to, and its rows.  Called by every thread of the workgroup;
-// `starts` is kMaxExperts + 2 ints of LDS (first tile of every expert), filled by the first wavefront.  The rows behind the last expert
-// are those of a last "expert" without a contraction when they are to be zeroed.
+// Row tiles of all experts in a row, BM rows each: the first tile of every expert in `starts` (kMaxExperts + 2 ints of LDS, filled by
+// the first wavefront for the whole workgroup); their number comes back.  The rows behind the last expert are those of a last "expert"
+// without a contraction when they are to be zeroed.
 template <int BM>
 __device__ __forceinline__ int fill_tiles(const GroupedParams& p, int* starts) {
   if (threadIdx.x < 64) {
@@ -71,5 +71,6 @@ __device__ __forceinline__ int expert_of_tile(const GroupedParams& p, const int*
 }
 
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
 
 }  // namespace cm

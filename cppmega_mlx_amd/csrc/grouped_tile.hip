@@ -1,0 +1,480 @@
+// Products grouped by expert for many rows (gfx950): 256 x 256 tiles, operands by the load unit into LDS.
+//
+// Needs rows that begin on 16 bytes and a contraction (and, where it is the slow axis, columns) in whole 16-byte pieces.
+//
+// Eight wavefronts, 128 x 64 of the tile each, two on every SIMD; a stage is 128 bytes of contraction of both operands (64 KB, two
+// stages in LDS).  Rows that are not there repeat the last one and are not stored; contraction that is not there comes from a piece of
+// zeros, for both operands (what lies behind a row may be NaN).  A wavefront whose rows are not there only loads.
+// Pieces are 16 bytes; in LDS
+//   contraction contiguous: [row][8 pieces], piece c of row r in place c ^ (r / 2 % 8);
+//   contraction slow: [step of 64][32 pieces of 8 channels], piece c of step s in place c ^ 4 (s % 4), read by the transposing load.
+
+#include <type_traits>
+
+#include "grouped_gemm.h"
+
+namespace cm {
+namespace {
+
+__device__ __align__(64) const unsigned char zeros[64] = {};
+
+template <int OP, int DT>
+struct Shape {
+  static constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
+  static constexpr bool TR = OP == kWeightsGrad, TQ = OP != kRows;      // the contraction is the operand's slow axis
+  // bytes of contraction in a stage, and how many stages of each operand LDS holds
+  static constexpr int KB = FP8 || !TQ ? 128 : 64, RS = FP8 ? 2 : TQ ? 5 : 3, QS = FP8 ? 2 : TQ ? 5 : 2;
+  static constexpr int BYTES = FP8 ? 1 : 2, STEP = KB / BYTES;
+  static constexpr int BM = 256, BN = 256, WN = 4;
+  static constexpr int RL = BM * KB / 8192, QL = BN * KB / 8192, L = RL + QL + (FP8 ? 1 : 0);   // load instructions per wavefront and stage
+  static constexpr int kR = BM * KB, kQ = BN * KB, kS = FP8 ? 8 * 256 : 0;
+  static constexpr int kQat = RS * kR, kSat = kQat + QS * kQ, kLds = kSat + QS * kS;            // where columns and scales begin
+  // the place of piece c of a row among its row's pieces is c ^ fold(row): sixteen rows with one piece lie in different banks
+  static __device__ __forceinline__ int fold(int row) { return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
+};
+
+template <int OP, int DT>
+__global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParams p) {
+  typedef Shape<OP, DT> S;
+  constexpr bool FP8 = S::FP8, F16 = S::F16, TR = S::TR, TQ = S::TQ;
+  constexpr int BYTES = S::BYTES, STEP = S::STEP, BM = S::BM, BN = S::BN, RS = S::RS, QS = S::QS, RL = S::RL, QL = S::QL, L = S::L, KB = S::KB;
+  __shared__ u32x4 smem[S::kLds / 16];
+  static_assert(sizeof(smem) >= (kMaxExperts + 2) * sizeof(int), "the tiles' table lies where the stages are later");
+  int* const starts = reinterpret_cast<int*>(smem);
+  char* const lds = reinterpret_cast<char*>(smem);
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = (wave / S::WN) * 128, wn = (wave % S::WN) * 64;
+
+  // ---- which tile: every XCD takes one run of the order, which goes through the experts; of each, up to four row tiles share the
+  // columns that pass, so that an expert's weight leaves memory once (groups of four rows of tiles whatever their experts: 5 % slower) ----
+  const int cols_c = OP == kRows ? p.n : p.k;
+  const int tiles_n = (cols_c + BN - 1) / BN;
+  const int per_expert = OP == kWeightsGrad ? (p.n + BM - 1) / BM : 0;
+  int e, m0, n0;
+  {
+    const int total = (OP == kWeightsGrad ? p.experts * per_expert : fill_tiles<BM>(p, starts)) * tiles_n;
+    const int q = total >> 3, r = total & 7, xcd = (int)blockIdx.x & 7, at = (int)blockIdx.x >> 3;
+    if (at >= q + (xcd < r ? 1 : 0)) return;
+    const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
+    e = OP == kWeightsGrad ? id / (per_expert * tiles_n) : expert_of_tile(p, starts, id / tiles_n);
+    const int first = OP == kWeightsGrad ? e * per_expert : starts[e], high = OP == kWeightsGrad ? per_expert : starts[e + 1] - first;
+    const int groups = (high + 3) / 4, step = (high + groups - 1) / groups;       // rows of tiles in a group
+    const int local = id - first * tiles_n, group = local / (step * tiles_n), in = local - group * step * tiles_n;
+    const int height = high - group * step < step ? high - group * step : step;
+    const int nt = in / height;
+    n0 = nt * BN;
+    m0 = (group * step + in - nt * height) * BM;
+  }
+  const int lo = __builtin_amdgcn_readfirstlane((int)offset_of(p, e));
+  const int hi = __builtin_amdgcn_readfirstlane(e < p.experts ? (int)offset_of(p, e + 1) : (int)p.rows);
+  const int tokens = hi > lo ? hi - lo : 0;
+  m0 = __builtin_amdgcn_readfirstlane(m0);
+  n0 = __builtin_amdgcn_readfirstlane(n0);
+  const int contraction = OP == kWeightsGrad ? tokens : (e == p.experts ? 0 : (OP == kRows ? p.k : p.n));
+  const int rows_here = (OP == kWeightsGrad ? p.n : tokens) - m0, cols_here = cols_c - n0;
+  const int stages = (contraction + STEP - 1) / STEP, whole = contraction / STEP;
+  const long long w_pitch = OP == kWeightsGrad ? p.w_pitch : p.k;
+
+  // ---- loads ----
+  const char* xb = (const char*)p.x + ((size_t)lo * p.x_pitch + (TR ? (size_t)m0 : (size_t)m0 * p.x_pitch)) * BYTES;
+  const char* wb = (const char*)p.w + ((OP == kWeightsGrad ? (size_t)lo * p.w_pitch : (size_t)(e < p.experts ? e : 0) * p.n * p.k) + (TQ ? (size_t)n0 : (size_t)n0 * p.k)) * BYTES;
+  const long long x_step = TR ? p.x_pitch * STEP * BYTES : KB, w_step = TQ ? w_pitch * STEP * BYTES : KB;
+  unsigned xoff[RL], woff[QL], soff = 0;
+  // where a lane's piece of load instruction u of an operand lies, and how far along the contraction that is
+  constexpr int PIECES = KB / 16;                                // of a row in a stage
+  auto piece_of = [&](bool transposed, int u, int limit, long long pitch) -> unsigned {
+    if (!transposed) {
+      const int row = u * (64 / PIECES) + lane / PIECES, c = (lane % PIECES) ^ S::fold(row);
+      return (unsigned)((row < limit ? row : limit - 1) * pitch * BYTES) + (unsigned)c * 16u;
+    }
+    const int step = u * 2 + (lane >> 5), c = (lane & 31) ^ ((step & 3) << 2);
+    return (unsigned)(step * pitch * BYTES) + (unsigned)(c * 8 < limit ? c : (limit - 1) >> 3) * 16u;
+  };
+  auto along = [&](bool transposed, int u) {
+    return transposed ? u * 2 + (lane >> 5) : ((lane % PIECES) ^ S::fold(u * (64 / PIECES) + lane / PIECES)) * (16 / BYTES);
+  };
+#pragma unroll
+  for (int i = 0; i < RL; ++i) xoff[i] = piece_of(TR, wave * RL + i, rows_here, p.x_pitch);
+#pragma unroll
+  for (int i = 0; i < QL; ++i) woff[i] = piece_of(TQ, wave * QL + i, cols_here, w_pitch);
+  const char* sb = nullptr;
+  unsigned s_step = 0;
+  if constexpr (FP8) {
+    // the first four wavefronts bring the scales of 64 rows each, the others those of the columns' two blocks
+    const int blocks_k = (p.k + 127) / 128, blocks_n = (p.n + 127) / 128;
+    if (wave < 4) {
+      const int row = wave * 64 + lane;
+      sb = (const char*)(p.x_scale + (size_t)(lo + m0) * (p.x_scale_block ? blocks_k : 1));
+      soff = (unsigned)(row < rows_here ? row : rows_here - 1) * (p.x_scale_block ? (unsigned)blocks_k * 4u : 4u);
+      s_step = p.x_scale_block ? 4u : 0u;
+    } else {
+      const int b = n0 / 128 + (lane & 1);
+      sb = (const char*)(p.w_scale + (size_t)(e < p.experts ? e : 0) * blocks_n * blocks_k);
+      soff = (unsigned)(b < blocks_n ? b : blocks_n - 1) * (unsigned)blocks_k * 4u;
+      s_step = 4u;
+    }
+  }
+  const unsigned lds_base = (unsigned)(size_t)(lds_void*)smem;
+  auto load16 = [&](const char* base, unsigned off, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+  };
+  auto load16_at = [&](const char* at, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory", "m0");
+  };
+  auto load4 = [&](const char* base, unsigned off, unsigned to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+  };
+  int next_r = 0, next_q = 0;                                   // stages of rows and of columns to be requested next
+  unsigned r_slot = lds_base, q_slot = lds_base + S::kQat, s_slot = lds_base + S::kSat;
+  // Requests instruction i of a stage: the columns' (and scales') first, then the rows', which may be a stage further on.  MORE:
+  // whole stages.  Otherwise the last one, of which a part may not be there, or one behind it: pieces of zeros (no branch here or in the
+  // loops below: the compiler moves products across branches, away from the reads that they cover).
+  auto issue = [&](auto more, int from, int to) {
+    constexpr bool MORE = decltype(more)::value;
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      if (i < from || i >= to) continue;
+      if (i < L - RL) {
+        if (i < QL) {
+          const int u = wave * QL + i;
+          unsigned off = woff[i < QL ? i : 0];
+          if (MORE) {
+            load16(wb, off, q_slot + (unsigned)(u * 1024));
+          } else {
+            asm("" : "+v"(off));                                // (the address is made here, not kept in registers throughout)
+            load16_at(next_q * STEP + along(TQ, u) < contraction ? wb + off : (const char*)zeros, q_slot + (unsigned)(u * 1024));
+          }
+        } else {
+          const bool there = MORE || next_q < stages;
+          load4(there ? sb : (const char*)zeros, there ? soff : 0u, s_slot + (unsigned)(wave * 256));
+        }
+        if (i == L - RL - 1) {
+          wb += w_step;
+          sb += s_step;
+          ++next_q;
+          q_slot = q_slot + S::kQ == lds_base + S::kSat ? lds_base + S::kQat : q_slot + S::kQ;
+          if (FP8) s_slot = s_slot + S::kS == lds_base + S::kLds ? lds_base + S::kSat : s_slot + S::kS;
+        }
+      } else {
+        const int u = wave * RL + i - (L - RL);
+        unsigned off = xoff[i < L - RL ? 0 : i - (L - RL)];
+        if (MORE) {
+          load16(xb, off, r_slot + (unsigned)(u * 1024));
+        } else {
+          asm("" : "+v"(off));
+          load16_at(next_r * STEP + along(TR, u) < contraction ? xb + off : (const char*)zeros, r_slot + (unsigned)(u * 1024));
+        }
+        if (i == L - 1) {
+          xb += x_step;
+          ++next_r;
+          r_slot = r_slot + S::kR == lds_base + S::kQat ? lds_base : r_slot + S::kR;
+        }
+      }
+    }
+  };
+  typedef std::integral_constant<bool, true> Whole;
+  typedef std::integral_constant<bool, false> Part;
+  if (OP != kWeightsGrad) __syncthreads();                       // (the tiles' table has been read)
+  if (stages > 0) {
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+      if (s < RS - QS) issue(Part(), L - RL, L);
+      else if (s < whole) issue(Whole(), 0, L);
+      else issue(Part(), 0, L);
+    }
+    // rows 0 .. RS - QS, columns 0 have arrived
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((QS - 1) * L) : "memory");
+  }
+  const int steady = whole - RS;                                 // stages while whose products whole ones are requested
+  // between a stage's last operand reads and its last products: the next stage has arrived, and everybody has read this one
+  constexpr int kYounger = (QS - 2) * L + (RS > QS ? RL : 0);    // instructions behind those of the next stage
+  auto turn = [&] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kYounger) : "memory"); };
+  const bool live = wm < rows_here;
+  auto follow = [&] {                                           // a wavefront without rows: its loads only
+    for (int s = 0; s + 1 < stages; ++s) {
+      turn();
+      if (s < steady) issue(Whole(), 0, L);
+      else issue(Part(), 0, L);
+    }
+  };
+  int r_at = 0, q_at = S::kQat, s_at = S::kSat;                  // where the stage that is multiplied lies
+  auto r_after = [&] { return r_at + S::kR == S::kQat ? 0 : r_at + S::kR; };
+  auto q_after = [&] { return q_at + S::kQ == S::kSat ? S::kQat : q_at + S::kQ; };
+  auto s_after = [&] { return s_at + S::kS == S::kLds ? S::kSat : s_at + S::kS; };
+  const size_t row0 = OP == kWeightsGrad ? (size_t)e * p.n + m0 : (size_t)lo + m0;
+  const long long y_pitch = OP == kWeightsGrad ? p.k : p.y_pitch;
+  // 8 (16-bit) or 4 (float32) values of a row, as far as the columns go
+  auto store = [&](int row, int col, const float* v, int count) {
+    if (row >= rows_here || col >= cols_here) return;
+    const size_t at = (row0 + row) * y_pitch + n0 + col;
+    if (col + count <= cols_here) {
+      if (p.y_dtype == CPPMEGA_MI355_F32) {
+        __builtin_memcpy((float*)p.y + at, v, 4 * count);
+      } else {
+        unsigned r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * i < count) r[i] = p.y_dtype == CPPMEGA_MI355_F16 ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
+        __builtin_memcpy((unsigned short*)p.y + at, r, 2 * count);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < count && col + i < cols_here) store_as(p.y, at + i, p.y_dtype, v[i]);
+    }
+  };
+
+  if constexpr (!FP8) {
+    constexpr int TI = 4, TJ = 2;                               // 32 x 32 tiles of the wavefront
+    const int l32 = lane & 31, half = lane >> 5, l16 = lane & 15;
+    constexpr int KS = KB / 32;                                 // 16 steps of contraction at a time
+    int rat[TR ? TI : KS], qat[TQ ? TJ : KS];                     // where a lane reads: per tile (transposing), or per 16 steps
+    if (TR) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int col = wm + i * 32 + (lane & 16) + (l16 & 3) * 4;
+        rat[i] = (half * 8 + (l16 >> 2)) * (BM * 2) + ((col >> 3) ^ ((l16 >> 2) << 2)) * 16 + (col & 4) * 2;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) rat[k] = (wm + l32) * KB + ((2 * k + half) ^ S::fold(l32)) * 16;
+    }
+    if (TQ) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int col = wn + j * 32 + (lane & 16) + (l16 & 3) * 4;
+        qat[j] = (half * 8 + (l16 >> 2)) * (BN * 2) + ((col >> 3) ^ ((l16 >> 2) << 2)) * 16 + (col & 4) * 2;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < KS; ++k) qat[k] = (wn + l32) * KB + ((2 * k + half) ^ S::fold(l32)) * 16;
+    }
+    auto transposed = [&](int at, int pitch4) -> bf16x8 {       // eight steps of a lane's channel
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at)));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at + pitch4)));
+      return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
+    };
+    bf16x8 r[2][TI], q[2][TJ];
+    auto read_ahead = [&](int rows, int cols, int ks) {
+      const int to = ks & 1;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) q[to][j] = TQ ? transposed(cols + qat[j] + ks * 16 * BN * 2, 4 * BN * 2) : *reinterpret_cast<const bf16x8*>(lds + cols + qat[TQ ? 0 : ks] + j * 32 * KB);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) r[to][i] = TR ? transposed(rows + rat[i] + ks * 16 * BM * 2, 4 * BM * 2) : *reinterpret_cast<const bf16x8*>(lds + rows + rat[TR ? 0 : ks] + i * 32 * KB);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    f32x16 acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+    // products of one 16 steps; between them load instructions from .. (all at once, the wavefronts stood still until the load
+    // unit's queue had room)
+    auto multiply = [&](int b, auto more, int from) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          if constexpr (F16) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, q[b][j]), __builtin_bit_cast(f16x8, r[b][i]), acc[i][j], 0, 0, 0);
+          else acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q[b][j], r[b][i], acc[i][j], 0, 0, 0);
+        }
+        if (from >= 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          issue(more, L * i / TI, L * (i + 1) / TI);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto stage = [&](auto more) {
+      const int rows = r_after(), cols = q_after();
+#pragma unroll
+      for (int ks = 0; ks + 1 < KS; ++ks) {
+        read_ahead(r_at, q_at, ks + 1);
+        multiply(ks & 1, more, -1);
+      }
+      turn();
+      read_ahead(rows, cols, 0);
+      multiply((KS - 1) & 1, more, 0);
+      r_at = rows;
+      q_at = cols;
+    };
+    if (!live) {
+      follow();
+    } else if (stages > 0) {
+      read_ahead(r_at, q_at, 0);
+      int s = 0;
+      for (; s < steady; ++s) stage(Whole());
+      for (; s + 1 < stages; ++s) stage(Part());
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 1 < KS) read_ahead(r_at, q_at, ks + 1);
+        multiply(ks & 1, Part(), -1);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // (what was requested behind the end still writes to LDS)
+    // lane: row l % 32, columns 8 q + 4 (l / 32) + 0..3; the halves change places so that a lane has 8 columns in a run
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][h * 8 + c]), __float_as_uint(acc[i][j][h * 8 + 4 + c]), false, false);
+              v[c] = __uint_as_float(x[0]);
+              v[4 + c] = __uint_as_float(x[1]);
+            }
+            store(wm + i * 32 + l32, wn + j * 32 + h * 16 + half * 8, v, 8);
+          }
+    }
+  } else {
+    constexpr int TI = 8, TJ = 4;                               // 16 x 16 tiles of the wavefront, a whole 128-channel block an instruction
+    const int l16 = lane & 15, quad = lane >> 4, f = (l16 >> 1) & 7;
+    const int rat[2] = {(wm + l16) * 128 + (quad ^ f) * 16, (wm + l16) * 128 + ((quad + 4) ^ f) * 16};
+    const int qat[2] = {(wn + l16) * 128 + (quad ^ f) * 16, (wn + l16) * 128 + ((quad + 4) ^ f) * 16};
+    const int xsat = (wm + l16) * 4, wsat = 4 * 256 + (wn >> 7) * 4;
+    auto operand = [&](int a, int b) -> i32x8 {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(lds + a), y = *reinterpret_cast<const u32x4*>(lds + b);
+      i32x8 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = (int)x[i];
+        o[4 + i] = (int)y[i];
+      }
+      return o;
+    };
+    f32x4 acc[TI][TJ];
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    i32x8 q[TJ], r[2];
+    float sx[TI], sw;
+    auto read_q = [&](int from, int j) { q[j] = operand(from + qat[0] + j * 2048, from + qat[1] + j * 2048); };
+    auto read_r = [&](int from, int i) { r[i & 1] = operand(from + rat[0] + i * 2048, from + rat[1] + i * 2048); };
+    auto read_scales = [&](int from) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) sx[i] = *reinterpret_cast<const float*>(lds + from + xsat + i * 64);
+      sw = *reinterpret_cast<const float*>(lds + from + wsat);
+    };
+    // a block's products are scaled and added while the matrix unit is at the next ones
+    f32x4 t[2][TJ];
+    auto product = [&](int i, int j) {
+      const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      t[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[j], r[i & 1], zero, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    };
+    auto add = [&](int i) {
+      const float s = sx[i] * sw;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, t[i & 1][j][v], acc[i][j][v]);
+    };
+    // all rows but the last ones; load instructions from .. between them, PER to a group of products
+    constexpr int PER = 2;
+    auto products = [&](auto more, int from) {
+#pragma unroll
+      for (int i = 0; i < TI - 1; ++i) {
+        read_r(r_at, i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) product(i, j);
+        __builtin_amdgcn_sched_barrier(0);
+        if (from >= 0 && from + PER * i < L) issue(more, from + PER * i, from + PER * i + PER < L ? from + PER * i + PER : L);
+        if (i > 0) add(i - 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if (!live) {
+      follow();
+    } else if (stages > 0) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) read_q(q_at, j);
+      read_r(r_at, 0);
+      read_scales(s_at);
+      // between a stage and the next: the last rows' products, and the next operands as soon as their registers are free
+      auto pass = [&](auto more) {
+        const int rows = r_after(), cols = q_after();
+        turn();
+        read_r(rows, 0);
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          product(TI - 1, j);
+          __builtin_amdgcn_sched_barrier(0);
+          read_q(cols, j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        issue(more, 0, PER);
+        add(TI - 2);
+        add(TI - 1);
+        s_at = s_after();
+        read_scales(s_at);
+        __builtin_amdgcn_sched_barrier(0);
+        r_at = rows;
+        q_at = cols;
+      };
+      products(Part(), -1);
+      int s = 0;
+      for (; s < steady; ++s) {
+        pass(Whole());
+        products(Whole(), PER);
+      }
+      for (; s + 1 < stages; ++s) {
+        pass(Part());
+        products(Part(), PER);
+      }
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) product(TI - 1, j);
+      add(TI - 2);
+      add(TI - 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // lane: row l % 16, columns 4 (l / 16) + 0..3; two tiles' quarters change places so that a lane has 8 columns in a run
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; j += 2) {
+          float v[8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const u32x2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][c]), __float_as_uint(acc[i][j + 1][c]), false, false);
+            v[c] = __uint_as_float(x[0]);
+            v[4 + c] = __uint_as_float(x[1]);
+          }
+          store(wm + i * 16 + l16, wn + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, 8);
+        }
+    }
+  }
+}
+
+}  // namespace
+
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream) {
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + 255) / 256;
+  const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + 255) / 256) : p.rows / 256 + p.experts + 1;
+  if (tiles_m * tiles_n > 0x3fffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles_m * tiles_n);
+  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), block(512);
+#define CM_TILE(op_, dt) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt>), grid, block, 0, stream, p)
+#define CM_TILE_OP(op_)                                           \
+  do {                                                            \
+    if (dtype == CPPMEGA_MI355_F16) CM_TILE(op_, CPPMEGA_MI355_F16); \
+    else CM_TILE(op_, CPPMEGA_MI355_BF16);                        \
+  } while (0)
+  if (dtype == CPPMEGA_MI355_E4M3) CM_TILE(kRows, CPPMEGA_MI355_E4M3);
+  else if (op == kRows) CM_TILE_OP(kRows);
+  else if (op == kRowsGrad) CM_TILE_OP(kRowsGrad);
+  else CM_TILE_OP(kWeightsGrad);
+#undef CM_TILE_OP
+#undef CM_TILE
+  CM_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+}  // namespace cm

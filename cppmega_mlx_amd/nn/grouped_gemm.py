@@ -3,7 +3,7 @@
 ``x [T, K]`` holds the rows sorted by expert: rows ``offsets[e] .. offsets[e + 1] - 1`` belong to expert e.  ``offsets`` is an int32 or
 int64 device tensor ``[E + 1]`` that begins with 0, does not decrease and ends with T at most; it is read by the kernels
 on the stream (no read-back: calls can be captured into graphs, and replayed with other offsets).  ``w [E, N, K]`` is dense, the contraction
-index contiguous as in ``ops.head_gemm``; up to 1024 experts.
+index contiguous as in ``ops.head_gemm``; up to 512 experts.
 
     grouped_gemm        y[t, n] = sum_k x[t, k] w[e(t), n, k]             float16 / bfloat16, float32 sums, rounded once
     grouped_gemm_bwd    dx[t, k] = sum_n dy[t, n] w[e(t), n, k],  dw[e, n, k] = sum_{t in e} dy[t, n] x[t, k]
