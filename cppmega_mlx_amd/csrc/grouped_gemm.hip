@@ -5,12 +5,10 @@
 namespace cm {
 namespace {
 
-// Whether the load unit can write the operands to LDS: rows that begin on 16 bytes, and the axes that are read in pieces of 16 bytes
-// made of whole ones (offsets within a tile are 32-bit, hence the bound on pitches).  Float32 results of e4m3 operands stay with the
-// general kernel, whose products are exact.
+// Whether rows begin on 16 bytes and the axes that are read in pieces of 16 bytes are made of whole ones (offsets within a tile are
+// 32-bit, hence the bound on pitches).
 bool pieces_whole(const GroupedParams& p, int op, int dtype) {
   const int piece = dtype == CPPMEGA_MI355_E4M3 ? 16 : 8;
-  if (dtype == CPPMEGA_MI355_E4M3 && p.y_dtype == CPPMEGA_MI355_F32) return false;
   if (((uintptr_t)p.x | (uintptr_t)p.w) & 15) return false;
   if (p.k % piece != 0 || p.x_pitch % piece != 0 || p.x_pitch > (1 << 22) || p.k > (1 << 22)) return false;
   if (op != kRows && p.n % piece != 0) return false;
@@ -43,7 +41,12 @@ int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t 
   p.rows = a.rows; p.x_pitch = a.x_pitch; p.w_pitch = a.w_pitch; p.y_pitch = a.y_pitch;
   p.experts = a.experts; p.n = a.n; p.k = a.k;
   p.y_dtype = a.y_dtype; p.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; p.x_scale_block = a.x_scale_block; p.zero_tail = a.zero_tail;
-  if (pieces_whole(p, a.op, a.x_dtype)) return grouped_tile_launch(p, a.op, a.x_dtype, stream);
+  if (pieces_whole(p, a.op, a.x_dtype)) {
+    const long long mean = a.rows / a.experts;                   // rows of an expert, as far as the host knows
+    if (a.op == kRows && mean < 32) return grouped_stream_launch(p, a.x_dtype, mean < 6 ? 1 : mean < 14 ? 2 : 4, stream);
+    // (float32 results of e4m3 operands stay with the general kernel, whose products are exact)
+    if (!(fp8 && a.y_dtype == CPPMEGA_MI355_F32)) return grouped_tile_launch(p, a.op, a.x_dtype, stream);
+  }
   return grouped_general_launch(p, a.op, a.x_dtype, stream);
 }
 

@@ -22,7 +22,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "../../include/cppmega_mi355.h"
+#include "../../include/cppmega_mi355_layer.h"
 
 namespace {
 
@@ -663,6 +663,174 @@ PyObject* indexer_loss(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   return wrap(fresh);
 }
 
+// ---- RMS norm, products grouped by expert --------------------------------------------------------
+PyObject* tuple_of(std::initializer_list<Tensor> parts) {
+  PyObject* result = PyTuple_New((Py_ssize_t)parts.size());
+  if (!result) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& t : parts) PyTuple_SET_ITEM(result, i++, wrap(t));
+  return result;
+}
+// Whether t is a norm's weight for rows like x; x has rows.
+bool norm_operands(const Place& at, const Tensor& x, const Tensor& weight) {
+  const auto type = x.scalar_type(), wt = weight.scalar_type();
+  if (!is_float(type) || x.dim() < 1 || x.numel() < 1 || !at.dense(x) || !at.dense(weight)) return false;
+  return (wt == type || wt == ScalarType::Float) && has_shape(weight, {x.size(-1)}) && x.size(-1) <= CPPMEGA_MI355_NORM_MAX_WIDTH && fits_int(x.numel() / x.size(-1));
+}
+bool like(const Place& at, const Tensor& t, const Tensor& x) { return at.dense(t) && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes(); }
+
+// rms_norm(x, weight, residual or None, eps, e4m3, scale_block, pow2_scales) -> (out[, scale][, sum]) or None; e4m3: codes and scales
+PyObject* rms_norm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 7) DECLINE;
+  const Tensor *x = tensor(arg[0]), *weight = tensor(arg[1]), *residual = tensor(arg[2]);
+  if (!x || !weight || (!residual && arg[2] != Py_None) || !PyFloat_CheckExact(arg[3]) || !PyLong_CheckExact(arg[5])) DECLINE;
+  const long long block = as_int(arg[5]);
+  const bool fp8 = arg[4] == Py_True;
+  Place at;
+  if (!at.take(*x) || !norm_operands(at, *x, *weight) || (residual && !like(at, *residual, *x)) || (fp8 && block != 0 && block != 128)) {
+    PyErr_Clear();
+    DECLINE;
+  }
+  const int64_t width = x->size(-1), rows = x->numel() / width;
+  cppmega_mi355_rms_norm_args_t a;
+  memset(&a, 0, sizeof(a));
+  a.struct_size = sizeof(a);
+  a.x_dtype = code(x->scalar_type());
+  a.weight_dtype = code(weight->scalar_type());
+  a.out_dtype = fp8 ? CPPMEGA_MI355_E4M3 : a.x_dtype;
+  a.x = x->data_ptr(); a.weight = weight->data_ptr();
+  a.rows = rows; a.width = (int32_t)width; a.eps = (float)PyFloat_AS_DOUBLE(arg[3]);
+  a.x_pitch = a.residual_pitch = a.out_pitch = a.residual_out_pitch = width;
+  a.scale_block = (int32_t)block;
+  a.pow2_scales = arg[6] == Py_True;
+  Tensor out = at::empty(x->sizes(), fp8 ? x->options().dtype(at::kByte) : x->options()), scale, sum;
+  a.out = out.data_ptr();
+  if (fp8) {
+    std::vector<int64_t> shape(x->sizes().begin(), x->sizes().end() - 1);
+    if (block) shape.push_back((width + 127) / 128);
+    scale = at::empty(shape, x->options().dtype(at::kFloat));
+    a.scale = (float*)scale.data_ptr();
+  }
+  if (residual) {
+    sum = at::empty(x->sizes(), x->options());
+    a.residual = residual->data_ptr();
+    a.residual_out = sum.data_ptr();
+  }
+  if (unlocked([&] { return cppmega_mi355_rms_norm(&a, sizeof(a), at.stream); })) DECLINE;
+  if (!fp8) return residual ? tuple_of({out, sum}) : wrap(out);
+  return residual ? tuple_of({out, scale, sum}) : tuple_of({out, scale});
+}
+
+// rms_norm_bwd(dy, h, weight, eps, dh or None) -> (dx, dweight) or None
+PyObject* rms_norm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 5) DECLINE;
+  const Tensor *dy = tensor(arg[0]), *h = tensor(arg[1]), *weight = tensor(arg[2]), *dh = tensor(arg[4]);
+  if (!dy || !h || !weight || (!dh && arg[4] != Py_None) || !PyFloat_CheckExact(arg[3])) DECLINE;
+  Place at;
+  if (!at.take(*h) || !norm_operands(at, *h, *weight) || !like(at, *dy, *h) || (dh && !like(at, *dh, *h))) DECLINE;
+  const int64_t width = h->size(-1);
+  cppmega_mi355_rms_norm_bwd_args_t a;
+  memset(&a, 0, sizeof(a));
+  a.struct_size = sizeof(a);
+  a.dtype = code(h->scalar_type());
+  a.weight_dtype = code(weight->scalar_type());
+  a.dy = dy->data_ptr(); a.h = h->data_ptr(); a.weight = weight->data_ptr();
+  if (dh) a.dh = dh->data_ptr();
+  a.rows = h->numel() / width; a.width = (int32_t)width; a.eps = (float)PyFloat_AS_DOUBLE(arg[3]);
+  a.dy_pitch = a.h_pitch = a.dh_pitch = a.dx_pitch = width;
+  size_t bytes = 0;
+  if (cppmega_mi355_rms_norm_bwd_workspace_bytes(&a, sizeof(a), &bytes)) DECLINE;
+  Tensor scratch = workspace(at.device, at.stream, bytes);
+  a.workspace = scratch.data_ptr();
+  a.workspace_bytes = (size_t)scratch.numel();
+  Tensor dx = at::empty(h->sizes(), h->options()), dweight = at::empty({width}, h->options().dtype(at::kFloat));
+  a.dx = dx.data_ptr();
+  a.dweight = (float*)dweight.data_ptr();
+  if (unlocked([&] { return cppmega_mi355_rms_norm_bwd(&a, sizeof(a), at.stream); })) DECLINE;
+  return tuple_of({dx, dweight});
+}
+
+// The operands that all grouped products share: rows [T, ..], w [E, N, K], offsets [E + 1]; false: not the plain case.
+bool grouped_operands(const Place& at, const Tensor& rows, const Tensor& w, const Tensor& offsets, cppmega_mi355_grouped_gemm_args_t& a) {
+  if (rows.dim() != 2 || w.dim() != 3 || !at.dense(rows) || !at.dense(w) || !at.dense(offsets) || rows.scalar_type() != w.scalar_type()) return false;
+  if (!is_index(offsets.scalar_type()) || !has_shape(offsets, {w.size(0) + 1}) || rows.size(0) < 1) return false;
+  for (int64_t x : {rows.size(0), w.size(0), w.size(1), w.size(2)})
+    if (!fits_int(x)) return false;
+  memset(&a, 0, sizeof(a));
+  a.struct_size = sizeof(a);
+  a.x_dtype = a.y_dtype = code(w.scalar_type());
+  a.offsets_dtype = code(offsets.scalar_type());
+  a.offsets = offsets.data_ptr();
+  a.rows = rows.size(0);
+  a.experts = (int32_t)w.size(0); a.n = (int32_t)w.size(1); a.k = (int32_t)w.size(2);
+  a.w = w.data_ptr();
+  a.zero_tail = 1;
+  return true;
+}
+bool is_half(const Tensor& t) { return t.scalar_type() == ScalarType::Half || t.scalar_type() == ScalarType::BFloat16; }
+
+// grouped_gemm(x, w, offsets) -> y or None
+PyObject* grouped_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 3) DECLINE;
+  const Tensor *x = tensor(arg[0]), *w = tensor(arg[1]), *offsets = tensor(arg[2]);
+  Place at;
+  cppmega_mi355_grouped_gemm_args_t a;
+  if (!x || !w || !offsets || !at.take(*x) || !is_half(*x) || !grouped_operands(at, *x, *w, *offsets, a) || x->size(1) != a.k) DECLINE;
+  Tensor y = at::empty({a.rows, a.n}, x->options());
+  a.op = CPPMEGA_MI355_GROUPED_ROWS;
+  a.x = x->data_ptr(); a.y = y.data_ptr();
+  a.x_pitch = a.k; a.y_pitch = a.n;
+  if (unlocked([&] { return cppmega_mi355_grouped_gemm(&a, sizeof(a), at.stream); })) DECLINE;
+  return wrap(y);
+}
+
+// grouped_gemm_bwd(dy, x, w, offsets) -> (dx, dw) or None
+PyObject* grouped_gemm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 4) DECLINE;
+  const Tensor *dy = tensor(arg[0]), *x = tensor(arg[1]), *w = tensor(arg[2]), *offsets = tensor(arg[3]);
+  Place at;
+  cppmega_mi355_grouped_gemm_args_t a;
+  if (!dy || !x || !w || !offsets || !at.take(*dy) || !is_half(*dy) || !grouped_operands(at, *dy, *w, *offsets, a) || dy->size(1) != a.n) DECLINE;
+  if (!at.dense(*x) || x->scalar_type() != dy->scalar_type() || !has_shape(*x, {a.rows, a.k})) DECLINE;
+  Tensor dx = at::empty({a.rows, a.k}, x->options()), dw = at::empty(w->sizes(), w->options());
+  a.op = CPPMEGA_MI355_GROUPED_ROWS_GRAD;
+  a.x = dy->data_ptr(); a.y = dx.data_ptr();
+  a.x_pitch = a.n; a.y_pitch = a.k;
+  cppmega_mi355_grouped_gemm_args_t b = a;
+  b.op = CPPMEGA_MI355_GROUPED_WEIGHTS_GRAD;
+  b.w = x->data_ptr(); b.y = dw.data_ptr();
+  b.w_pitch = a.k;
+  if (unlocked([&] {
+        const int rc = cppmega_mi355_grouped_gemm(&a, sizeof(a), at.stream);
+        return rc ? rc : cppmega_mi355_grouped_gemm(&b, sizeof(b), at.stream);
+      }))
+    DECLINE;
+  return tuple_of({dx, dw});
+}
+
+// grouped_fp8_gemm(x, x_scale, w, w_scale, offsets) -> y (bfloat16) or None
+PyObject* grouped_fp8_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 5) DECLINE;
+  const Tensor *x = tensor(arg[0]), *xs = tensor(arg[1]), *w = tensor(arg[2]), *ws = tensor(arg[3]), *offsets = tensor(arg[4]);
+  Place at;
+  cppmega_mi355_grouped_gemm_args_t a;
+  if (!x || !xs || !w || !ws || !offsets || !at.take(*x) || x->scalar_type() != ScalarType::Byte || !grouped_operands(at, *x, *w, *offsets, a) || x->size(1) != a.k) DECLINE;
+  const int64_t blocks_n = ((int64_t)a.n + 127) / 128, blocks_k = ((int64_t)a.k + 127) / 128;
+  for (const Tensor* t : {xs, ws})
+    if (!at.dense(*t) || t->scalar_type() != ScalarType::Float) DECLINE;
+  if (has_shape(*xs, {a.rows, blocks_k})) a.x_scale_block = 128;
+  else if (!has_shape(*xs, {a.rows})) DECLINE;
+  if (!has_shape(*ws, {a.experts, blocks_n, blocks_k})) DECLINE;
+  Tensor y = at::empty({a.rows, a.n}, x->options().dtype(at::kBFloat16));
+  a.op = CPPMEGA_MI355_GROUPED_ROWS;
+  a.y_dtype = CPPMEGA_MI355_BF16;
+  a.x = x->data_ptr(); a.y = y.data_ptr();
+  a.x_scale = (const float*)xs->data_ptr(); a.w_scale = (const float*)ws->data_ptr();
+  a.x_pitch = a.k; a.y_pitch = a.n;
+  if (unlocked([&] { return cppmega_mi355_grouped_gemm(&a, sizeof(a), at.stream); })) DECLINE;
+  return wrap(y);
+}
+
 // ---- workspace of the Python launch helpers, release ---------------------------------------------
 // workspace(device, bytes, stream) -> tensor
 PyObject* workspace_of(PyObject*, PyObject* const* arg, Py_ssize_t n) {
@@ -694,6 +862,8 @@ PyMethodDef methods[] = {
     CALL("fused_gemm", fused_gemm),     CALL("vecmat", vecmat),     CALL("head_gemm", head_gemm),
     CALL("absorb_query", absorb_query), CALL("cache_append", cache_append), CALL("workspace", workspace_of),
     CALL("mla_backward", mla_backward), CALL("indexer_loss", indexer_loss),
+    CALL("rms_norm", rms_norm),         CALL("rms_norm_bwd", rms_norm_bwd), CALL("grouped_gemm", grouped_gemm),
+    CALL("grouped_gemm_bwd", grouped_gemm_bwd), CALL("grouped_fp8_gemm", grouped_fp8_gemm),
     {"release_workspaces", release_workspaces, METH_NOARGS, "Give the kept scratch tensors back to torch's allocator."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Launch path of the per-step calls.", -1, methods};

@@ -34,6 +34,10 @@ def _shape3(w: torch.Tensor, name: str) -> tuple[int, int, int]:
 
 def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """y [T, N] in x's type (a caller-owned ``out`` may be float32)."""
+    if out is None:
+        done = ops.host.grouped_gemm(x, w, offsets)
+        if done is not None:
+            return done
     fresh = out is None
     if fresh:
         out = torch.empty((x.shape[0], _shape3(w, "w")[1]), dtype=x.dtype, device=x.device)
@@ -43,6 +47,10 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
 def grouped_gemm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, dx: torch.Tensor | None = None,
                      dw: torch.Tensor | None = None, need_dx: bool = True, need_dw: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """``(dx [T, K], dw [E, N, K])`` in the operands' type (caller-owned ones may be float32); one that is not needed is None."""
+    if dx is None and dw is None and need_dx and need_dw:
+        done = ops.host.grouped_gemm_bwd(dy, x, w, offsets)
+        if done is not None:
+            return done
     E, N, K = _shape3(w, "w")
     if dy.ndim != 2 or x.ndim != 2 or tuple(dy.shape) != (x.shape[0], N) or x.shape[1] != K:
         raise ValueError(f"grouped_gemm_bwd shape mismatch: dy {tuple(dy.shape)}, x {tuple(x.shape)}, w {tuple(w.shape)}")
@@ -68,6 +76,10 @@ def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_
 
     ``x`` uint8 e4m3 [T, K] with float32 ``x_scale`` [T] or [T, ceil(K / 128)] (what ``rms_norm_fp8`` writes); ``w`` uint8 e4m3
     [E, N, K] with float32 ``w_scale`` [E, ceil(N / 128), ceil(K / 128)]."""
+    if out is None:
+        done = ops.host.grouped_fp8_gemm(x, x_scale, w, w_scale, offsets)
+        if done is not None:
+            return done
     fresh = out is None
     if fresh:
         out = torch.empty((x.shape[0], _shape3(w, "w")[1]), dtype=torch.bfloat16, device=x.device)

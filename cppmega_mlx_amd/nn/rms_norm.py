@@ -27,6 +27,10 @@ __all__ = ["rms_norm", "rms_norm_apply", "rms_norm_bwd", "rms_norm_fp8"]
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residual: torch.Tensor | None = None,
              out: torch.Tensor | None = None, residual_out: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
     """``y``, or ``(y, h)`` with a residual."""
+    if out is None and residual_out is None:
+        done = ops.host.rms_norm(x, weight, residual, eps, False, 0, False)
+        if done is not None:
+            return done
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if residual is not None and residual_out is None:
@@ -39,6 +43,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, re
                  pow2_scales: bool = False, codes: torch.Tensor | None = None, scale: torch.Tensor | None = None,
                  residual_out: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
     """``(codes, scale)``, or ``(codes, scale, h)`` with a residual."""
+    if codes is None and scale is None and residual_out is None:
+        done = ops.host.rms_norm(x, weight, residual, eps, True, scale_block, bool(pow2_scales))
+        if done is not None:
+            return done
     if codes is None:
         codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
     if scale is None:
@@ -57,6 +65,10 @@ def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *, eps
                  dx: torch.Tensor | None = None, dweight: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(dx, dweight)`` for the rows ``h`` that were normalised: ``dx`` (in h's type; of x and of the residual alike) includes
     ``dh``, the gradient that reaches the stream past the norm; ``dweight`` is float32, added in the same order on every run."""
+    if dx is None and dweight is None:
+        done = ops.host.rms_norm_bwd(dy, h, weight, eps, dh)
+        if done is not None:
+            return done
     if dx is None:
         dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     if dweight is None:

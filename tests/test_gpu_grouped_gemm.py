@@ -299,6 +299,27 @@ def test_streams_of_their_own(device):
     assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(got))
 
 
+def test_native_launch_path_and_helpers_agree(device, monkeypatch):
+    n, k, rows, e = 136, 192, 150, 5
+    x, w, dy = _normal(device, rows, k, dtype=F16), _normal(device, e, n, k, dtype=F16), _normal(device, rows, n, dtype=F16)
+    x8, w8, ws, xs = _e4m3(device, rows, k, seed=1), _e4m3(device, e, n, k, seed=2), _normal(device, e, 2, 2).exp(), _normal(device, rows, 2).exp()
+    off = _offsets([50, 0, 60, 1, 30], device)
+    host = ops.host
+    assert host.grouped_gemm(x[:, :184], w, off) is None and host.grouped_gemm(x, w.bfloat16(), off) is None and host.grouped_gemm(x, w, off[:5]) is None
+    assert host.grouped_gemm_bwd(dy[:9], x, w, off) is None and host.grouped_fp8_gemm(x8, xs[:9], w8, ws, off) is None and host.grouped_fp8_gemm(x8, xs, w8, ws[:1], off) is None
+    calls = [lambda: (grouped_gemm(x, w, off),), lambda: grouped_gemm_bwd(dy, x, w, off.long()), lambda: (grouped_fp8_gemm(x8, xs, w8, ws, off),),
+             lambda: (grouped_fp8_gemm(x8, xs[:, 0].contiguous(), w8, ws, off),)]
+    native = [c() for c in calls]
+
+    class Declines:
+        def __getattr__(self, name):
+            return getattr(host, name) if "workspace" in name else (lambda *args: None)
+
+    monkeypatch.setattr(ops, "host", Declines())
+    for a, b in zip(native, [c() for c in calls]):
+        assert len(a) == len(b) and all(s.shape == t.shape and s.dtype == t.dtype and torch.equal(s, t) for s, t in zip(a, b))
+
+
 def test_refusals(device):
     x, w, off = torch.zeros(8, 32, dtype=BF16, device=device), torch.zeros(2, 16, 32, dtype=BF16, device=device), _offsets([4, 4], device)
     x8, w8, xs, ws = x.to(torch.uint8), w.to(torch.uint8), torch.ones(8, device=device), torch.ones(2, 1, 1, device=device)

@@ -8,7 +8,7 @@ the sums of magnitudes."""
 import pytest
 import torch
 
-from cppmega_mlx_amd import _lib
+from cppmega_mlx_amd import _lib, ops
 from cppmega_mlx_amd.nn.rms_norm import rms_norm, rms_norm_apply, rms_norm_bwd, rms_norm_fp8
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +287,23 @@ def test_refusals(device):
         with pytest.raises(error):
             call()
             print("not refused:", i)
+
+
+def test_native_launch_path_and_helpers_agree(device, monkeypatch):
+    x, w, r = _inputs(device, 6, 320, BF16, seed=160)
+    g = _normal(device, 6, 320, dtype=BF16, seed=170)
+    host = ops.host
+    assert host.rms_norm(x[:, :300], w[:300].contiguous(), None, 1e-6, False, 0, False) is None and host.rms_norm(x, w, None, -1.0, False, 0, False) is None
+    assert host.rms_norm(x, w.half(), None, 1e-6, False, 0, False) is None and host.rms_norm(x, w, None, 1e-6, True, 64, False) is None
+    assert host.rms_norm_bwd(g[:, :319], x, w, 1e-6, None) is None and host.rms_norm_bwd(g, x, w, 1e-6, g.float()) is None
+    calls = [lambda: (rms_norm(x, w),), lambda: rms_norm(x.view(2, 3, 320), w, residual=r.view(2, 3, 320)), lambda: rms_norm_fp8(x, w, scale_block=128, pow2_scales=True),
+             lambda: rms_norm_fp8(x.view(2, 3, 320), w, residual=r.view(2, 3, 320)), lambda: rms_norm_bwd(g, x, w), lambda: rms_norm_bwd(g, x, w, dh=r)]
+    native = [c() for c in calls]
+
+    class Declines:
+        def __getattr__(self, name):
+            return getattr(host, name) if "workspace" in name else (lambda *args: None)
+
+    monkeypatch.setattr(ops, "host", Declines())
+    for a, b in zip(native, [c() for c in calls]):
+        assert len(a) == len(b) and all(s.shape == t.shape and s.dtype == t.dtype and torch.equal(s, t) for s, t in zip(a, b))
