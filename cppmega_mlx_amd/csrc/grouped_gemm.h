@@ -71,7 +71,7 @@ __device__ __forceinline__ int expert_of_tile(const GroupedParams& p, const int*
 }
 
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
-int grouped_tile_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
-int grouped_stream_launch(const GroupedParams& p, int dtype, int tm, hipStream_t stream);
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream);
+int grouped_stream_launch(const GroupedParams& p, int dtype, hipStream_t stream);
 
 }  // namespace cm

@@ -15,6 +15,21 @@ bool pieces_whole(const GroupedParams& p, int op, int dtype) {
   return op != kWeightsGrad || (p.w_pitch % piece == 0 && p.w_pitch <= (1 << 22));
 }
 
+// 256 x 256 tiles, one to a CU, or 128 x 128, two to a CU: by the expected rounds of tiles over 256 CUs (half a tile of rows of each expert is
+// padding, half a round is idle at the end).  Two low tiles side by side take 0.68 of a high one's time for half its products.  Measured, us high /
+// low, rows x experts x n x k: 16384 x 32 x 4096 x 2048 324 / 371 (bf16), 4096 x 1 x 4096 x 4096 116 / 131, 8192 x 64 x 2048 x 2048 187 / 174,
+// 6144 x 16 x 2048 x 2048 96 / 83, 1024 x 1 x 4096 x 4096 82 / 48.  Gradients of weights have as many tiles whatever the rows; few rows leave
+// them short, and two workgroups cover each other's stores: 4096 rows of 32 experts 233 / 224 (with the rows' gradient), of 8 121 / 134.
+bool high_tiles(const GroupedParams& p, int op) {
+  if (op == kWeightsGrad) return p.rows >= 192ll * p.experts;
+  const int cols = op == kRows ? p.n : p.k;
+  auto rounds = [&](int b, int at_once) {
+    const double tiles = ((double)p.rows / b + 0.5 * p.experts) * ((cols + b - 1) / b) / at_once;
+    return tiles > 0.5 ? tiles + 0.5 : 1.0;
+  };
+  return rounds(256, 256) <= 0.68 * rounds(128, 512);
+}
+
 }  // namespace
 
 int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
@@ -42,10 +57,13 @@ int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t 
   p.experts = a.experts; p.n = a.n; p.k = a.k;
   p.y_dtype = a.y_dtype; p.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; p.x_scale_block = a.x_scale_block; p.zero_tail = a.zero_tail;
   if (pieces_whole(p, a.op, a.x_dtype)) {
-    const long long mean = a.rows / a.experts;                   // rows of an expert, as far as the host knows
-    if (a.op == kRows && mean < 32) return grouped_stream_launch(p, a.x_dtype, mean < 6 ? 1 : mean < 14 ? 2 : 4, stream);
+    // Few rows to an expert: the kernel that streams the weights.  Measured against tiles, us, 64 experts of 2048 x 2048: 8 rows each 102 / 130
+    // (bf16) and 56 / 60 (e4m3), 12 rows 104 / 130 and 61 / 60, 16 rows 117 / 130 and 69 / 59, 24 rows 152 / 132 and 88 / 61.  (For float32
+    // results of e4m3 operands there is the general kernel instead of tiles, which takes three times as long.)
+    const bool exact = fp8 && a.y_dtype == CPPMEGA_MI355_F32;
+    if (a.op == kRows && a.rows < (fp8 && !exact ? 12ll : 20ll) * a.experts) return grouped_stream_launch(p, a.x_dtype, stream);
     // (float32 results of e4m3 operands stay with the general kernel, whose products are exact)
-    if (!(fp8 && a.y_dtype == CPPMEGA_MI355_F32)) return grouped_tile_launch(p, a.op, a.x_dtype, stream);
+    if (!exact) return grouped_tile_launch(p, a.op, a.x_dtype, high_tiles(p, a.op), stream);
   }
   return grouped_general_launch(p, a.op, a.x_dtype, stream);
 }

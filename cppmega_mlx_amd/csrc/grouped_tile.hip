@@ -18,24 +18,26 @@ namespace {
 
 __device__ __align__(64) const unsigned char zeros[64] = {};
 
-template <int OP, int DT>
+// HIGH: 256 x 256 tiles, eight wavefronts of 128 x 64.  Otherwise 128 x 128, four of 64 x 64, two workgroups to a CU.
+template <int OP, int DT, bool HIGH>
 struct Shape {
   static constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
   static constexpr bool TR = OP == kWeightsGrad, TQ = OP != kRows;      // the contraction is the operand's slow axis
+  static constexpr int BM = HIGH ? 256 : 128, BN = BM, WN = HIGH ? 4 : 2, kWaves = 2 * WN;
+  static constexpr int kHeight = BM / 2, kWidth = BN / WN;              // of a wavefront
   // bytes of contraction in a stage, and how many stages of each operand LDS holds
-  static constexpr int KB = FP8 || !TQ ? 128 : 64, RS = FP8 ? 2 : TQ ? 5 : 3, QS = FP8 ? 2 : TQ ? 5 : 2;
+  static constexpr int KB = FP8 || !TQ ? 128 : 64, RS = FP8 || !HIGH ? (KB == 64 ? 4 : 2) : TQ ? 5 : 3, QS = FP8 || !HIGH ? RS : TQ ? 5 : 2;
   static constexpr int BYTES = FP8 ? 1 : 2, STEP = KB / BYTES;
-  static constexpr int BM = 256, BN = 256, WN = 4;
-  static constexpr int RL = BM * KB / 8192, QL = BN * KB / 8192, L = RL + QL + (FP8 ? 1 : 0);   // load instructions per wavefront and stage
-  static constexpr int kR = BM * KB, kQ = BN * KB, kS = FP8 ? 8 * 256 : 0;
+  static constexpr int RL = BM * KB / 1024 / kWaves, QL = BN * KB / 1024 / kWaves, L = RL + QL + (FP8 ? 1 : 0);   // load instructions per wavefront and stage
+  static constexpr int kR = BM * KB, kQ = BN * KB, kS = FP8 ? kWaves * 256 : 0;
   static constexpr int kQat = RS * kR, kSat = kQat + QS * kQ, kLds = kSat + QS * kS;            // where columns and scales begin
   // the place of piece c of a row among its row's pieces is c ^ fold(row): sixteen rows with one piece lie in different banks
   static __device__ __forceinline__ int fold(int row) { return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 };
 
-template <int OP, int DT>
-__global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParams p) {
-  typedef Shape<OP, DT> S;
+template <int OP, int DT, bool HIGH>
+__global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
+  typedef Shape<OP, DT, HIGH> S;
   constexpr bool FP8 = S::FP8, F16 = S::F16, TR = S::TR, TQ = S::TQ;
   constexpr int BYTES = S::BYTES, STEP = S::STEP, BM = S::BM, BN = S::BN, RS = S::RS, QS = S::QS, RL = S::RL, QL = S::QL, L = S::L, KB = S::KB;
   __shared__ u32x4 smem[S::kLds / 16];
@@ -43,7 +45,7 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
   int* const starts = reinterpret_cast<int*>(smem);
   char* const lds = reinterpret_cast<char*>(smem);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (wave / S::WN) * 128, wn = (wave % S::WN) * 64;
+  const int wm = (wave / S::WN) * S::kHeight, wn = (wave % S::WN) * S::kWidth;
 
   // ---- which tile: every XCD takes one run of the order, which goes through the experts; of each, up to four row tiles share the
   // columns that pass, so that an expert's weight leaves memory once (groups of four rows of tiles whatever their experts: 5 % slower) ----
@@ -87,11 +89,11 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
       const int row = u * (64 / PIECES) + lane / PIECES, c = (lane % PIECES) ^ S::fold(row);
       return (unsigned)((row < limit ? row : limit - 1) * pitch * BYTES) + (unsigned)c * 16u;
     }
-    const int step = u * 2 + (lane >> 5), c = (lane & 31) ^ ((step & 3) << 2);
+    const int step = u * (512 / BM) + lane / (BM / 8), c = (lane % (BM / 8)) ^ ((step & 3) << 2);
     return (unsigned)(step * pitch * BYTES) + (unsigned)(c * 8 < limit ? c : (limit - 1) >> 3) * 16u;
   };
   auto along = [&](bool transposed, int u) {
-    return transposed ? u * 2 + (lane >> 5) : ((lane % PIECES) ^ S::fold(u * (64 / PIECES) + lane / PIECES)) * (16 / BYTES);
+    return transposed ? u * (512 / BM) + lane / (BM / 8) : ((lane % PIECES) ^ S::fold(u * (64 / PIECES) + lane / PIECES)) * (16 / BYTES);
   };
 #pragma unroll
   for (int i = 0; i < RL; ++i) xoff[i] = piece_of(TR, wave * RL + i, rows_here, p.x_pitch);
@@ -100,15 +102,15 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
   const char* sb = nullptr;
   unsigned s_step = 0;
   if constexpr (FP8) {
-    // the first four wavefronts bring the scales of 64 rows each, the others those of the columns' two blocks
+    // half of the wavefronts bring the scales of 64 rows each, the others those of the columns' blocks
     const int blocks_k = (p.k + 127) / 128, blocks_n = (p.n + 127) / 128;
-    if (wave < 4) {
+    if (wave < BM / 64) {
       const int row = wave * 64 + lane;
       sb = (const char*)(p.x_scale + (size_t)(lo + m0) * (p.x_scale_block ? blocks_k : 1));
       soff = (unsigned)(row < rows_here ? row : rows_here - 1) * (p.x_scale_block ? (unsigned)blocks_k * 4u : 4u);
       s_step = p.x_scale_block ? 4u : 0u;
     } else {
-      const int b = n0 / 128 + (lane & 1);
+      const int b = n0 / 128 + (BN > 128 ? lane & 1 : 0);
       sb = (const char*)(p.w_scale + (size_t)(e < p.experts ? e : 0) * blocks_n * blocks_k);
       soff = (unsigned)(b < blocks_n ? b : blocks_n - 1) * (unsigned)blocks_k * 4u;
       s_step = 4u;
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
   };
 
   if constexpr (!FP8) {
-    constexpr int TI = 4, TJ = 2;                               // 32 x 32 tiles of the wavefront
+    constexpr int TI = S::kHeight / 32, TJ = S::kWidth / 32;        // 32 x 32 tiles of the wavefront
     const int l32 = lane & 31, half = lane >> 5, l16 = lane & 15;
     constexpr int KS = KB / 32;                                 // 16 steps of contraction at a time
     int rat[TR ? TI : KS], qat[TQ ? TJ : KS];                     // where a lane reads: per tile (transposing), or per 16 steps
@@ -334,11 +336,11 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
           }
     }
   } else {
-    constexpr int TI = 8, TJ = 4;                               // 16 x 16 tiles of the wavefront, a whole 128-channel block an instruction
+    constexpr int TI = S::kHeight / 16, TJ = S::kWidth / 16;        // 16 x 16 tiles of the wavefront, a whole 128-channel block an instruction
     const int l16 = lane & 15, quad = lane >> 4, f = (l16 >> 1) & 7;
     const int rat[2] = {(wm + l16) * 128 + (quad ^ f) * 16, (wm + l16) * 128 + ((quad + 4) ^ f) * 16};
     const int qat[2] = {(wn + l16) * 128 + (quad ^ f) * 16, (wn + l16) * 128 + ((quad + 4) ^ f) * 16};
-    const int xsat = (wm + l16) * 4, wsat = 4 * 256 + (wn >> 7) * 4;
+    const int xsat = (wm + l16) * 4, wsat = BM / 64 * 256 + (wn >> 7) * 4;
     auto operand = [&](int a, int b) -> i32x8 {
       const u32x4 x = *reinterpret_cast<const u32x4*>(lds + a), y = *reinterpret_cast<const u32x4*>(lds + b);
       i32x8 o;
@@ -377,7 +379,7 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
         for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, t[i & 1][j][v], acc[i][j][v]);
     };
     // all rows but the last ones; load instructions from .. between them, PER to a group of products
-    constexpr int PER = 2;
+    constexpr int PER = (L + TI - 1) / TI;
     auto products = [&](auto more, int from) {
 #pragma unroll
       for (int i = 0; i < TI - 1; ++i) {
@@ -456,12 +458,17 @@ __global__ __launch_bounds__(512, 2) void grouped_tile_kernel(const GroupedParam
 
 }  // namespace
 
-int grouped_tile_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream) {
-  const long long tiles_n = ((op == kRows ? p.n : p.k) + 255) / 256;
-  const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + 255) / 256) : p.rows / 256 + p.experts + 1;
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream) {
+  const int b = high ? 256 : 128;
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b;
+  const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + b - 1) / b) : p.rows / b + p.experts + 1;
   if (tiles_m * tiles_n > 0x3fffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles_m * tiles_n);
-  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), block(512);
-#define CM_TILE(op_, dt) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt>), grid, block, 0, stream, p)
+  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), block(high ? 512 : 256);
+#define CM_TILE(op_, dt)                                                                              \
+  do {                                                                                                \
+    if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true>), grid, block, 0, stream, p);    \
+    else hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, false>), grid, block, 0, stream, p);        \
+  } while (0)
 #define CM_TILE_OP(op_)                                           \
   do {                                                            \
     if (dtype == CPPMEGA_MI355_F16) CM_TILE(op_, CPPMEGA_MI355_F16); \
