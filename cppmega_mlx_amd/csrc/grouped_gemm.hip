@@ -16,9 +16,9 @@ bool pieces_whole(const GroupedParams& p, int op, int dtype) {
 }
 
 // 256 x 256 tiles, one to a CU, or 128 x 128, two to a CU: by the expected rounds of tiles over 256 CUs (half a tile of rows of each expert is
-// padding, half a round is idle at the end).  Two low tiles side by side take 0.68 of a high one's time for half its products.  Measured, us high /
+// padding, half a round is idle at the end).  Two low tiles side by side take 0.64 of a high one's time for half its products.  Measured, us high /
 // low, rows x experts x n x k: 16384 x 32 x 4096 x 2048 324 / 371 (bf16), 4096 x 1 x 4096 x 4096 116 / 131, 8192 x 64 x 2048 x 2048 187 / 174,
-// 6144 x 16 x 2048 x 2048 96 / 83, 1024 x 1 x 4096 x 4096 82 / 48.  Gradients of weights have as many tiles whatever the rows; few rows leave
+// 6144 x 16 x 2048 x 2048 96 / 82, 1024 x 1 x 4096 x 4096 82 / 48.  Gradients of weights have as many tiles whatever the rows; few rows leave
 // them short, and two workgroups cover each other's stores: 4096 rows of 32 experts 233 / 224 (with the rows' gradient), of 8 121 / 134.
 bool high_tiles(const GroupedParams& p, int op) {
   if (op == kWeightsGrad) return p.rows >= 192ll * p.experts;
@@ -27,7 +27,7 @@ bool high_tiles(const GroupedParams& p, int op) {
     const double tiles = ((double)p.rows / b + 0.5 * p.experts) * ((cols + b - 1) / b) / at_once;
     return tiles > 0.5 ? tiles + 0.5 : 1.0;
   };
-  return rounds(256, 256) <= 0.68 * rounds(128, 512);
+  return rounds(256, 256) <= 0.64 * rounds(128, 512);
 }
 
 }  // namespace

@@ -1,13 +1,25 @@
-// Products grouped by expert for many rows (gfx950): 256 x 256 tiles, operands by the load unit into LDS.
+// Products grouped by expert for many rows (gfx950): 256 x 256 and 128 x 128 tiles, operands by the load unit into LDS.
 //
 // Needs rows that begin on 16 bytes and a contraction (and, where it is the slow axis, columns) in whole 16-byte pieces.
 //
-// Eight wavefronts, 128 x 64 of the tile each, two on every SIMD; a stage is 128 bytes of contraction of both operands (64 KB, two
-// stages in LDS).  Rows that are not there repeat the last one and are not stored; contraction that is not there comes from a piece of
-// zeros, for both operands (what lies behind a row may be NaN).  A wavefront whose rows are not there only loads.
+// LDS holds rings of stages of both operands, 128 or 64 bytes of contraction each, filled by global_load_lds as far ahead as there is room;
+// two wavefronts on a SIMD, one barrier a stage, behind which the next stage's first operands are read under this one's last products.
+// Rows that are not there repeat the last one and are not stored; contraction that is not there comes from a piece of zeros, for both
+// operands (what lies behind a row may be NaN).  A wavefront whose rows are not there only loads.  16-bit products by 32 x 32 x 16
+// instructions; e4m3 by 16 x 16 x 128, a scale block each, whose sums are scaled and added while the matrix unit is at the next ones (that
+// instruction aligns eight products to the largest and drops what lies below 2^-13 of it: results of 16 bits do not show it).
 // Pieces are 16 bytes; in LDS
-//   contraction contiguous: [row][8 pieces], piece c of row r in place c ^ (r / 2 % 8);
-//   contraction slow: [step of 64][32 pieces of 8 channels], piece c of step s in place c ^ 4 (s % 4), read by the transposing load.
+//   contraction contiguous: [row][pieces], piece c of row r in place c ^ fold(r);
+//   contraction slow: [step][pieces of 8 channels], piece c of step s in place c ^ 4 (s % 4), read by the transposing load.
+// (No bank conflicts in either: counted.)
+//
+// Measured, us (TFLOP/s): 16384 rows of 32 experts, 4096 x 2048 bf16 315 (870); of one expert 248 (1110), and 4096 x 8192 833 (1320), where a library's
+// product of that size reaches 1390: at 1.3 PFLOP/s the clock is down at 1.7 GHz, power is the bound, and neither deeper rings nor other orders
+// of loads change it.  e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 515 (2130): products 2048 of 4000 clocks a stage, the scaling's vector
+// instructions 1000 and the operand reads 1900 beside them.  What short contractions lose: 10 to 12 us a tile for its first loads and for stores that all
+// CUs send at once; persistent workgroups with the next tile's first stages under the stores were not faster, and tiles of few rows after all
+// others 5 % slower (the weights are read twice).
+// Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16: 400 (690); the rows' 320 tiles take two rounds of 256 CUs.
 
 #include <type_traits>
 
@@ -18,15 +30,18 @@ namespace {
 
 __device__ __align__(64) const unsigned char zeros[64] = {};
 
-// HIGH: 256 x 256 tiles, eight wavefronts of 128 x 64.  Otherwise 128 x 128, four of 64 x 64, two workgroups to a CU.
+// HIGH: 256 x 256 tiles, eight wavefronts of 128 x 64, one workgroup to a CU.  Otherwise 128 x 128, four of 64 x 64, two to a CU.
 template <int OP, int DT, bool HIGH>
 struct Shape {
   static constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
   static constexpr bool TR = OP == kWeightsGrad, TQ = OP != kRows;      // the contraction is the operand's slow axis
   static constexpr int BM = HIGH ? 256 : 128, BN = BM, WN = HIGH ? 4 : 2, kWaves = 2 * WN;
   static constexpr int kHeight = BM / 2, kWidth = BN / WN;              // of a wavefront
-  // bytes of contraction in a stage, and how many stages of each operand LDS holds
-  static constexpr int KB = FP8 || !TQ ? 128 : 64, RS = FP8 || !HIGH ? (KB == 64 ? 4 : 2) : TQ ? 5 : 3, QS = FP8 || !HIGH ? RS : TQ ? 5 : 2;
+  // Bytes of contraction in a stage, and how many stages of each operand LDS holds.  Pieces of 64 bytes of a row arrive at half the
+  // rate of whole lines (5 % of a large product); of the slow axis a stage has whole rows of the tile either way, and more of them on
+  // their way are worth 7 %.
+  static constexpr int KB = FP8 || !TQ ? 128 : 64;
+  static constexpr int RS = KB == 64 ? (HIGH ? 5 : 4) : FP8 || !HIGH ? 2 : 3, QS = KB == 64 ? RS : 2;
   static constexpr int BYTES = FP8 ? 1 : 2, STEP = KB / BYTES;
   static constexpr int RL = BM * KB / 1024 / kWaves, QL = BN * KB / 1024 / kWaves, L = RL + QL + (FP8 ? 1 : 0);   // load instructions per wavefront and stage
   static constexpr int kR = BM * KB, kQ = BN * KB, kS = FP8 ? kWaves * 256 : 0;
@@ -54,14 +69,26 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   const int per_expert = OP == kWeightsGrad ? (p.n + BM - 1) / BM : 0;
   int e, m0, n0;
   {
-    const int total = (OP == kWeightsGrad ? p.experts * per_expert : fill_tiles<BM>(p, starts)) * tiles_n;
-    const int q = total >> 3, r = total & 7, xcd = (int)blockIdx.x & 7, at = (int)blockIdx.x >> 3;
-    if (at >= q + (xcd < r ? 1 : 0)) return;
-    const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
-    e = OP == kWeightsGrad ? id / (per_expert * tiles_n) : expert_of_tile(p, starts, id / tiles_n);
-    const int first = OP == kWeightsGrad ? e * per_expert : starts[e], high = OP == kWeightsGrad ? per_expert : starts[e + 1] - first;
+    const int xcd = (int)blockIdx.x & 7, at = (int)blockIdx.x >> 3;
+    int local, high;                                             // tile of the expert, its rows of tiles
+    if (OP == kWeightsGrad) {
+      // (experts differ in length here, not in tiles: every XCD takes an eighth of each expert; whole experts to an XCD left CUs idle
+      // for a third of the time)
+      const int share = (per_expert * tiles_n + 7) / 8;
+      e = at / share;
+      local = xcd * share + at - e * share;
+      if (local >= per_expert * tiles_n) return;
+      high = per_expert;
+    } else {
+      const int total = fill_tiles<BM>(p, starts) * tiles_n, q = total >> 3, r = total & 7;
+      if (at >= q + (xcd < r ? 1 : 0)) return;
+      const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
+      e = expert_of_tile(p, starts, id / tiles_n);
+      local = id - starts[e] * tiles_n;
+      high = starts[e + 1] - starts[e];
+    }
     const int groups = (high + 3) / 4, step = (high + groups - 1) / groups;       // rows of tiles in a group
-    const int local = id - first * tiles_n, group = local / (step * tiles_n), in = local - group * step * tiles_n;
+    const int group = local / (step * tiles_n), in = local - group * step * tiles_n;
     const int height = high - group * step < step ? high - group * step : step;
     const int nt = in / height;
     n0 = nt * BN;
@@ -460,19 +487,19 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
 
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream) {
   const int b = high ? 256 : 128;
-  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b;
-  const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + b - 1) / b) : p.rows / b + p.experts + 1;
-  if (tiles_m * tiles_n > 0x3fffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles_m * tiles_n);
-  const dim3 grid((unsigned)((tiles_m * tiles_n + 7) / 8 * 8)), block(high ? 512 : 256);
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
+  const long long eights = op == kWeightsGrad ? p.experts * ((tiles_w + 7) / 8) : ((p.rows / b + p.experts + 1) * tiles_n + 7) / 8;
+  if (eights > 0x7ffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", eights * 8);
+  const dim3 grid((unsigned)(eights * 8)), block(high ? 512 : 256);
 #define CM_TILE(op_, dt)                                                                              \
   do {                                                                                                \
     if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true>), grid, block, 0, stream, p);    \
     else hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, false>), grid, block, 0, stream, p);        \
   } while (0)
-#define CM_TILE_OP(op_)                                           \
-  do {                                                            \
+#define CM_TILE_OP(op_)                                              \
+  do {                                                               \
     if (dtype == CPPMEGA_MI355_F16) CM_TILE(op_, CPPMEGA_MI355_F16); \
-    else CM_TILE(op_, CPPMEGA_MI355_BF16);                        \
+    else CM_TILE(op_, CPPMEGA_MI355_BF16);                           \
   } while (0)
   if (dtype == CPPMEGA_MI355_E4M3) CM_TILE(kRows, CPPMEGA_MI355_E4M3);
   else if (op == kRows) CM_TILE_OP(kRows);

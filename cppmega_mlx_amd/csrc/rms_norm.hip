@@ -378,8 +378,18 @@ __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float* par
   __shared__ float runs[16][64];
   const int lane = lane_id(), run = (int)(threadIdx.x >> 6), c = (int)blockIdx.x * 64 + lane;
   float sum = 0.0f;
-  if (c < width)
-    for (int g = run; g < groups; g += 16) sum += partial[(size_t)g * width + c];
+  if (c < width) {
+    // (eight loads on their way at a time: one after the other, 512 groups took 11 us)
+    int g = run;
+    for (; g + 7 * 16 < groups; g += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = partial[(size_t)(g + 16 * i) * width + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += v[i];
+    }
+    for (; g < groups; g += 16) sum += partial[(size_t)g * width + c];
+  }
   runs[run][lane] = sum;
   __syncthreads();
   if (run == 0 && c < width) {
