@@ -5,7 +5,8 @@
 // LDS holds rings of stages of both operands, 128 or 64 bytes of contraction each, filled by global_load_lds as far ahead as there is room;
 // two wavefronts on a SIMD, one barrier a stage, behind which the next stage's first operands are read under this one's last products.
 // Rows that are not there repeat the last one and are not stored; contraction that is not there comes from a piece of zeros, for both
-// operands (what lies behind a row may be NaN).  A wavefront whose rows are not there only loads.  16-bit products by 32 x 32 x 16
+// operands (what lies behind a row may be NaN).  Each wavefront has
+// every other 32 rows of the tile and multiplies as many of them as there are; one without rows only loads.  16-bit products by 32 x 32 x 16
 // instructions; e4m3 by 16 x 16 x 128, a scale block each, whose sums are scaled and added while the matrix unit is at the next ones (that
 // instruction aligns eight products to the largest and drops what lies below 2^-13 of it: results of 16 bits do not show it).
 // Pieces are 16 bytes; in LDS
@@ -50,6 +51,9 @@ struct Shape {
   static __device__ __forceinline__ int fold(int row) { return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
 };
 
+template <int N>
+using Count = std::integral_constant<int, N>;
+
 template <int OP, int DT, bool HIGH>
 __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
   typedef Shape<OP, DT, HIGH> S;
@@ -60,7 +64,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   int* const starts = reinterpret_cast<int*>(smem);
   char* const lds = reinterpret_cast<char*>(smem);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (wave / S::WN) * S::kHeight, wn = (wave % S::WN) * S::kWidth;
+  const int wn = (wave % S::WN) * S::kWidth, upper = wave / S::WN;   // a wavefront's columns; every other 32 rows are its rows
 
   // ---- which tile: every XCD takes one run of the order, which goes through the experts; of each, up to four row tiles share the
   // columns that pass, so that an expert's weight leaves memory once (groups of four rows of tiles whatever their experts: 5 % slower) ----
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   // between a stage's last operand reads and its last products: the next stage has arrived, and everybody has read this one
   constexpr int kYounger = (QS - 2) * L + (RS > QS ? RL : 0);    // instructions behind those of the next stage
   auto turn = [&] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kYounger) : "memory"); };
-  const bool live = wm < rows_here;
+  const int runs = rows_here - upper * 32 > 0 ? (rows_here - upper * 32 + 63) / 64 : 0;   // of 32 rows that a wavefront has, the last one in part
   auto follow = [&] {                                           // a wavefront without rows: its loads only
     for (int s = 0; s + 1 < stages; ++s) {
       turn();
@@ -261,12 +265,12 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
     if (TR) {
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
-        const int col = wm + i * 32 + (lane & 16) + (l16 & 3) * 4;
+        const int col = i * 64 + upper * 32 + (lane & 16) + (l16 & 3) * 4;
         rat[i] = (half * 8 + (l16 >> 2)) * (BM * 2) + ((col >> 3) ^ ((l16 >> 2) << 2)) * 16 + (col & 4) * 2;
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) rat[k] = (wm + l32) * KB + ((2 * k + half) ^ S::fold(l32)) * 16;
+      for (int k = 0; k < KS; ++k) rat[k] = (upper * 32 + l32) * KB + ((2 * k + half) ^ S::fold(l32)) * 16;
     }
     if (TQ) {
 #pragma unroll
@@ -285,12 +289,12 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
     };
     bf16x8 r[2][TI], q[2][TJ];
-    auto read_ahead = [&](int rows, int cols, int ks) {
+    auto read_ahead = [&](auto n, int rows, int cols, int ks) {
       const int to = ks & 1;
 #pragma unroll
       for (int j = 0; j < TJ; ++j) q[to][j] = TQ ? transposed(cols + qat[j] + ks * 16 * BN * 2, 4 * BN * 2) : *reinterpret_cast<const bf16x8*>(lds + cols + qat[TQ ? 0 : ks] + j * 32 * KB);
 #pragma unroll
-      for (int i = 0; i < TI; ++i) r[to][i] = TR ? transposed(rows + rat[i] + ks * 16 * BM * 2, 4 * BM * 2) : *reinterpret_cast<const bf16x8*>(lds + rows + rat[TR ? 0 : ks] + i * 32 * KB);
+      for (int i = 0; i < decltype(n)::value; ++i) r[to][i] = TR ? transposed(rows + rat[i] + ks * 16 * BM * 2, 4 * BM * 2) : *reinterpret_cast<const bf16x8*>(lds + rows + rat[TR ? 0 : ks] + i * 64 * KB);
       __builtin_amdgcn_sched_barrier(0);
     };
     f32x16 acc[TI][TJ];
@@ -300,11 +304,12 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
-    // products of one 16 steps; between them load instructions from .. (all at once, the wavefronts stood still until the load
-    // unit's queue had room)
-    auto multiply = [&](int b, auto more, int from) {
+    // products of one 16 steps of the first n of the rows' tiles; between them load instructions from .. (all at once, the wavefronts
+    // stood still until the load unit's queue had room)
+    auto multiply = [&](auto n, int b, auto more, int from) {
+      constexpr int N = decltype(n)::value;
 #pragma unroll
-      for (int i = 0; i < TI; ++i) {
+      for (int i = 0; i < N; ++i) {
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
           if constexpr (F16) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, q[b][j]), __builtin_bit_cast(f16x8, r[b][i]), acc[i][j], 0, 0, 0);
@@ -312,40 +317,45 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
         }
         if (from >= 0) {
           __builtin_amdgcn_sched_barrier(0);
-          issue(more, L * i / TI, L * (i + 1) / TI);
+          issue(more, L * i / N, L * (i + 1) / N);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     };
-    auto stage = [&](auto more) {
+    auto stage = [&](auto n, auto more) {
       const int rows = r_after(), cols = q_after();
 #pragma unroll
       for (int ks = 0; ks + 1 < KS; ++ks) {
-        read_ahead(r_at, q_at, ks + 1);
-        multiply(ks & 1, more, -1);
+        read_ahead(n, r_at, q_at, ks + 1);
+        multiply(n, ks & 1, more, -1);
       }
       turn();
-      read_ahead(rows, cols, 0);
-      multiply((KS - 1) & 1, more, 0);
+      read_ahead(n, rows, cols, 0);
+      multiply(n, (KS - 1) & 1, more, 0);
       r_at = rows;
       q_at = cols;
     };
-    if (!live) {
-      follow();
-    } else if (stages > 0) {
-      read_ahead(r_at, q_at, 0);
+    auto all = [&](auto n) {
+      read_ahead(n, r_at, q_at, 0);
       int s = 0;
-      for (; s < steady; ++s) stage(Whole());
-      for (; s + 1 < stages; ++s) stage(Part());
+      for (; s < steady; ++s) stage(n, Whole());
+      for (; s + 1 < stages; ++s) stage(n, Part());
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        if (ks + 1 < KS) read_ahead(r_at, q_at, ks + 1);
-        multiply(ks & 1, Part(), -1);
+        if (ks + 1 < KS) read_ahead(n, r_at, q_at, ks + 1);
+        multiply(n, ks & 1, Part(), -1);
       }
+    };
+    if (stages > 0) {
+      if (runs == 0) follow();
+      else if (runs >= TI || OP == kWeightsGrad) all(Count<TI>());
+      else if (runs == 1) all(Count<1>());
+      else if (runs == 2) all(Count<(TI > 2 ? 2 : 1)>());
+      else all(Count<(TI > 3 ? 3 : 1)>());
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // (what was requested behind the end still writes to LDS)
     // lane: row l % 32, columns 8 q + 4 (l / 32) + 0..3; the halves change places so that a lane has 8 columns in a run
-    if (live) {
+    if (runs > 0) {
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -359,15 +369,15 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
               v[c] = __uint_as_float(x[0]);
               v[4 + c] = __uint_as_float(x[1]);
             }
-            store(wm + i * 32 + l32, wn + j * 32 + h * 16 + half * 8, v, 8);
+            store(i * 64 + upper * 32 + l32, wn + j * 32 + h * 16 + half * 8, v, 8);
           }
     }
   } else {
     constexpr int TI = S::kHeight / 16, TJ = S::kWidth / 16;        // 16 x 16 tiles of the wavefront, a whole 128-channel block an instruction
     const int l16 = lane & 15, quad = lane >> 4, f = (l16 >> 1) & 7;
-    const int rat[2] = {(wm + l16) * 128 + (quad ^ f) * 16, (wm + l16) * 128 + ((quad + 4) ^ f) * 16};
+    const int rat[2] = {(upper * 32 + l16) * 128 + (quad ^ f) * 16, (upper * 32 + l16) * 128 + ((quad + 4) ^ f) * 16};
     const int qat[2] = {(wn + l16) * 128 + (quad ^ f) * 16, (wn + l16) * 128 + ((quad + 4) ^ f) * 16};
-    const int xsat = (wm + l16) * 4, wsat = BM / 64 * 256 + (wn >> 7) * 4;
+    const int xsat = (upper * 32 + l16) * 4, wsat = BM / 64 * 256 + (wn >> 7) * 4;
     auto operand = [&](int a, int b) -> i32x8 {
       const u32x4 x = *reinterpret_cast<const u32x4*>(lds + a), y = *reinterpret_cast<const u32x4*>(lds + b);
       i32x8 o;
@@ -386,10 +396,11 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
     i32x8 q[TJ], r[2];
     float sx[TI], sw;
     auto read_q = [&](int from, int j) { q[j] = operand(from + qat[0] + j * 2048, from + qat[1] + j * 2048); };
-    auto read_r = [&](int from, int i) { r[i & 1] = operand(from + rat[0] + i * 2048, from + rat[1] + i * 2048); };
-    auto read_scales = [&](int from) {
+    auto row_of = [](int i) { return (i >> 1) * 64 + (i & 1) * 16; };   // where the rows' tile i begins
+    auto read_r = [&](int from, int i) { r[i & 1] = operand(from + rat[0] + row_of(i) * 128, from + rat[1] + row_of(i) * 128); };
+    auto read_scales = [&](auto n, int from) {
 #pragma unroll
-      for (int i = 0; i < TI; ++i) sx[i] = *reinterpret_cast<const float*>(lds + from + xsat + i * 64);
+      for (int i = 0; i < decltype(n)::value; ++i) sx[i] = *reinterpret_cast<const float*>(lds + from + xsat + row_of(i) * 4);
       sw = *reinterpret_cast<const float*>(lds + from + wsat);
     };
     // a block's products are scaled and added while the matrix unit is at the next ones
@@ -405,11 +416,11 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
 #pragma unroll
         for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, t[i & 1][j][v], acc[i][j][v]);
     };
-    // all rows but the last ones; load instructions from .. between them, PER to a group of products
-    constexpr int PER = (L + TI - 1) / TI;
-    auto products = [&](auto more, int from) {
+    // the first n of the rows' tiles (an even number) but the last; load instructions from .. between them, a share to a group of products
+    auto products = [&](auto n, auto more, int from) {
+      constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
 #pragma unroll
-      for (int i = 0; i < TI - 1; ++i) {
+      for (int i = 0; i < N - 1; ++i) {
         read_r(r_at, i + 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -420,52 +431,59 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    if (!live) {
-      follow();
-    } else if (stages > 0) {
+    // between a stage and the next: the last rows' products, and the next operands as soon as their registers are free
+    auto pass = [&](auto n, auto more) {
+      constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
+      const int rows = r_after(), cols = q_after();
+      turn();
+      read_r(rows, 0);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        product(N - 1, j);
+        __builtin_amdgcn_sched_barrier(0);
+        read_q(cols, j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      issue(more, 0, PER);
+      add(N - 2);
+      add(N - 1);
+      s_at = s_after();
+      read_scales(n, s_at);
+      __builtin_amdgcn_sched_barrier(0);
+      r_at = rows;
+      q_at = cols;
+    };
+    auto all = [&](auto n) {
+      constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
 #pragma unroll
       for (int j = 0; j < TJ; ++j) read_q(q_at, j);
       read_r(r_at, 0);
-      read_scales(s_at);
-      // between a stage and the next: the last rows' products, and the next operands as soon as their registers are free
-      auto pass = [&](auto more) {
-        const int rows = r_after(), cols = q_after();
-        turn();
-        read_r(rows, 0);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) {
-          product(TI - 1, j);
-          __builtin_amdgcn_sched_barrier(0);
-          read_q(cols, j);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        issue(more, 0, PER);
-        add(TI - 2);
-        add(TI - 1);
-        s_at = s_after();
-        read_scales(s_at);
-        __builtin_amdgcn_sched_barrier(0);
-        r_at = rows;
-        q_at = cols;
-      };
-      products(Part(), -1);
+      read_scales(n, s_at);
+      products(n, Part(), -1);
       int s = 0;
       for (; s < steady; ++s) {
-        pass(Whole());
-        products(Whole(), PER);
+        pass(n, Whole());
+        products(n, Whole(), PER);
       }
       for (; s + 1 < stages; ++s) {
-        pass(Part());
-        products(Part(), PER);
+        pass(n, Part());
+        products(n, Part(), PER);
       }
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) product(TI - 1, j);
-      add(TI - 2);
-      add(TI - 1);
+      for (int j = 0; j < TJ; ++j) product(N - 1, j);
+      add(N - 2);
+      add(N - 1);
+    };
+    if (stages > 0) {
+      if (runs == 0) follow();
+      else if (runs >= TI / 2) all(Count<TI>());
+      else if (runs == 1) all(Count<2>());
+      else if (runs == 2) all(Count<(TI > 4 ? 4 : 2)>());
+      else all(Count<(TI > 6 ? 6 : 2)>());
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // lane: row l % 16, columns 4 (l / 16) + 0..3; two tiles' quarters change places so that a lane has 8 columns in a run
-    if (live) {
+    if (runs > 0) {
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -477,7 +495,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
             v[c] = __uint_as_float(x[0]);
             v[4 + c] = __uint_as_float(x[1]);
           }
-          store(wm + i * 16 + l16, wn + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, 8);
+          store(row_of(i) + upper * 32 + l16, wn + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, 8);
         }
     }
   }
