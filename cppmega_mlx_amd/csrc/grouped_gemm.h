@@ -36,7 +36,7 @@ __device__ __forceinline__ long long offset_of(const GroupedParams& p, int e) {
 
 // Row tiles of all experts in a row, BM rows each: the first tile of every expert in `starts` (kMaxExperts + 2 ints of LDS, filled by
 // the first wavefront for the whole workgroup); their number comes back.  The rows behind the last expert are those of a last "expert"
-// without a contraction when they are to be zeroed.
+// without a contraction when they are to be zeroed.  (Offsets that overlap may make more tiles than the launch has.)
 template <int BM>
 __device__ __forceinline__ int fill_tiles(const GroupedParams& p, int* starts) {
   if (threadIdx.x < 64) {
@@ -58,7 +58,8 @@ __device__ __forceinline__ int fill_tiles(const GroupedParams& p, int* starts) {
     if (lane == 0) starts[entries] = before;
   }
   __syncthreads();
-  return starts[p.experts + 1];
+  const int total = starts[p.experts + 1], most = (int)(p.rows / BM) + p.experts + 1;
+  return total < most ? total : most;
 }
 // the last entry whose first tile is <= t (entries without rows share their first tile with the next one)
 __device__ __forceinline__ int expert_of_tile(const GroupedParams& p, const int* starts, int t) {
@@ -68,6 +69,11 @@ __device__ __forceinline__ int expert_of_tile(const GroupedParams& p, const int*
     found += __popcll(__ballot(e <= p.experts && starts[e] <= t));
   }
   return __builtin_amdgcn_readfirstlane(found - 1);
+}
+
+// A launch has fewer than 2^32 threads.
+inline int check_tiles(long long tiles, int threads) {
+  return tiles * threads > 0xffffffffll ? fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles) : 0;
 }
 
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);

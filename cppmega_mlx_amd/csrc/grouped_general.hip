@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream) {
   const long long tiles_n = ((op == kRows ? p.n : p.k) + BN - 1) / BN;
   const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + BM - 1) / BM) : p.rows / BM + p.experts + 1;
-  if (tiles_m * tiles_n > 0x7fffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles_m * tiles_n);
+  if (int rc = check_tiles(tiles_m * tiles_n, 256)) return rc;
   const dim3 grid((unsigned)(tiles_m * tiles_n)), block(256);
 #define CM_GENERAL(op_, dt) hipLaunchKernelGGL((grouped_general_kernel<op_, dt>), grid, block, 0, stream, p)
 #define CM_GENERAL_OP(op_)                                           \

@@ -154,7 +154,7 @@ int launch(const GroupedParams& p, hipStream_t stream) {
   const long long tiles_m = p.rows / 16 + tails < p.rows ? p.rows / 16 + tails : p.rows;
   const bool wide = tiles_m * ((p.n + 63) / 64) >= 512;                          // (two workgroups to a CU at least)
   const long long tiles = tiles_m * (wide ? (p.n + 63) / 64 : (p.n + 15) / 16);
-  if (tiles > 0x7fffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles);
+  if (int rc = check_tiles(tiles, 64 * kWaves)) return rc;
   const dim3 grid((unsigned)tiles), block(64 * kWaves);
   if (wide) hipLaunchKernelGGL((grouped_stream_kernel<DT, 4>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((grouped_stream_kernel<DT, 1>), grid, block, 0, stream, p);

@@ -71,10 +71,10 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   const int cols_c = OP == kRows ? p.n : p.k;
   const int tiles_n = (cols_c + BN - 1) / BN;
   const int per_expert = OP == kWeightsGrad ? (p.n + BM - 1) / BM : 0;
-  int e, m0, n0;
+  int e, m0, n0, part_rows = BM;
   {
     const int xcd = (int)blockIdx.x & 7, at = (int)blockIdx.x >> 3;
-    int local, high;                                             // tile of the expert, its rows of tiles
+    int local, high, part = 0;                                   // tile of the expert, its rows of tiles
     if (OP == kWeightsGrad) {
       // (experts differ in length here, not in tiles: every XCD takes an eighth of each expert; whole experts to an XCD left CUs idle
       // for a third of the time)
@@ -85,8 +85,18 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       high = per_expert;
     } else {
       const int total = fill_tiles<BM>(p, starts) * tiles_n, q = total >> 3, r = total & 7;
-      if (at >= q + (xcd < r ? 1 : 0)) return;
-      const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + at;
+      // A last round that leaves half of the XCD's CUs idle or more is made of halves or quarters of its tiles (128 or 64 rows: 0.67 and
+      // 0.5 of a tile's time).
+      constexpr int kSlots = HIGH ? 32 : 64, kParts = BM / 64;
+      const int mine = q + (xcd < r ? 1 : 0), last = mine % kSlots, from = mine - last;
+      const int parts = last * 4 <= kSlots && kParts >= 4 ? 4 : last * 2 <= kSlots ? 2 : 1;
+      if (at >= from + last * parts) return;
+      const int tile = at < from ? at : from + (at - from) / parts;
+      if (at >= from) {
+        part = (at - from) % parts;
+        part_rows = BM / parts;
+      }
+      const int id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + tile;
       e = expert_of_tile(p, starts, id / tiles_n);
       local = id - starts[e] * tiles_n;
       high = starts[e + 1] - starts[e];
@@ -96,7 +106,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
     const int height = high - group * step < step ? high - group * step : step;
     const int nt = in / height;
     n0 = nt * BN;
-    m0 = (group * step + in - nt * height) * BM;
+    m0 = (group * step + in - nt * height) * BM + part * part_rows;
   }
   const int lo = __builtin_amdgcn_readfirstlane((int)offset_of(p, e));
   const int hi = __builtin_amdgcn_readfirstlane(e < p.experts ? (int)offset_of(p, e + 1) : (int)p.rows);
@@ -104,7 +114,8 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   m0 = __builtin_amdgcn_readfirstlane(m0);
   n0 = __builtin_amdgcn_readfirstlane(n0);
   const int contraction = OP == kWeightsGrad ? tokens : (e == p.experts ? 0 : (OP == kRows ? p.k : p.n));
-  const int rows_here = (OP == kWeightsGrad ? p.n : tokens) - m0, cols_here = cols_c - n0;
+  const int rows_left = (OP == kWeightsGrad ? p.n : tokens) - m0, rows_here = rows_left < part_rows ? rows_left : part_rows, cols_here = cols_c - n0;
+  if (rows_here <= 0) return;                                   // (a part behind the expert's last row)
   const int stages = (contraction + STEP - 1) / STEP, whole = contraction / STEP;
   const long long w_pitch = OP == kWeightsGrad ? p.w_pitch : p.k;
 
@@ -506,8 +517,8 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream) {
   const int b = high ? 256 : 128;
   const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
-  const long long eights = op == kWeightsGrad ? p.experts * ((tiles_w + 7) / 8) : ((p.rows / b + p.experts + 1) * tiles_n + 7) / 8;
-  if (eights > 0x7ffffffll) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", eights * 8);
+  const long long eights = op == kWeightsGrad ? p.experts * ((tiles_w + 7) / 8) : ((p.rows / b + p.experts + 1) * tiles_n + 7) / 8 + (high ? 24 : 32);   // (parts of the last tiles)
+  if (int rc = check_tiles(eights * 8, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)(eights * 8)), block(high ? 512 : 256);
 #define CM_TILE(op_, dt)                                                                              \
   do {                                                                                                \

@@ -99,7 +99,7 @@ typedef struct cppmega_mi355_grouped_gemm_args {
   int32_t y_dtype;            /* x_dtype or F32; E4M3 operands: BF16 / F16 / F32             */
   int32_t offsets_dtype;      /* I32 / I64                                                   */
   int32_t x_scale_block;      /* 0 or 128                                                    */
-  int64_t rows;
+  int64_t rows;               /* below 2^29                                                  */
   int64_t x_pitch;            /* elements between rows of x                                  */
   int64_t w_pitch;            /* WEIGHTS_GRAD: elements between rows of w                    */
   int64_t y_pitch;            /* ROWS, ROWS_GRAD: elements between rows of y                 */

@@ -79,6 +79,67 @@ def test_rows_and_gradients(device, case, dtype):
     assert torch.equal(wx.to(dtype), dx) and torch.equal(ww.to(dtype), dw)
 
 
+# Many rows, whose results (or, of the second numbers, gradients) come in large tiles: a last round of whole tiles, halves and quarters, experts of
+# one row and none, rows and outputs that end inside a tile, short and odd contractions, and rows that only the kernel for any alignment takes.
+MANY = [
+    ([4200], 4104, 64), ([5000, 1, 0, 250], 4104, 80), ([3300, 0, 700, 37], 2600, 144), ([5120, 700, 65, 0, 1, 3], 2056, 128),
+    ([257] * 20 + [0] * 12 + [100] * 10, 1032, 272), ([4700], 4104, 528), ([2900, 0, 1400], 2600, 208), ([1900, 5], 1501, 131),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{sum(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+def test_many_rows(device, case):
+    counts, n, k = case
+    rows, tail = sum(counts), 300
+    offsets = _offsets(counts, device)
+    for dtype in (BF16, F16):
+        wide = torch.full((rows + tail, k + 8), float("nan"), dtype=dtype, device=device)
+        x, w = wide[:, :k], _normal(device, len(counts), n, k, dtype=dtype, seed=2)
+        x[:rows] = _normal(device, rows, k, dtype=dtype, seed=1)
+        for e, c in enumerate(counts):
+            if c == 0:
+                w[e] = float("nan")
+        want, size = _plain(x[:rows], w, offsets)
+        out = torch.full((rows + tail, n + 8), 7.0, dtype=dtype, device=device)
+        y = grouped_gemm(x, w, offsets, out=out[:, :n])
+        _assert_near(y[:rows], want, size, k)
+        assert (out[rows:] == 7).all() and (out[:, n:] == 7).all()
+        fresh = grouped_gemm(x, w, offsets)
+        assert torch.equal(fresh[:rows], y[:rows]) and (fresh[rows:] == 0).all()
+        # the same products as a gradient of rows: outputs and inputs change places
+        turned = w.transpose(1, 2).contiguous()
+        dx = torch.full((rows + tail, n), 5.0, dtype=dtype, device=device)
+        grouped_gemm_bwd(x, fresh, turned, offsets, dx=dx, need_dw=False)
+        _assert_near(dx[:rows], want, size, k)
+        assert (dx[rows:] == 5).all()
+        fresh = grouped_gemm_bwd(x, fresh, turned, offsets, need_dw=False)[0]
+        assert torch.equal(fresh[:rows], dx[:rows]) and (fresh[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{sum(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+def test_many_fp8_rows(device, case):
+    counts, n, k = case
+    rows, tail, e = sum(counts), 300, len(counts)
+    offsets = _offsets(counts, device)
+    wide = torch.full((rows + tail, k + 16 - k % 16), 0x7F, dtype=torch.uint8, device=device)
+    x, xs = wide[:, :k], torch.full((rows + tail, (k + 127) // 128), float("nan"), device=device)
+    x[:rows], xs[:rows] = _e4m3(device, rows, k, seed=4), _normal(device, rows, (k + 127) // 128, seed=6).exp() * 1e-2
+    w, ws = _e4m3(device, e, n, k, seed=5), _normal(device, e, (n + 127) // 128, (k + 127) // 128, seed=7).exp() * 1e-2
+    for i, c in enumerate(counts):
+        if c == 0:
+            w[i], ws[i] = 0x7F, float("nan")
+    for scales in (xs, xs[:, 0].contiguous()):
+        want, size = _plain_fp8(x[:rows], scales[:rows], w, ws, offsets)
+        for dtype in (BF16, F32):
+            out = torch.full((rows + tail, n), 7.0, dtype=dtype, device=device)
+            grouped_fp8_gemm(x, scales, w, ws, offsets, out=out)
+            _assert_near(out[:rows], want, size, k + 4 + (DROPPED if dtype == BF16 else 0))
+            assert (out[rows:] == 7).all()
+        fresh = grouped_fp8_gemm(x, scales, w, ws, offsets)
+        assert (fresh[rows:] == 0).all()
+        _assert_near(fresh[:rows], want, size, k + 4 + DROPPED)
+
+
 def _e4m3(device, *shape, seed):
     return (_normal(device, *shape, seed=seed) * 60).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
 

@@ -94,7 +94,7 @@ def test_norm_gradient_refusals(over, code):
 
 @pytest.mark.parametrize("over, code", [
     (dict(op=3), _lib.ERR_SHAPE), (dict(experts=0), _lib.ERR_SHAPE), (dict(experts=_lib.GROUPED_MAX_EXPERTS + 1), _lib.ERR_UNSUPPORTED), (dict(n=0), _lib.ERR_SHAPE),
-    (dict(k=0), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(x_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(y_dtype=_lib.F16), _lib.ERR_DTYPE),
+    (dict(k=0), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(rows=1 << 29), _lib.ERR_SHAPE), (dict(x_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(y_dtype=_lib.F16), _lib.ERR_DTYPE),
     (dict(offsets_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(x_dtype=_lib.E4M3, op=1), _lib.ERR_DTYPE), (dict(x_dtype=_lib.E4M3, x_scale_block=64), _lib.ERR_SHAPE),
     (dict(x_dtype=_lib.E4M3), _lib.ERR_NULL), (dict(offsets=None), _lib.ERR_NULL), (dict(y=None), _lib.ERR_NULL), (dict(w=None), _lib.ERR_NULL),
     (dict(rows=0), _lib.OK), (dict(op=2, rows=0, y=None), _lib.ERR_NULL)])
