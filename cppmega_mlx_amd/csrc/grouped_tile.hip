@@ -14,13 +14,15 @@
 //   contraction slow: [step][pieces of 8 channels], piece c of step s in place c ^ 4 (s % 4), read by the transposing load.
 // (No bank conflicts in either: counted.)
 //
-// Measured, us (TFLOP/s): 16384 rows of 32 experts, 4096 x 2048 bf16 315 (870); of one expert 248 (1110), and 4096 x 8192 833 (1320), where a library's
+// Measured, us (TFLOP/s): 16384 rows of 32 experts, 4096 x 2048 bf16 308 (890); of one expert 248 (1110), and 4096 x 8192 833 (1320), where a library's
 // product of that size reaches 1390: at 1.3 PFLOP/s the clock is down at 1.7 GHz, power is the bound, and neither deeper rings nor other orders
-// of loads change it.  e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 515 (2130): products 2048 of 4000 clocks a stage, the scaling's vector
-// instructions 1000 and the operand reads 1900 beside them.  What short contractions lose: 10 to 12 us a tile for its first loads and for stores that all
-// CUs send at once; persistent workgroups with the next tile's first stages under the stores were not faster, and tiles of few rows after all
-// others 5 % slower (the weights are read twice).
-// Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16: 400 (690); the rows' 320 tiles take two rounds of 256 CUs.
+// of loads change it.  What short contractions lose: 10 to 12 us a tile for its first loads and for stores that all CUs send at once; persistent
+// workgroups with the next tile's first stages under the stores were not faster, and tiles of few rows after all others 5 % slower (the weights are
+// read twice).  Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16: 379 (725), where 320 tiles of rows meet 256 CUs and a gradient's
+// contraction is 512 rows.
+// e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 510 (2150): of a stage's 4000 clocks the products take 2048, what LDS gives and takes
+// 2048 as well (wavefronts of 128 x 128, which would read a third less, have no registers for sums that vector instructions add to), and the
+// scaling's vector instructions 1000 beside them; spread between single products they took as long.
 
 #include <type_traits>
 
