@@ -740,9 +740,10 @@ PyObject* rms_norm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   a.dy_pitch = a.h_pitch = a.dh_pitch = a.dx_pitch = width;
   size_t bytes = 0;
   if (cppmega_mi355_rms_norm_bwd_workspace_bytes(&a, sizeof(a), &bytes)) DECLINE;
-  Tensor scratch = workspace(at.device, at.stream, bytes);
+  // (a tensor of the call's own: within a capture it belongs to the graph, so that graphs of one stream may be replayed side by side)
+  Tensor scratch = at::empty({(int64_t)bytes}, h->options().dtype(at::kByte));
   a.workspace = scratch.data_ptr();
-  a.workspace_bytes = (size_t)scratch.numel();
+  a.workspace_bytes = bytes;
   Tensor dx = at::empty(h->sizes(), h->options()), dweight = at::empty({width}, h->options().dtype(at::kFloat));
   a.dx = dx.data_ptr();
   a.dweight = (float*)dweight.data_ptr();

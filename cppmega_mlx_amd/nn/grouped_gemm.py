@@ -10,7 +10,7 @@ index contiguous as in ``ops.head_gemm``; up to 512 experts.
     grouped_fp8_gemm    the same product of e4m3 rows and block-128 e4m3 weights, every 128-channel block scaled in float32
 
 Experts without rows cost nothing (their ``dw`` is zeros).  Rows behind the last expert's: zeros in an output made here, left as
-they were in a caller-owned one.  Rows may have a pitch of their own; sizes of any kind are served, rows that begin on 16 bytes
+they were in a caller-owned one, which must not overlap the operands.  Rows may have a pitch of their own; sizes of any kind are served, rows that begin on 16 bytes
 by faster kernels.  ``grouped_gemm_apply`` is the differentiable form; a backward pass that is to be captured into a graph must not share its
 leaves with an eager autograd graph that is still alive: capture ``grouped_gemm_bwd``, or drop the eager graph first.
 
@@ -20,6 +20,7 @@ The single-matrix sibling is ``nn/_tilelang/fused_fp8_gemm.py`` (operator caller
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -93,6 +94,7 @@ class _GroupedGemmFunction(torch.autograd.Function):
         return grouped_gemm(x, w, offsets)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         dy = dy if dy.is_contiguous() else dy.contiguous()

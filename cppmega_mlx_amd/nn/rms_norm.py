@@ -18,6 +18,7 @@ the eager graph first.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -95,6 +96,7 @@ class _RmsNormFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         h, weight = ctx.saved_tensors
         if dy is None:                                   # only the stream was used

@@ -945,6 +945,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float, out: torch.Te
             raise ValueError("residual_out without a residual")
         a.residual_out_pitch = _like_rows(residual_out, "residual_out", x, x.dtype)
         _own_rows(residual_out, "residual_out", rows, a.residual_out_pitch)
+        if rows and residual_out.data_ptr() == out.data_ptr():
+            raise ValueError("out and residual_out are one place")
     a.x, a.residual, a.weight, a.out = x.data_ptr(), _lib.ptr(residual), weight.data_ptr(), out.data_ptr()
     a.residual_out, a.scale = _lib.ptr(residual_out), _lib.ptr(scale)
     a.rows, a.width, a.x_pitch, a.eps = rows, n, x_pitch, float(eps)
@@ -957,7 +959,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float, out: torch.Te
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *, eps: float, dx: torch.Tensor, dweight: torch.Tensor,
                       dh: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> None:
     """Gradients of :func:`rms_norm` for the rows ``h`` that were normalised, into caller-owned ``dx`` (like h) and float32
-    ``dweight``; ``dh`` is the gradient that reaches the stream past the norm."""
+    ``dweight``; ``dh`` is the gradient that reaches the stream past the norm.  Scratch belongs to the call (to the graph, within a capture)."""
     rows, h_pitch = _lib.require_rows(h, "h")
     n = int(h.shape[-1])
     a = _lib.RmsNormBwdArgs()
@@ -981,7 +983,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *
     _lib.check(lib.cppmega_mi355_rms_norm_bwd_workspace_bytes(C.byref(a), C.sizeof(a), C.byref(need)), "rms_norm_bwd")
     if need.value:
         if workspace is None:
-            workspace = _workspace(h.device, need.value, stream)
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=h.device)
         else:
             _lib.require_device_tensor(workspace, "workspace", h)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()

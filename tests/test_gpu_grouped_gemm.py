@@ -322,6 +322,13 @@ def test_differentiable_form(device):
     assert torch.equal(x.grad, grouped_gemm_bwd(torch.ones_like(g), x.detach(), w.detach(), offsets, need_dw=False)[0])
 
 
+def test_second_derivatives_are_refused(device):
+    x, w = _normal(device, 8, 16, dtype=BF16, seed=1).requires_grad_(), _normal(device, 2, 8, 16, dtype=BF16, seed=2).requires_grad_()
+    (g,) = torch.autograd.grad(grouped_gemm_apply(x, w, _offsets([3, 5], device)).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
 def test_captured_calls_replay_on_new_values_and_offsets(device):
     n, k, rows, e = 136, 192, 150, 5
     x, w, dy = _normal(device, rows, k, dtype=BF16), _normal(device, e, n, k, dtype=BF16), _normal(device, rows, n, dtype=BF16)

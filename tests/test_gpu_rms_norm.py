@@ -267,6 +267,35 @@ def test_captured_calls_replay_on_new_values(device):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
 
 
+def test_graphs_of_one_stream_side_by_side(device):
+    """Two captures on one stream, replayed on two: neither uses the other's scratch."""
+    sets = [(_normal(device, 4096, 1024, dtype=BF16, seed=70 + i), _normal(device, 4096, 1024, dtype=BF16, seed=80 + i), torch.ones(1024, dtype=BF16, device=device)) for i in range(2)]
+    want = [rms_norm_bwd(*s) for s in sets]
+    side, graphs, got = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            got.append(rms_norm_bwd(*s))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(4):
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+            a[1].zero_()
+        torch.cuda.synchronize()
+
+
+def test_second_derivatives_are_refused(device):
+    x, w = _normal(device, 4, 64, dtype=F32, seed=1).requires_grad_(), torch.ones(64, device=device, requires_grad=True)
+    (g,) = torch.autograd.grad(rms_norm_apply(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_two_streams_at_once(device):
     """The gradient's workspace is one per stream."""
     sets = [(_normal(device, 3000, 2048, dtype=BF16, seed=140 + i), _inputs(device, 3000, 2048, BF16, seed=150 + i)) for i in range(2)]
@@ -284,7 +313,7 @@ def test_two_streams_at_once(device):
 
 
 def test_refusals(device):
-    x, w = torch.zeros(4, 64, dtype=BF16, device=device), torch.ones(64, dtype=BF16, device=device)
+    x, y, w = torch.zeros(4, 64, dtype=BF16, device=device), torch.zeros(4, 64, dtype=BF16, device=device), torch.ones(64, dtype=BF16, device=device)
     bad = [
         (ValueError, lambda: rms_norm(x, w[:60])), (TypeError, lambda: rms_norm(x, w.half())), (TypeError, lambda: rms_norm(x.double(), w.double())),
         (ValueError, lambda: rms_norm(x.t(), w[:4].contiguous())), (ValueError, lambda: rms_norm(x, w, residual=x[:2])), (ValueError, lambda: rms_norm(x, w, residual=x.float())),
@@ -293,7 +322,7 @@ def test_refusals(device):
         (ValueError, lambda: rms_norm_fp8(x, w, scale_block=32)), (ValueError, lambda: rms_norm_fp8(x, w, scale=torch.zeros(3, device=device))),
         (ValueError, lambda: rms_norm_bwd(x[:3], x, w)), (ValueError, lambda: rms_norm_bwd(x.half(), x, w)), (ValueError, lambda: rms_norm_bwd(x, x, w, dweight=torch.zeros(64, dtype=BF16, device=device))),
         (ValueError, lambda: rms_norm(torch.zeros(1, _lib.NORM_MAX_WIDTH + 1, device=device), torch.zeros(_lib.NORM_MAX_WIDTH + 1, device=device))),
-        (_lib.NativeCallError, lambda: rms_norm(x, w.cpu())), (TypeError, lambda: rms_norm(x, w, residual=1.0)),
+        (_lib.NativeCallError, lambda: rms_norm(x, w.cpu())), (TypeError, lambda: rms_norm(x, w, residual=1.0)), (ValueError, lambda: rms_norm(x, w, residual=x, out=y, residual_out=y)),
     ]
     for i, (error, call) in enumerate(bad):
         with pytest.raises(error):
