@@ -6,7 +6,7 @@
 // Bound by memory: a row is read once into registers, reduced, and written from there.  A lane owns 8 consecutive channels of
 // every THREADS * 8 (16-byte loads of 16-bit rows, at whatever alignment the row has), so that a 128-channel block of scales is
 // 16 lanes.  Sums of squares, products with the weight, scales and the weight's gradient are float32; h is rounded once (it is
-// the stream that the next layer reads, so y is the norm of what is stored), y once, from its float32 value, codes as well.
+// the stream that the next layer reads, so y is the norm of what is stored), y once, from its float32 value, codes from float32 as well.
 //
 // Measured with cold caches, bf16 with the residual: 8192 x 7168 82 us (5.7 TB/s; a copy of that size 4.9), e4m3 rows in blocks 74 us (4.8); 32768 x 1536
 // 72 and 63; 4 x 7168 3.3 us, a launch.  Gradients: 8192 x 7168 75 us (6.3 TB/s), 4096 x 7168 41, 32768 x 1536 70.
@@ -118,7 +118,7 @@ __device__ __forceinline__ float over_row(float v, float* slots) {
 }
 
 __device__ __forceinline__ float scale_of(float amax, bool pow2) {
-  if (!pow2) return fmaxf(amax * (1.0f / 448.0f), 1.0e-12f);
+  if (!pow2) return fmaxf(amax / 448.0f, 1.0e-12f);
   float s = 1.0f;                              // amax = fr * 2^ex, fr in [0.5, 1): the smallest power of two with 448 s >= amax
   if (amax > 0.0f) {
     int ex;
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
     float wv[8];
     unpack8<WT>(w[i], wv);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * s * wv[e];
+    for (int e = 0; e < 8; ++e) v[i][e] = FP8 ? v[i][e] * wv[e] : v[i][e] * s * wv[e];
   }
   if constexpr (!FP8) {
 #pragma unroll
@@ -232,10 +232,14 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * THREADS + tid) * 8, valid = p.width - c;
-      const float sc = scale_of(p.scale_block ? over16<true>(am[i]) : am[0], p.pow2), r = 1.0f / sc;
+      // y / scale = h w s / (max |h w| s / 448) = h w / (max |h w| / 448): without s and the roundings that come with it (8192 x 7168
+      // bf16 rows: 159 codes are not those of 64 bits, 4000 with y / scale).  A scale that is rounded to a power of two or held at its least divides y itself.
+      const float top = p.scale_block ? over16<true>(am[i]) : am[0], sc = scale_of(top * s, p.pow2);
+      const bool cancels = !p.pow2 && sc > 1.0e-12f;
+      const float d = cancels ? top / 448.0f : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
       float q[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e], sc, r);
+      for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e] * f, d, r);
       const uint2 codes = make_uint2(codes4(q[0], q[1], q[2], q[3]), codes4(q[4], q[5], q[6], q[7]));
       unsigned char* const to = (unsigned char*)p.out + row * p.out_pitch + c;
       if (valid >= 8) {
