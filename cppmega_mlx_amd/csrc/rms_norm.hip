@@ -410,12 +410,13 @@ __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float* par
 // a workgroup for every CU at least, and at most 1024 threads of them to a CU (512 of narrow rows).  Measured, us with 256 / 512 / 1024 groups:
 // 512 x 7168 14 / 17 / 17, 2048 x 4096 22 / 18 / 21, 8192 x 4096 61 / 44 / 42, 4096 x 7168 50 / 41 / 48, 2048 x 16384 54 / 59 / 71.
 int bwd_groups(long long rows, int width) {
-  const long long most = width <= 512 ? 2048 : width <= 4096 ? 1024 : width <= 8192 ? 512 : 256;
+  const long long most = width <= 1024 ? 2048 : width <= 4096 ? 1024 : width <= 8192 ? 512 : 256;
   const long long groups = rows / 4 < 256 ? 256 : rows / 4 < most ? rows / 4 : most;
   return (int)(rows < groups ? rows : groups);
 }
 
-// Rows of up to 8192 channels: a thread for every 8 of them where rows are few and latency counts (7168 channels, us of 1 / 512 rows: 3.2 / 7.2,
+// Rows of up to 1024 channels: one wavefront, without a barrier (32768 x 1024 42 us, e4m3 39; 256 threads 50 and 58; of 2048 channels 93 and 84; 92 and 81).
+// Of up to 8192: a thread for every 8 channels where rows are few and latency counts (7168 channels, us of 1 / 512 rows: 3.2 / 7.2,
 // with 512 threads 3.5 / 7.7), half as many where they are not (4096 rows, e4m3: 37, with 1024 threads 39).  A launch has fewer than 2^32 threads.
 template <int DT, bool WF32, bool FP8>
 void launch_norm(NormParams p, hipStream_t stream) {
@@ -426,6 +427,7 @@ void launch_norm(NormParams p, hipStream_t stream) {
 #define CM_NORM(threads, per) \
   hipLaunchKernelGGL((rms_norm_kernel<DT, WF32, FP8, threads, per>), dim3(threads == 64 ? (rows + 3) / 4 : rows), dim3(threads == 64 ? 256 : threads), 0, stream, p)
     if (p.width <= 512) CM_NORM(64, 1);
+    else if (p.width <= 1024) CM_NORM(64, 2);
     else if (p.width <= 2048) CM_NORM(256, 1);
     else if (p.width <= 4096) CM_NORM(256, 2);
     else if (p.width <= 8192 && total > 512) CM_NORM(512, 2);
@@ -442,6 +444,7 @@ void launch_bwd(const NormBwdParams& p, hipStream_t stream) {
 #define CM_BWD(threads, per) \
   hipLaunchKernelGGL((rms_norm_bwd_kernel<DT, WF32, threads, per, (threads == 1024 && per > 1)>), dim3(threads == 64 ? (groups + 3) / 4 : groups), dim3(threads == 64 ? 256 : threads), 0, stream, p)
   if (p.width <= 512) CM_BWD(64, 1);
+  else if (p.width <= 1024) CM_BWD(64, 2);
   else if (p.width <= 2048) CM_BWD(256, 1);
   else if (p.width <= 4096) CM_BWD(256, 2);
   else if (p.width <= 8192) CM_BWD(512, 2);

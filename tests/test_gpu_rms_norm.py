@@ -176,7 +176,7 @@ def _plain_bwd(g, h, w, eps, dh=None):
     return dx, (g * h * s).sum(0), size, (g * h * s).abs().sum(0)
 
 
-@pytest.mark.parametrize("shape", SHAPES + [(513, 96), (2500, 64), (1027, 5000), (5001, 1030), (9001, 40), (2101, 9000)])
+@pytest.mark.parametrize("shape", SHAPES + [(513, 96), (2500, 64), (1027, 5000), (5001, 1030), (9001, 40), (2101, 9000), (2049, 1000)])
 @pytest.mark.parametrize("dtype, wdtype", [(BF16, BF16), (F16, F32), (F32, F32)])
 @pytest.mark.parametrize("past", [False, True])
 def test_gradients(device, shape, dtype, wdtype, past):
