@@ -66,6 +66,7 @@ LAYER_SYMBOLS = (
     "cppmega_mi355_rms_norm_bwd_workspace_bytes",
     "cppmega_mi355_rms_norm_bwd",
     "cppmega_mi355_grouped_gemm",
+    "cppmega_mi355_grouped_gemm_bwd",
 )
 NORM_MAX_WIDTH = 32768                # CPPMEGA_MI355_NORM_MAX_WIDTH
 GROUPED_MAX_EXPERTS = 512             # CPPMEGA_MI355_GROUPED_MAX_EXPERTS
@@ -529,6 +530,8 @@ def load() -> C.CDLL:
                            (lib.cppmega_mi355_grouped_gemm, GroupedGemmArgs)):
             fn.argtypes = [C.POINTER(struct), C.c_size_t, C.c_void_p]
             fn.restype = C.c_int
+        lib.cppmega_mi355_grouped_gemm_bwd.argtypes = [C.POINTER(GroupedGemmArgs), C.POINTER(GroupedGemmArgs), C.c_size_t, C.c_void_p]
+        lib.cppmega_mi355_grouped_gemm_bwd.restype = C.c_int
         lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.argtypes = [C.POINTER(RmsNormBwdArgs), C.c_size_t, C.POINTER(C.c_size_t)]
         lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.restype = C.c_int
         lib.cppmega_mi355_fp8_vecmat_workspace_bytes.argtypes = [

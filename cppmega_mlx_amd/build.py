@@ -44,7 +44,7 @@ NO_SCRATCH = {
     "sparse_mla_latent.hip": ("sparse_mla_latent_kernel",),
     "sparse_mla_rows16.hip": ("sparse_mla_rows16_kernel",),
     "fp8_gemm.hip": ("fp8_gemm_kernel",),
-    "grouped_tile.hip": ("grouped_tile_kernel",),
+    "grouped_tile.hip": ("grouped_tile_kernel", "grouped_tile_grads_kernel"),
 }
 
 

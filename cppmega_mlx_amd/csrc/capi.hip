@@ -46,6 +46,7 @@ int rms_norm_launch(const cppmega_mi355_rms_norm_args_t& a, hipStream_t stream);
 int rms_norm_bwd_launch(const cppmega_mi355_rms_norm_bwd_args_t& a, hipStream_t stream);
 int rms_norm_bwd_workspace_bytes(const cppmega_mi355_rms_norm_bwd_args_t& a, size_t* bytes);
 int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream);
+int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream);
 int indexer_topk_launch(const cppmega_mi355_indexer_args_t& a, hipStream_t stream);
 int indexer_topk_workspace_bytes(const cppmega_mi355_indexer_args_t& a, size_t* bytes);
 
@@ -418,6 +419,12 @@ int cppmega_mi355_rms_norm_bwd(const cppmega_mi355_rms_norm_bwd_args_t* args, si
 int cppmega_mi355_grouped_gemm(const cppmega_mi355_grouped_gemm_args_t* args, size_t args_size, void* stream) {
   CM_CHECK_ARGS(args, args_size, cppmega_mi355_grouped_gemm_args_t);
   return grouped_gemm_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_grouped_gemm_bwd(const cppmega_mi355_grouped_gemm_args_t* rows, const cppmega_mi355_grouped_gemm_args_t* weights, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(rows, args_size, cppmega_mi355_grouped_gemm_args_t);
+  CM_CHECK_ARGS(weights, args_size, cppmega_mi355_grouped_gemm_args_t);
+  return grouped_gemm_bwd_launch(*rows, *weights, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -78,6 +78,7 @@ inline int check_tiles(long long tiles, int threads) {
 
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream);
+int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream);
 int grouped_stream_launch(const GroupedParams& p, int dtype, hipStream_t stream);
 
 }  // namespace cm

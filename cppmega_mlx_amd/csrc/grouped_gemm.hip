@@ -32,9 +32,16 @@ bool high_tiles(const GroupedParams& p, int op) {
   return rounds(256, 256, 0.5, 0.67) <= 0.63 * rounds(128, 512, 0.62, 0.62);
 }
 
-}  // namespace
+// What a call runs: nothing, or one of the kernels.
+enum Kind { kNothing, kGeneral, kStream, kTile };
+struct Plan {
+  GroupedParams p;
+  Kind kind;
+  bool high;
+};
 
-int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
+int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
+  to.kind = kNothing;
   if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: unknown op %d", a.op);
   if (a.rows < 0 || a.rows > 0x1fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
     return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
@@ -53,21 +60,52 @@ int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t 
   if (a.rows == 0 && a.op != kWeightsGrad) return 0;
   if (!a.y || !a.offsets || (a.rows > 0 && (!a.x || !a.w)) || (fp8 && (!a.x_scale || !a.w_scale)))
     return fail(CPPMEGA_MI355_ERR_NULL, "grouped_gemm: x / w / y / offsets / scales is NULL");
-  GroupedParams p;
+  GroupedParams& p = to.p;
   p.x = a.x; p.w = a.w; p.y = a.y; p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale;
   p.rows = a.rows; p.x_pitch = a.x_pitch; p.w_pitch = a.w_pitch; p.y_pitch = a.y_pitch;
   p.experts = a.experts; p.n = a.n; p.k = a.k;
   p.y_dtype = a.y_dtype; p.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; p.x_scale_block = a.x_scale_block; p.zero_tail = a.zero_tail;
+  to.kind = kGeneral;
   if (pieces_whole(p, a.op, a.x_dtype)) {
     // Few rows to an expert: the kernel that streams the weights.  Measured against tiles, us, 64 experts of 2048 x 2048: 8 rows each 102 / 130
     // (bf16) and 56 / 60 (e4m3), 12 rows 104 / 130 and 61 / 60, 16 rows 117 / 130 and 69 / 59, 24 rows 152 / 132 and 88 / 61.  (For float32
     // results of e4m3 operands there is the general kernel instead of tiles, which takes three times as long.)
     const bool exact = fp8 && a.y_dtype == CPPMEGA_MI355_F32;
-    if (a.op == kRows && a.rows < (fp8 && !exact ? 12ll : 20ll) * a.experts) return grouped_stream_launch(p, a.x_dtype, stream);
-    // (float32 results of e4m3 operands stay with the general kernel, whose products are exact)
-    if (!exact) return grouped_tile_launch(p, a.op, a.x_dtype, high_tiles(p, a.op), stream);
+    if (a.op == kRows && a.rows < (fp8 && !exact ? 12ll : 20ll) * a.experts) {
+      to.kind = kStream;
+    } else if (!exact) {                                         // (float32 results of e4m3 operands stay with the general kernel, whose products are exact)
+      to.kind = kTile;
+      to.high = high_tiles(p, a.op);
+    }
   }
-  return grouped_general_launch(p, a.op, a.x_dtype, stream);
+  return 0;
+}
+
+int launch(const Plan& plan, int op, int dtype, hipStream_t stream) {
+  if (plan.kind == kTile) return grouped_tile_launch(plan.p, op, dtype, plan.high, stream);
+  if (plan.kind == kStream) return grouped_stream_launch(plan.p, dtype, stream);
+  return plan.kind == kGeneral ? grouped_general_launch(plan.p, op, dtype, stream) : 0;
+}
+
+}  // namespace
+
+int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
+  Plan plan;
+  if (int rc = plan_of(a, plan)) return rc;
+  return launch(plan, a.op, a.x_dtype, stream);
+}
+
+int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream) {
+  if (rows.op != kRowsGrad || weights.op != kWeightsGrad)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm_bwd: ops %d and %d are not the rows' and the weights' gradient", rows.op, weights.op);
+  Plan r, w;
+  int rc = plan_of(rows, r);
+  if (!rc) rc = plan_of(weights, w);
+  if (rc) return rc;
+  if (r.kind == kTile && w.kind == kTile && r.high == w.high && rows.x_dtype == weights.x_dtype)
+    return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, r.high, stream);
+  rc = launch(r, kRowsGrad, rows.x_dtype, stream);
+  return rc ? rc : launch(w, kWeightsGrad, weights.x_dtype, stream);
 }
 
 }  // namespace cm

@@ -56,13 +56,14 @@ struct Shape {
 template <int N>
 using Count = std::integral_constant<int, N>;
 
+// Tile `block` of a product (of the launch's order, or none: every XCD's blocks are counted up to the same number), in S::kLds bytes of LDS.
+// `cut`: the last round's tiles in parts.
 template <int OP, int DT, bool HIGH>
-__global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
-  typedef Shape<OP, DT, HIGH> S;
+__device__ __forceinline__ void tile_of(const GroupedParams& p, const int block, u32x4* const smem, const bool cut) {
+  typedef Shape<OP, DT, HIGH> S;                                 // (inlined throughout: a call would put the sums into memory)
   constexpr bool FP8 = S::FP8, F16 = S::F16, TR = S::TR, TQ = S::TQ;
   constexpr int BYTES = S::BYTES, STEP = S::STEP, BM = S::BM, BN = S::BN, RS = S::RS, QS = S::QS, RL = S::RL, QL = S::QL, L = S::L, KB = S::KB;
-  __shared__ u32x4 smem[S::kLds / 16];
-  static_assert(sizeof(smem) >= (kMaxExperts + 2) * sizeof(int), "the tiles' table lies where the stages are later");
+  static_assert(S::kLds >= (kMaxExperts + 2) * (int)sizeof(int), "the tiles' table lies where the stages are later");
   int* const starts = reinterpret_cast<int*>(smem);
   char* const lds = reinterpret_cast<char*>(smem);
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   const int per_expert = OP == kWeightsGrad ? (p.n + BM - 1) / BM : 0;
   int e, m0, n0, part_rows = BM;
   {
-    const int xcd = (int)blockIdx.x & 7, at = (int)blockIdx.x >> 3;
+    const int xcd = block & 7, at = block >> 3;
     int local, high, part = 0;                                   // tile of the expert, its rows of tiles
     if (OP == kWeightsGrad) {
       // (experts differ in length here, not in tiles: every XCD takes an eighth of each expert; whole experts to an XCD left CUs idle
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       // 0.5 of a tile's time).
       constexpr int kSlots = HIGH ? 32 : 64, kParts = BM / 64;
       const int mine = q + (xcd < r ? 1 : 0), last = mine % kSlots, from = mine - last;
-      const int parts = last * 4 <= kSlots && kParts >= 4 ? 4 : last * 2 <= kSlots ? 2 : 1;
+      const int parts = !cut ? 1 : last * 4 <= kSlots && kParts >= 4 ? 4 : last * 2 <= kSlots ? 2 : 1;
       if (at >= from + last * parts) return;
       const int tile = at < from ? at : from + (at - from) / parts;
       if (at >= from) {
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   // Requests instruction i of a stage: the columns' (and scales') first, then the rows', which may be a stage further on.  MORE:
   // whole stages.  Otherwise the last one, of which a part may not be there, or one behind it: pieces of zeros (no branch here or in the
   // loops below: the compiler moves products across branches, away from the reads that they cover).
-  auto issue = [&](auto more, int from, int to) {
+  auto issue = [&](auto more, int from, int to) __attribute__((always_inline)) {
     constexpr bool MORE = decltype(more)::value;
 #pragma unroll
     for (int i = 0; i < L; ++i) {
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   constexpr int kYounger = (QS - 2) * L + (RS > QS ? RL : 0);    // instructions behind those of the next stage
   auto turn = [&] { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kYounger) : "memory"); };
   const int runs = rows_here - upper * 32 > 0 ? (rows_here - upper * 32 + 63) / 64 : 0;   // of 32 rows that a wavefront has, the last one in part
-  auto follow = [&] {                                           // a wavefront without rows: its loads only
+  auto follow = [&]() __attribute__((always_inline)) {            // a wavefront without rows: its loads only
     for (int s = 0; s + 1 < stages; ++s) {
       turn();
       if (s < steady) issue(Whole(), 0, L);
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   const size_t row0 = OP == kWeightsGrad ? (size_t)e * p.n + m0 : (size_t)lo + m0;
   const long long y_pitch = OP == kWeightsGrad ? p.k : p.y_pitch;
   // 8 (16-bit) or 4 (float32) values of a row, as far as the columns go
-  auto store = [&](int row, int col, const float* v, int count) {
+  auto store = [&](int row, int col, const float* v, int count) __attribute__((always_inline)) {
     if (row >= rows_here || col >= cols_here) return;
     const size_t at = (row0 + row) * y_pitch + n0 + col;
     if (col + count <= cols_here) {
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
     };
     bf16x8 r[2][TI], q[2][TJ];
-    auto read_ahead = [&](auto n, int rows, int cols, int ks) {
+    auto read_ahead = [&](auto n, int rows, int cols, int ks) __attribute__((always_inline)) {
       const int to = ks & 1;
 #pragma unroll
       for (int j = 0; j < TJ; ++j) q[to][j] = TQ ? transposed(cols + qat[j] + ks * 16 * BN * 2, 4 * BN * 2) : *reinterpret_cast<const bf16x8*>(lds + cols + qat[TQ ? 0 : ks] + j * 32 * KB);
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
         for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
     // products of one 16 steps of the first n of the rows' tiles; between them load instructions from .. (all at once, the wavefronts
     // stood still until the load unit's queue had room)
-    auto multiply = [&](auto n, int b, auto more, int from) {
+    auto multiply = [&](auto n, int b, auto more, int from) __attribute__((always_inline)) {
       constexpr int N = decltype(n)::value;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       }
       __builtin_amdgcn_sched_barrier(0);
     };
-    auto stage = [&](auto n, auto more) {
+    auto stage = [&](auto n, auto more) __attribute__((always_inline)) {
       const int rows = r_after(), cols = q_after();
 #pragma unroll
       for (int ks = 0; ks + 1 < KS; ++ks) {
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       r_at = rows;
       q_at = cols;
     };
-    auto all = [&](auto n) {
+    auto all = [&](auto n) __attribute__((always_inline)) {
       read_ahead(n, r_at, q_at, 0);
       int s = 0;
       for (; s < steady; ++s) stage(n, Whole());
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
         for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, t[i & 1][j][v], acc[i][j][v]);
     };
     // the first n of the rows' tiles (an even number) but the last; load instructions from .. between them, a share to a group of products
-    auto products = [&](auto n, auto more, int from) {
+    auto products = [&](auto n, auto more, int from) __attribute__((always_inline)) {
       constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
 #pragma unroll
       for (int i = 0; i < N - 1; ++i) {
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       }
     };
     // between a stage and the next: the last rows' products, and the next operands as soon as their registers are free
-    auto pass = [&](auto n, auto more) {
+    auto pass = [&](auto n, auto more) __attribute__((always_inline)) {
       constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
       const int rows = r_after(), cols = q_after();
       turn();
@@ -466,7 +467,7 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
       r_at = rows;
       q_at = cols;
     };
-    auto all = [&](auto n) {
+    auto all = [&](auto n) __attribute__((always_inline)) {
       constexpr int N = decltype(n)::value, PER = (L + N - 1) / N;
 #pragma unroll
       for (int j = 0; j < TJ; ++j) read_q(q_at, j);
@@ -514,14 +515,35 @@ __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const
   }
 }
 
+template <int OP, int DT, bool HIGH>
+__global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
+  __shared__ u32x4 smem[Shape<OP, DT, HIGH>::kLds / 16];
+  tile_of<OP, DT, HIGH>(p, (int)blockIdx.x, smem, true);
+}
+
+// Both gradients: the weights' tiles fill the CUs that the rows' last round leaves idle.
+template <int DT, bool HIGH>
+__global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_grads_kernel(const GroupedParams rows, const GroupedParams weights, const int first) {
+  constexpr int kLds = Shape<kRowsGrad, DT, HIGH>::kLds, kLdsW = Shape<kWeightsGrad, DT, HIGH>::kLds;
+  __shared__ u32x4 smem[(kLds > kLdsW ? kLds : kLdsW) / 16];
+  if ((int)blockIdx.x < first) tile_of<kRowsGrad, DT, HIGH>(rows, (int)blockIdx.x, smem, false);
+  else tile_of<kWeightsGrad, DT, HIGH>(weights, (int)blockIdx.x - first, smem, false);
+}
+
+// Blocks of a product, a multiple of eight.
+long long blocks_of(const GroupedParams& p, int op, bool high, bool cut) {
+  const int b = high ? 256 : 128;
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
+  if (op == kWeightsGrad) return p.experts * ((tiles_w + 7) / 8) * 8;
+  return (((p.rows / b + p.experts + 1) * tiles_n + 7) / 8 + (!cut ? 0 : high ? 24 : 32)) * 8;   // (parts of the last tiles)
+}
+
 }  // namespace
 
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream) {
-  const int b = high ? 256 : 128;
-  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
-  const long long eights = op == kWeightsGrad ? p.experts * ((tiles_w + 7) / 8) : ((p.rows / b + p.experts + 1) * tiles_n + 7) / 8 + (high ? 24 : 32);   // (parts of the last tiles)
-  if (int rc = check_tiles(eights * 8, high ? 512 : 256)) return rc;
-  const dim3 grid((unsigned)(eights * 8)), block(high ? 512 : 256);
+  const long long blocks = blocks_of(p, op, high, true);
+  if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
+  const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
 #define CM_TILE(op_, dt)                                                                              \
   do {                                                                                                \
     if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true>), grid, block, 0, stream, p);    \
@@ -538,6 +560,22 @@ int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hi
   else CM_TILE_OP(kWeightsGrad);
 #undef CM_TILE_OP
 #undef CM_TILE
+  CM_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream) {
+  const long long first = blocks_of(rows, kRowsGrad, high, false), blocks = first + blocks_of(weights, kWeightsGrad, high, false);
+  if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
+  const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
+#define CM_GRADS(dt)                                                                                                              \
+  do {                                                                                                                            \
+    if (high) hipLaunchKernelGGL((grouped_tile_grads_kernel<dt, true>), grid, block, 0, stream, rows, weights, (int)first);       \
+    else hipLaunchKernelGGL((grouped_tile_grads_kernel<dt, false>), grid, block, 0, stream, rows, weights, (int)first);           \
+  } while (0)
+  if (dtype == CPPMEGA_MI355_F16) CM_GRADS(CPPMEGA_MI355_F16);
+  else CM_GRADS(CPPMEGA_MI355_BF16);
+#undef CM_GRADS
   CM_HIP_CHECK(hipGetLastError());
   return 0;
 }

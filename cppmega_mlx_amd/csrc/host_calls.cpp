@@ -801,11 +801,7 @@ PyObject* grouped_gemm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   b.op = CPPMEGA_MI355_GROUPED_WEIGHTS_GRAD;
   b.w = x->data_ptr(); b.y = dw.data_ptr();
   b.w_pitch = a.k;
-  if (unlocked([&] {
-        const int rc = cppmega_mi355_grouped_gemm(&a, sizeof(a), at.stream);
-        return rc ? rc : cppmega_mi355_grouped_gemm(&b, sizeof(b), at.stream);
-      }))
-    DECLINE;
+  if (unlocked([&] { return cppmega_mi355_grouped_gemm_bwd(&a, &b, sizeof(a), at.stream); })) DECLINE;
   return tuple_of({dx, dw});
 }
 

@@ -57,16 +57,18 @@ def grouped_gemm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets
         raise ValueError(f"grouped_gemm_bwd shape mismatch: dy {tuple(dy.shape)}, x {tuple(x.shape)}, w {tuple(w.shape)}")
     if not (dy.dtype == x.dtype == w.dtype):
         raise TypeError(f"dy, x and w must have one type; got {dy.dtype}, {x.dtype}, {w.dtype}")
-    if need_dx:
-        fresh = dx is None
-        if fresh:
-            dx = torch.empty((x.shape[0], K), dtype=x.dtype, device=x.device)
+    fresh = dx is None
+    if need_dx and fresh:
+        dx = torch.empty((x.shape[0], K), dtype=x.dtype, device=x.device)
+    if need_dw and dw is None:
+        dw = torch.empty((E, N, K), dtype=w.dtype, device=w.device)
+    elif need_dw and tuple(dw.shape) != (E, N, K):
+        raise ValueError(f"dw must have shape {(E, N, K)}; got {tuple(dw.shape)}")
+    if need_dx and need_dw:
+        ops.grouped_gemm_backward(dy, x, w, offsets, dx=dx, dw=dw, zero_tail=fresh)
+    elif need_dx:
         ops.grouped_gemm(dy, w, offsets, out=dx, zero_tail=fresh, transposed=True)
-    if need_dw:
-        if dw is None:
-            dw = torch.empty((E, N, K), dtype=w.dtype, device=w.device)
-        elif tuple(dw.shape) != (E, N, K):
-            raise ValueError(f"dw must have shape {(E, N, K)}; got {tuple(dw.shape)}")
+    elif need_dw:
         ops.grouped_weights_grad(dy, x, offsets, out=dw)
     return (dx if need_dx else None), (dw if need_dw else None)
 

@@ -1032,11 +1032,7 @@ def _grouped_call(a: _lib.GroupedGemmArgs, device: torch.device) -> None:
 _HALF = (torch.float16, torch.bfloat16)
 
 
-def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor, zero_tail: bool = False,
-                 transposed: bool = False) -> torch.Tensor:
-    """out[t, n] = sum_k x[t, k] w[e(t), n, k] into caller-owned ``out``; ``transposed``: out[t, k] = sum_n x[t, n] w[e(t), n, k].
-
-    Rows ``offsets[e] .. offsets[e + 1]`` belong to expert e; rows behind the last expert are left as they are, or zeroed."""
+def _grouped_rows_args(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor, zero_tail: bool, transposed: bool) -> _lib.GroupedGemmArgs:
     _lib.require_rows(x, "x")
     if x.ndim != 2 or x.dtype not in _HALF:
         raise TypeError(f"x must be a 2D float16 or bfloat16 tensor of rows; got {x.dtype} {tuple(x.shape)}")
@@ -1051,12 +1047,10 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     _own_rows(out, "out", T, a.y_pitch)
     a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, a.x_dtype))
     a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
-    _grouped_call(a, x.device)
-    return out
+    return a
 
 
-def grouped_weights_grad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor) -> torch.Tensor:
-    """out[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k] (zeros for an expert without rows)."""
+def _grouped_weights_args(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out: torch.Tensor) -> _lib.GroupedGemmArgs:
     _lib.require_rows(x, "x")
     if x.ndim != 2 or x.dtype not in _HALF:
         raise TypeError(f"x must be a 2D float16 or bfloat16 tensor of rows; got {x.dtype} {tuple(x.shape)}")
@@ -1069,8 +1063,33 @@ def grouped_weights_grad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tenso
     a.x_pitch = _rows2d(dy, "dy", (T, N), x)
     a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, a.x_dtype))
     a.x, a.w, a.y = dy.data_ptr(), x.data_ptr(), out.data_ptr()
-    _grouped_call(a, x.device)
+    return a
+
+
+def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor, zero_tail: bool = False,
+                 transposed: bool = False) -> torch.Tensor:
+    """out[t, n] = sum_k x[t, k] w[e(t), n, k] into caller-owned ``out``; ``transposed``: out[t, k] = sum_n x[t, n] w[e(t), n, k].
+
+    Rows ``offsets[e] .. offsets[e + 1]`` belong to expert e; rows behind the last expert are left as they are, or zeroed."""
+    _grouped_call(_grouped_rows_args(x, w, offsets, out, zero_tail, transposed), x.device)
     return out
+
+
+def grouped_weights_grad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor) -> torch.Tensor:
+    """out[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k] (zeros for an expert without rows)."""
+    _grouped_call(_grouped_weights_args(dy, x, offsets, out), x.device)
+    return out
+
+
+def grouped_gemm_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, dx: torch.Tensor, dw: torch.Tensor,
+                          zero_tail: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """``grouped_gemm(dy, w, offsets, out=dx, transposed=True)`` and ``grouped_weights_grad(dy, x, offsets, out=dw)``, in one launch
+    where their kernels allow it."""
+    a, b = _grouped_rows_args(dy, w, offsets, dx, zero_tail, True), _grouped_weights_args(dy, x, offsets, dw)
+    with torch.cuda.device(dy.device):
+        rc = _lib.load().cppmega_mi355_grouped_gemm_bwd(C.byref(a), C.byref(b), C.sizeof(a), _lib.current_stream(dy.device))
+    _lib.check(rc, "grouped_gemm_bwd")
+    return dx, dw
 
 
 def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor, *,

@@ -109,6 +109,10 @@ typedef struct cppmega_mi355_grouped_gemm_args {
 
 int cppmega_mi355_grouped_gemm(const cppmega_mi355_grouped_gemm_args_t* args, size_t args_size, void* stream);
 
+/* The calls of a ROWS_GRAD and a WEIGHTS_GRAD block (independent of each other), in one launch where their kernels allow it. */
+int cppmega_mi355_grouped_gemm_bwd(const cppmega_mi355_grouped_gemm_args_t* rows, const cppmega_mi355_grouped_gemm_args_t* weights,
+                                   size_t args_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,26 @@ def test_grouped_refusals(over, code):
     assert _lib.load().cppmega_mi355_grouped_gemm(C.byref(a), C.sizeof(a), None) == code
 
 
+@pytest.mark.parametrize("rows, weights, code", [
+    (dict(op=2), dict(), _lib.ERR_SHAPE), (dict(), dict(op=1), _lib.ERR_SHAPE), (dict(op=0), dict(), _lib.ERR_SHAPE), (dict(n=0), dict(), _lib.ERR_SHAPE),
+    (dict(), dict(k=0), _lib.ERR_SHAPE), (dict(y=None), dict(), _lib.ERR_NULL), (dict(), dict(y=None), _lib.ERR_NULL), (dict(), dict(x_dtype=_lib.E4M3), _lib.ERR_DTYPE),
+    (dict(struct_size=8), dict(), _lib.ERR_STRUCT_SIZE), (dict(), dict(struct_size=8), _lib.ERR_STRUCT_SIZE), (dict(rows=0), dict(rows=0, offsets=None), _lib.ERR_NULL)])
+def test_both_gradients_refusals(rows, weights, code):
+    """Both blocks are checked before either is launched."""
+    blocks = []
+    for op, over in ((1, rows), (2, weights)):
+        a = _lib.GroupedGemmArgs()
+        a.struct_size, a.op = C.sizeof(a), op
+        a.x = a.w = a.y = a.offsets = FAKE
+        a.x_dtype = a.y_dtype = _lib.BF16
+        a.offsets_dtype = _lib.I32
+        a.rows, a.experts, a.n, a.k, a.x_pitch, a.y_pitch, a.w_pitch = 4, 2, 64, 64, 64, 64, 64
+        for k, v in over.items():
+            setattr(a, k, v)
+        blocks.append(a)
+    assert _lib.load().cppmega_mi355_grouped_gemm_bwd(C.byref(blocks[0]), C.byref(blocks[1]), C.sizeof(blocks[0]), None) == code
+
+
 def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
     x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
     off = torch.tensor([0, 4], dtype=torch.int32)
