@@ -117,8 +117,13 @@ __device__ __forceinline__ float over_row(float v, float* slots) {
   return v;
 }
 
+// v / 448: the product with 1 / 448, corrected by its remainder (infinities have none)
+__device__ __forceinline__ float over448(float v) {
+  const float q = v * (1.0f / 448.0f);
+  return v < __builtin_inff() ? fmaf(fmaf(-448.0f, q, v), 1.0f / 448.0f, q) : q;
+}
 __device__ __forceinline__ float scale_of(float amax, bool pow2) {
-  if (!pow2) return fmaxf(amax / 448.0f, 1.0e-12f);
+  if (!pow2) return fmaxf(over448(amax), 1.0e-12f);
   float s = 1.0f;                              // amax = fr * 2^ex, fr in [0.5, 1): the smallest power of two with 448 s >= amax
   if (amax > 0.0f) {
     int ex;
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
       // bf16 rows: 159 codes are not those of 64 bits, 4000 with y / scale).  A scale that is rounded to a power of two or held at its least divides y itself.
       const float top = p.scale_block ? over16<true>(am[i]) : am[0], sc = scale_of(top * s, p.pow2);
       const bool cancels = !p.pow2 && sc > 1.0e-12f;
-      const float d = cancels ? top / 448.0f : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
+      const float d = cancels ? over448(top) : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
       float q[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e] * f, d, r);
