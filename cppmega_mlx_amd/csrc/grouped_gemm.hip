@@ -15,21 +15,36 @@ bool pieces_whole(const GroupedParams& p, int op, int dtype) {
   return op != kWeightsGrad || (p.w_pitch % piece == 0 && p.w_pitch <= (1 << 22));
 }
 
-// 256 x 256 tiles, one to a CU, or 128 x 128, two to a CU: by the rounds of tiles that 256 CUs are expected to take, a high one's as 1, a low one's as
-// 0.63 (for half the products), the last one less when its tiles are cut (half a tile of rows of each of several experts is padding).  Measured, us
-// high / low, rows x experts x n x k, bf16: 16384 x 32 x 4096 x 2048 329 / 380, 4096 x 1 x 4096 x 4096 120 / 139, 8192 x 64 x 2048 x 2048 185 / 159,
-// 4096 x 16 x 2048 x 2048 64 / 76, 1024 x 1 x 4096 x 4096 60 / 55, 2048 x 8 x 2048 x 4096 93 / 73; over 85 such sizes, e4m3 too, the rule's choice
-// loses 0.5 % to the better one.  Gradients of weights have as many tiles whatever the rows; few rows leave them short, and two workgroups cover each
-// other's stores: 4096 rows of 32 experts 233 / 224 (with the rows' gradient), of 8 121 / 134.
+// How often b x b tiles of a product, `at_once` at a time, are expected to go round (half a tile of rows of each of several experts is padding).
+double rounds_of(const GroupedParams& p, int op, int b, int at_once) {
+  const double across = ((op == kRows ? p.n : p.k) + b - 1) / b;
+  if (op == kWeightsGrad) return (double)p.experts * ((p.n + b - 1) / b) * across / at_once;
+  return (p.experts > 1 ? (double)p.rows / b + 0.5 * p.experts : (double)((p.rows + b - 1) / b)) * across / at_once;
+}
+
+// 256 x 256 tiles, one to a CU, or 128 x 128, two to a CU: by the rounds that 256 CUs take, a low one's as 0.63 of a high one's (for half the products).
+//   Rows: the last round counts less when its tiles are cut.  Measured, us high / low, rows x experts x n x k, bf16: 16384 x 32 x 4096 x 2048 329 / 380,
+//   4096 x 1 x 4096 x 4096 120 / 139, 8192 x 64 x 2048 x 2048 185 / 159, 4096 x 16 x 2048 x 2048 64 / 76, 1024 x 1 x 4096 x 4096 60 / 55, 2048 x 8 x 2048 x
+//   4096 93 / 73; over 85 such sizes, e4m3 too, the choice loses 0.5 % to the better one.
+//   Weights: half a round is idle at the end.  512 x 16 x 4096 x 2048 75 / 96, 8192 x 1 x 4096 x 4096 216 / 254, 1024 x 1 x 2048 x 1024 29 / 16, 2048 x 8 x 1000 x
+//   1544 31 / 20; the worst of 56 sizes 12 % (512 x 32 x 2048 x 2048 92 / 83).
 bool high_tiles(const GroupedParams& p, int op) {
-  if (op == kWeightsGrad) return p.rows >= 192ll * p.experts;
-  const int cols = op == kRows ? p.n : p.k;
   auto rounds = [&](int b, int at_once, double quarter, double half) {
-    const double high = p.experts > 1 ? (double)p.rows / b + 0.5 * p.experts : (double)((p.rows + b - 1) / b);
-    const double x = high * ((cols + b - 1) / b) / at_once, whole = (double)(long long)x, last = x - whole;
+    const double x = rounds_of(p, op, b, at_once), whole = (double)(long long)x, last = x - whole;
+    if (op == kWeightsGrad) return x > 0.5 ? x + 0.5 : 1.0;
     return whole + (last == 0.0 ? 0.0 : last <= 0.25 ? quarter : last <= 0.5 ? half : 1.0);
   };
   return rounds(256, 256, 0.5, 0.67) <= 0.63 * rounds(128, 512, 0.62, 0.62);
+}
+
+// Both gradients in one launch: whole rounds of all tiles, the rows' first and uncut.  Measured as above: 8192 x 16 x 4096 x 2048 327 / 389, 512 x 16 x 4096 x
+// 2048 126 / 162, 512 x 1 x 4096 x 4096 86 / 49, 2048 x 8 x 2048 x 4096 119 / 135, 2048 x 1 x 4096 x 4096 122 / 145 (where the rule takes the low ones).
+bool high_grads(const GroupedParams& rows, const GroupedParams& weights) {
+  auto rounds = [&](int b, int at_once) {
+    const double x = rounds_of(rows, kRowsGrad, b, at_once) + rounds_of(weights, kWeightsGrad, b, at_once), whole = (double)(long long)x;
+    return x > whole ? whole + 1.0 : whole;
+  };
+  return rounds(256, 256) <= 0.63 * rounds(128, 512);
 }
 
 // What a call runs: nothing, or one of the kernels.
@@ -102,8 +117,8 @@ int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const
   int rc = plan_of(rows, r);
   if (!rc) rc = plan_of(weights, w);
   if (rc) return rc;
-  if (r.kind == kTile && w.kind == kTile && r.high == w.high && rows.x_dtype == weights.x_dtype)
-    return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, r.high, stream);
+  if (r.kind == kTile && w.kind == kTile && rows.x_dtype == weights.x_dtype)
+    return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, high_grads(r.p, w.p), stream);
   rc = launch(r, kRowsGrad, rows.x_dtype, stream);
   return rc ? rc : launch(w, kWeightsGrad, weights.x_dtype, stream);
 }

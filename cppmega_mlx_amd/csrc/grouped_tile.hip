@@ -18,8 +18,8 @@
 // product of that size reaches 1390: at 1.3 PFLOP/s the clock is down at 1.7 GHz, power is the bound, and neither deeper rings nor other orders
 // of loads change it.  What short contractions lose: 10 to 12 us a tile for its first loads and for stores that all CUs send at once; persistent
 // workgroups with the next tile's first stages under the stores were not faster, and tiles of few rows after all others 5 % slower (the weights are
-// read twice).  Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16: 379 (725), where 320 tiles of rows meet 256 CUs and a gradient's
-// contraction is 512 rows.
+// read twice).  Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16, in one launch 329 (835); one after the other 375: the
+// rows' 320 tiles leave 192 of 512 places empty, and a gradient's contraction is 512 rows.
 // e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 510 (2150): the matrix cores are busy 0.41 of the time, the scaling's vector
 // instructions take 0.30 (one multiply-add per result and block: none to spare), wavefronts wait 0.28 of theirs, at 1.9 GHz; the multiply-adds spread
 // between single products changed nothing.

@@ -116,7 +116,7 @@ def test_many_rows(device, case):
         assert torch.equal(fresh[:rows], dx[:rows]) and (fresh[rows:] == 0).all()
 
 
-@pytest.mark.parametrize("case", MANY + [([30, 0, 90, 1], 200, 4104), ([600] * 4, 264, 1032), ([0, 0], 40, 48)], ids=lambda c: f"{sum(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+@pytest.mark.parametrize("case", MANY + [([30, 0, 90, 1], 200, 4104), ([600] * 4, 264, 1032), ([30] * 20 + [0] * 6 + [61] * 6, 1008, 1016), ([900, 0, 1, 700] + [250] * 12, 1288, 1016), ([0, 0], 40, 48)], ids=lambda c: f"{sum(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
 def test_both_gradients_are_the_ones_of_separate_calls(device, case):
     counts, k, n = case                                            # (the rows' gradient has the many columns)
     rows, tail = sum(counts), 300
@@ -126,6 +126,10 @@ def test_both_gradients_are_the_ones_of_separate_calls(device, case):
     assert torch.equal(dx, grouped_gemm_bwd(dy, x, w, offsets, need_dw=False)[0]) and torch.equal(dw, grouped_gemm_bwd(dy, x, w, offsets, need_dx=False)[1])
     _assert_near(dx[:rows], *_plain(dy[:rows], w.transpose(1, 2), offsets), n)
     assert (dx[rows:] == 0).all()
+    b = offsets.tolist()
+    for e, (lo, hi) in enumerate(zip(b, b[1:])):
+        g, v = dy[lo:hi].double().T, x[lo:hi].double()
+        _assert_near(dw[e], g @ v, g.abs() @ v.abs(), hi - lo)
     held = torch.full((rows + tail, k), 5.0, dtype=BF16, device=device), torch.full((len(counts), n, k), 5.0, device=device)
     grouped_gemm_bwd(dy, x, w, offsets, dx=held[0], dw=held[1])
     assert torch.equal(held[0][:rows], dx[:rows]) and (held[0][rows:] == 5).all() and torch.equal(held[1].to(BF16), dw)
