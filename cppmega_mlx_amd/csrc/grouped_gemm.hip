@@ -82,11 +82,12 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   p.y_dtype = a.y_dtype; p.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; p.x_scale_block = a.x_scale_block; p.zero_tail = a.zero_tail;
   to.kind = kGeneral;
   if (pieces_whole(p, a.op, a.x_dtype)) {
-    // Few rows to an expert: the kernel that streams the weights.  Measured against tiles, us, 64 experts of 2048 x 2048: 8 rows each 102 / 130
-    // (bf16) and 56 / 60 (e4m3), 12 rows 104 / 130 and 61 / 60, 16 rows 117 / 130 and 69 / 59, 24 rows 152 / 132 and 88 / 61.  (For float32
-    // results of e4m3 operands there is the general kernel instead of tiles, which takes three times as long.)
+    // Few rows to an expert: the kernel that streams the weights, 16 rows at a time.  Measured against tiles, us, rows to an expert on average (drawn
+    // at random): 64 experts of 2048 x 2048, bf16 8 96 / 129, 14 109 / 130, 20 143 / 131; of 4096 x 2048 8 184 / 185, 14 209 / 187, 20 275 / 189; e4m3 8
+    // 48 / 49 and 97 / 108, 12 51 / 49 and 104 / 109, 20 77 / 50 and 151 / 121.  float32 results of e4m3 operands have the general kernel instead of
+    // tiles: 20 78 / 136, 48 145 / 149.
     const bool exact = fp8 && a.y_dtype == CPPMEGA_MI355_F32;
-    if (a.op == kRows && a.rows < (fp8 && !exact ? 12ll : 20ll) * a.experts) {
+    if (a.op == kRows && a.rows < (exact ? 48ll : fp8 ? 12ll : 14ll) * a.experts) {
       to.kind = kStream;
     } else if (!exact) {                                         // (float32 results of e4m3 operands stay with the general kernel, whose products are exact)
       to.kind = kTile;
