@@ -8,8 +8,8 @@
 // 16 lanes.  Sums of squares, products with the weight, scales and the weight's gradient are float32; h is rounded once (it is
 // the stream that the next layer reads, so y is the norm of what is stored), y once, from its float32 value, codes from float32 as well.
 //
-// Measured with cold caches, bf16 with the residual: 8192 x 7168 82 us (5.7 TB/s; a copy of that size 4.9), e4m3 rows in blocks 74 us (4.8); 32768 x 1536
-// 72 and 63; 4 x 7168 3.3 us, a launch.  Gradients: 8192 x 7168 75 us (6.3 TB/s), 4096 x 7168 41, 32768 x 1536 70.
+// Measured in a replayed graph, inputs in turn, bf16 with the residual: 8192 x 7168 82 us (5.7 TB/s; a large copy 4.9), e4m3 rows 74 us (5.6); 32768 x 1536
+// 71 and 64; 1 x 7168 3.3 us, a launch.  Gradients: 8192 x 7168 75 us (6.3 TB/s), 4096 x 7168 41, 32768 x 1536 70.
 
 #include "common.h"
 #include "mfma_util.h"
