@@ -122,15 +122,15 @@ __device__ __forceinline__ float over448(float v) {
   const float q = v * (1.0f / 448.0f);
   return v < __builtin_inff() ? fmaf(fmaf(-448.0f, q, v), 1.0f / 448.0f, q) : q;
 }
-__device__ __forceinline__ float scale_of(float amax, bool pow2) {
-  if (!pow2) return fmaxf(over448(amax), 1.0e-12f);
-  float s = 1.0f;                              // amax = fr * 2^ex, fr in [0.5, 1): the smallest power of two with 448 s >= amax
-  if (amax > 0.0f) {
-    int ex;
-    const float fr = frexpf(amax, &ex);
-    s = ldexpf(1.0f, (ex - 1) - 8 + (fr > 0.875f ? 1 : 0));
-  }
-  return s;
+// The exponent of the smallest power of two s with 448 s >= amax: amax = fr * 2^ex, fr in [0.5, 1), and 448 = 0.875 * 2^9.  float32 has none below
+// 2^-149; no power reaches an infinite amax, whose scale is infinite like the other kind's.  0 for zeros and NaN.
+__device__ __forceinline__ int exponent_of(float amax) {
+  if (!(amax > 0.0f)) return 0;
+  if (!(amax < __builtin_inff())) return 1024;
+  int ex;
+  const float fr = frexpf(amax, &ex);
+  ex += fr > 0.875f ? -8 : -9;
+  return ex < -149 ? -149 : ex;
 }
 
 // v / s for r = 1 / s, to the last bit but for rare ties of the quotient: the remainder corrects the product.  An infinite
@@ -239,12 +239,21 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
       const int c = (i * THREADS + tid) * 8, valid = p.width - c;
       // y / scale = h w s / (max |h w| s / 448) = h w / (max |h w| / 448): without s and the roundings that come with it (8192 x 7168
       // bf16 rows: 159 codes are not those of 64 bits, 4000 with y / scale).  A scale that is rounded to a power of two or held at its least divides y itself.
-      const float top = p.scale_block ? over16<true>(am[i]) : am[0], sc = scale_of(top * s, p.pow2);
-      const bool cancels = !p.pow2 && sc > 1.0e-12f;
-      const float d = cancels ? over448(top) : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
-      float q[8];
+      const float top = p.scale_block ? over16<true>(am[i]) : am[0];
+      float q[8], sc;
+      if (p.pow2) {
+        // (by the exponent: the reciprocal of a scale of 2^-128 or less is no float32)
+        const int ex = exponent_of(top * s);
+        sc = ldexpf(1.0f, ex);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e] * f, d, r);
+        for (int e = 0; e < 8; ++e) q[e] = ldexpf(v[i][e] * s, -ex);
+      } else {
+        sc = fmaxf(over448(top * s), 1.0e-12f);
+        const bool cancels = sc > 1.0e-12f;
+        const float d = cancels ? over448(top) : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e] * f, d, r);
+      }
       const uint2 codes = make_uint2(codes4(q[0], q[1], q[2], q[3]), codes4(q[4], q[5], q[6], q[7]));
       unsigned char* const to = (unsigned char*)p.out + row * p.out_pitch + c;
       if (valid >= 8) {

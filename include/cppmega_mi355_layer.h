@@ -20,8 +20,8 @@ extern "C" {
  *   y = h / sqrt(mean(h^2) + eps) * weight,  in 32 bits, rounded once to `out`
  * out_dtype E4M3: `scale` float32 per row (scale_block 0) or per 128 channels (scale_block 128, the last
  * block may be shorter): max(amax|y| / 448, 1e-12), or with pow2_scales the smallest power of two with
- * 448 * scale >= amax (1 for a block of zeros); codes are y / scale rounded to nearest even (a NaN gives a
- * NaN code).  Rows may be up to CPPMEGA_MI355_NORM_MAX_WIDTH wide.  out may be x, residual_out may be x or
+ * 448 * scale >= amax (1 for a block of zeros; infinite for an infinite amax); codes are y / scale rounded to
+ * nearest even (a NaN gives a NaN code).  Rows may be up to CPPMEGA_MI355_NORM_MAX_WIDTH wide.  out may be x, residual_out may be x or
  * residual. */
 #define CPPMEGA_MI355_NORM_MAX_WIDTH 32768
 typedef struct cppmega_mi355_rms_norm_args {

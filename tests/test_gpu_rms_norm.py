@@ -348,3 +348,31 @@ def test_native_launch_path_and_helpers_agree(device, monkeypatch):
     monkeypatch.setattr(ops, "host", Declines())
     for a, b in zip(native, [c() for c in calls]):
         assert len(a) == len(b) and all(s.shape == t.shape and s.dtype == t.dtype and torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("block", [0, 128])
+def test_power_of_two_scales_at_the_ends_of_float32(device, dtype, block):
+    """Blocks (rows) whose largest value is next to float32's least numbers, beside ordinary ones: 448 * scale reaches it with the smallest
+    power of two, 2^-149 at least.  y = (h w) s has an absolute error of at most 2^-149 there (two roundings of 2^-150, s <= 1) beside the relative one."""
+    sizes = [1.0, 1e-30, 1e-35, 3e-36, 1e-36, 1e-37, 1e-38, 1e-40, 1e-42, 3e-44, 3e-45, 0.0]
+    for widths in ([sizes] if block else [[c] for c in sizes]):
+        x, w, _ = _inputs(device, 5, 128 * len(widths) if block else 333, dtype, F32, seed=200)
+        for i, c in enumerate(widths):
+            w[(slice(128 * i, 128 * (i + 1)) if block else slice(None))] *= c
+        codes, scale = rms_norm_fp8(x, w, scale_block=block, pow2_scales=True)
+        want, size = _plain(x, w, 1e-6), block or x.shape[1]
+        per = (scale if block else scale[:, None]).double()
+        amax = torch.stack([want[:, i:i + size].abs().amax(1) for i in range(0, x.shape[1], size)], 1)
+        least = lambda a: torch.where(a > 0, torch.exp2(torch.ceil(torch.log2(a / 448)).clamp_min(-149)), torch.ones_like(a))
+        off = amax * 40 * U + 2.0 ** -149 * (amax > 0)
+        assert ((per >= least((amax - off).clamp_min(2.0 ** -150) * (amax > 0))) & (per <= least(amax + off))).all()
+        spread = per.repeat_interleave(size, 1)[:, :x.shape[1]]
+        v, off = want / spread, 2.0 ** -149 / spread
+        slack = (v.abs() * 40 * U + off) * (1 + 1 / 16)
+        assert ((_value(codes) - v).abs() <= torch.maximum(v.abs() / 16, torch.tensor(2.0 ** -10, device=device, dtype=torch.float64)) + slack).all()
+    # no power of two reaches an infinite value: like the other scales, an infinite one, codes of 0, and NaN in its place
+    w = torch.ones(256, device=device)
+    w[130] = float("inf")
+    codes, scale = rms_norm_fp8(x[:, :256].contiguous(), w, scale_block=block, pow2_scales=True)
+    assert scale.reshape(5, -1)[:, -1].isinf().all() and _value(codes[:, 130]).isnan().all() and (_value(codes[:, 131:]) == 0).all()
