@@ -77,6 +77,9 @@ def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """y [T, N] in bfloat16 (or a caller-owned ``out``'s type: bfloat16, float16, float32).
 
+    float16 and float32 results are sums of exact products; bfloat16 ones of many rows drop, of every eight products, what lies below
+    2^-13 of the largest.
+
     ``x`` uint8 e4m3 [T, K] with float32 ``x_scale`` [T] or [T, ceil(K / 128)] (what ``rms_norm_fp8`` writes); ``w`` uint8 e4m3
     [E, N, K] with float32 ``w_scale`` [E, ceil(N / 128), ceil(K / 128)]."""
     if out is None:

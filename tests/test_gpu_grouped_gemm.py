@@ -496,3 +496,35 @@ def test_training_step_of_a_layers_second_half(device):
         assert float((got.grad.double() - want.grad).norm() / want.grad.norm()) < 20 * 2.0 ** -8
     assert torch.equal(rms_norm(leaves[0], leaves[2], residual=leaves[1])[1], (leaves[0].float() + leaves[1].float()).to(BF16))
     assert rms_norm_bwd(leaves[0], leaves[1], leaves[2])[1].dtype == F32
+
+
+# ---- float16 results of codes: sums of exact products on every kernel ------------------------------
+@pytest.mark.parametrize("counts, n, k", [([3, 0, 2], 96, 256), ([40, 0, 90, 200], 300, 640), ([40, 0, 90, 200], 77, 264), ([5000, 1, 0, 250], 520, 128)])
+@pytest.mark.parametrize("block", [0, 128])
+def test_float16_and_float32_results_of_codes_keep_small_products_beside_large_ones(device, counts, n, k, block):
+    """Of every eight products two of 448^2 cancel and six are 14: 84, a whole number on the way and at the end."""
+    offsets, rows = _offsets(counts, device), sum(counts)
+    encode = lambda v: torch.tensor(v, device=device).repeat(k // 8).to(torch.float8_e4m3fn).view(torch.uint8)
+    x = encode([448.0, 448.0, 4.0, 4.0, 4.0, 4.0, 4.0, 4.0]).expand(rows, k).contiguous()
+    w = encode([448.0, -448.0, 3.5, 3.5, 3.5, 3.5, 3.5, 3.5]).expand(len(counts), n, k).contiguous()
+    xs = torch.ones((rows, (k + 127) // 128) if block else (rows,), device=device)
+    ws = torch.full((len(counts), (n + 127) // 128, (k + 127) // 128), 0.125, device=device)
+    for dtype in (F16, F32):
+        out = torch.empty(rows, n, dtype=dtype, device=device)
+        grouped_fp8_gemm(x, xs, w, ws, offsets, out=out)
+        assert (out == k // 8 * 84 / 8).all()
+
+
+@pytest.mark.parametrize("case", CASES + MANY, ids=lambda c: f"{sum(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+@pytest.mark.parametrize("block", [0, 128])
+def test_float16_results_of_codes(device, case, block):
+    counts, n, k = case
+    offsets, rows, e = _offsets(counts, device), sum(counts), len(counts)
+    x, w = _e4m3(device, rows, k, seed=4), _e4m3(device, e, n, k, seed=5)
+    xs = _normal(device, rows, (k + 127) // 128, seed=6).exp() * 1e-2
+    if not block:
+        xs = xs[:, 0].contiguous()
+    ws = _normal(device, e, (n + 127) // 128, (k + 127) // 128, seed=7).exp() * 1e-3
+    out = torch.empty(rows, n, dtype=F16, device=device)
+    assert grouped_fp8_gemm(x, xs, w, ws, offsets, out=out) is out
+    _assert_near(out, *_plain_fp8(x, xs, w, ws, offsets), k + 4)
