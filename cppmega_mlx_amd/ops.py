@@ -909,6 +909,12 @@ def _own_rows(t: torch.Tensor, name: str, rows: int, pitch: int) -> None:
         raise ValueError(f"the rows of {name} overlap: strides {t.stride()}")
 
 
+def _written(*results: torch.Tensor | None) -> None:
+    """Tells autograd of results in caller-owned tensors, as torch's own in-place operations do: a graph that has saved one of them (the
+    stream, say) refuses its backward pass, where it would go on with the new values."""
+    torch.autograd.graph.increment_version([t for t in results if t is not None])
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float, out: torch.Tensor, residual: torch.Tensor | None = None,
              residual_out: torch.Tensor | None = None, scale: torch.Tensor | None = None, scale_block: int = 0,
              pow2_scales: bool = False) -> None:
@@ -954,6 +960,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float, out: torch.Te
     with torch.cuda.device(x.device):
         rc = _lib.load().cppmega_mi355_rms_norm(C.byref(a), C.sizeof(a), _lib.current_stream(x.device))
     _lib.check(rc, "rms_norm")
+    _written(out, residual_out, scale)
 
 
 def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *, eps: float, dx: torch.Tensor, dweight: torch.Tensor,
@@ -990,6 +997,7 @@ def rms_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, *
     with torch.cuda.device(h.device):
         rc = lib.cppmega_mi355_rms_norm_bwd(C.byref(a), C.sizeof(a), stream)
     _lib.check(rc, "rms_norm_bwd")
+    _written(dx, dweight)
 
 
 # ---------------------------------------------------------------------------
@@ -1023,10 +1031,12 @@ def _expert_weights(w: torch.Tensor, name: str, ref: torch.Tensor) -> tuple[int,
     return tuple(int(d) for d in w.shape)
 
 
-def _grouped_call(a: _lib.GroupedGemmArgs, device: torch.device) -> None:
-    with torch.cuda.device(device):
-        rc = _lib.load().cppmega_mi355_grouped_gemm(C.byref(a), C.sizeof(a), _lib.current_stream(device))
+def _grouped_call(a: _lib.GroupedGemmArgs, out: torch.Tensor) -> torch.Tensor:
+    with torch.cuda.device(out.device):
+        rc = _lib.load().cppmega_mi355_grouped_gemm(C.byref(a), C.sizeof(a), _lib.current_stream(out.device))
     _lib.check(rc, "grouped_gemm")
+    _written(out)
+    return out
 
 
 _HALF = (torch.float16, torch.bfloat16)
@@ -1071,14 +1081,12 @@ def grouped_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, out
     """out[t, n] = sum_k x[t, k] w[e(t), n, k] into caller-owned ``out``; ``transposed``: out[t, k] = sum_n x[t, n] w[e(t), n, k].
 
     Rows ``offsets[e] .. offsets[e + 1]`` belong to expert e; rows behind the last expert are left as they are, or zeroed."""
-    _grouped_call(_grouped_rows_args(x, w, offsets, out, zero_tail, transposed), x.device)
-    return out
+    return _grouped_call(_grouped_rows_args(x, w, offsets, out, zero_tail, transposed), out)
 
 
 def grouped_weights_grad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, *, out: torch.Tensor) -> torch.Tensor:
     """out[e, n, k] = sum over the rows t of expert e of dy[t, n] x[t, k] (zeros for an expert without rows)."""
-    _grouped_call(_grouped_weights_args(dy, x, offsets, out), x.device)
-    return out
+    return _grouped_call(_grouped_weights_args(dy, x, offsets, out), out)
 
 
 def grouped_gemm_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *, dx: torch.Tensor, dw: torch.Tensor,
@@ -1089,6 +1097,7 @@ def grouped_gemm_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, of
     with torch.cuda.device(dy.device):
         rc = _lib.load().cppmega_mi355_grouped_gemm_bwd(C.byref(a), C.byref(b), C.sizeof(a), _lib.current_stream(dy.device))
     _lib.check(rc, "grouped_gemm_bwd")
+    _written(dx, dw)
     return dx, dw
 
 
@@ -1121,5 +1130,4 @@ def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_
         raise ValueError(f"w_scale must have shape {(E, blocks_n, blocks_k)}; got {tuple(w_scale.shape)}")
     a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
     a.x_scale, a.w_scale = x_scale.data_ptr(), w_scale.data_ptr()
-    _grouped_call(a, x.device)
-    return out
+    return _grouped_call(a, out)

@@ -528,3 +528,18 @@ def test_float16_results_of_codes(device, case, block):
     out = torch.empty(rows, n, dtype=F16, device=device)
     assert grouped_fp8_gemm(x, xs, w, ws, offsets, out=out) is out
     _assert_near(out, *_plain_fp8(x, xs, w, ws, offsets), k + 4)
+
+
+def test_caller_owned_results_count_as_changed(device):
+    """autograd refuses a backward pass whose saved operands were overwritten, as it does after a torch operation."""
+    x, w, off = _normal(device, 9, 16, dtype=BF16), _normal(device, 2, 16, 16, dtype=BF16), _offsets([4, 5], device)
+    y = grouped_gemm_apply(x, w.requires_grad_(), off)
+    grouped_gemm(_normal(device, 9, 16, dtype=BF16, seed=1), w.detach(), off, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    w = w.detach()
+    dx, dw, other, out = torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(w), torch.zeros_like(x)
+    before = [t._version for t in (dx, dw, other, out)]
+    grouped_gemm_bwd(x, x, w, off, dx=dx, dw=dw), grouped_gemm_bwd(x, x, w, off, dw=other, need_dx=False)
+    grouped_fp8_gemm(x.to(torch.uint8), torch.ones(9, device=device), w.to(torch.uint8), torch.ones(2, 1, 1, device=device), off, out=out)
+    assert all(t._version > v for t, v in zip((dx, dw, other, out), before))

@@ -376,3 +376,19 @@ def test_power_of_two_scales_at_the_ends_of_float32(device, dtype, block):
     w[130] = float("inf")
     codes, scale = rms_norm_fp8(x[:, :256].contiguous(), w, scale_block=block, pow2_scales=True)
     assert scale.reshape(5, -1)[:, -1].isinf().all() and _value(codes[:, 130]).isnan().all() and (_value(codes[:, 131:]) == 0).all()
+
+
+def test_caller_owned_results_count_as_changed(device):
+    """autograd refuses a backward pass whose saved rows were overwritten, as it does after a torch operation."""
+    x, w, r = _inputs(device, 4, 96, BF16, seed=210)
+    x.requires_grad_()
+    y, h = rms_norm_apply(x, w, r)
+    rms_norm(r, w, residual=r, residual_out=h.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    a, codes, scale, dx, dw = (torch.zeros(s, dtype=t, device=device) for s, t in (((4, 96), BF16), ((4, 96), torch.uint8), ((4,), F32), ((4, 96), BF16), ((96,), F32)))
+    before = [t._version for t in (a, codes, scale, dx, dw)]
+    rms_norm(r, w, out=a), rms_norm_fp8(r, w, codes=codes, scale=scale), rms_norm_bwd(r, r, w, dx=dx, dweight=dw)
+    assert all(t._version > v for t, v in zip((a, codes, scale, dx, dw), before))
+    with torch.inference_mode():
+        assert rms_norm(r, w, out=torch.zeros_like(r)).shape == r.shape
