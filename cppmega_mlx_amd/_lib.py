@@ -70,6 +70,7 @@ LAYER_SYMBOLS = (
 )
 NORM_MAX_WIDTH = 32768                # CPPMEGA_MI355_NORM_MAX_WIDTH
 GROUPED_MAX_EXPERTS = 512             # CPPMEGA_MI355_GROUPED_MAX_EXPERTS
+GROUPED_MAX_SIZE = 1 << 30            # CPPMEGA_MI355_GROUPED_MAX_SIZE
 # operations of the grouped products
 GROUPED_ROWS, GROUPED_ROWS_GRAD, GROUPED_WEIGHTS_GRAD = range(3)
 

@@ -60,6 +60,9 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: unknown op %d", a.op);
   if (a.rows < 0 || a.rows > 0x1fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
     return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
+  // (columns and contraction are counted in 32 bits, a tile past the end)
+  if (a.n > CPPMEGA_MI355_GROUPED_MAX_SIZE || a.k > CPPMEGA_MI355_GROUPED_MAX_SIZE)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: n=%d k=%d, at most 2^30 are served", a.n, a.k);
   if (a.experts > kMaxExperts) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %d experts, at most %d are served", a.experts, kMaxExperts);
   const bool fp8 = a.x_dtype == CPPMEGA_MI355_E4M3;
   if (!fp8 && a.x_dtype != CPPMEGA_MI355_F16 && a.x_dtype != CPPMEGA_MI355_BF16)

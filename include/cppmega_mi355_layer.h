@@ -87,6 +87,7 @@ int cppmega_mi355_rms_norm_bwd(const cppmega_mi355_rms_norm_bwd_args_t* args, si
  * Rows of y from offsets[experts] on are left as they were, or zeroed with zero_tail. */
 enum { CPPMEGA_MI355_GROUPED_ROWS = 0, CPPMEGA_MI355_GROUPED_ROWS_GRAD = 1, CPPMEGA_MI355_GROUPED_WEIGHTS_GRAD = 2 };
 #define CPPMEGA_MI355_GROUPED_MAX_EXPERTS 512
+#define CPPMEGA_MI355_GROUPED_MAX_SIZE 1073741824   /* of n and of k */
 
 typedef struct cppmega_mi355_grouped_gemm_args {
   uint32_t struct_size;

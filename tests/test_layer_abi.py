@@ -160,3 +160,18 @@ def test_row_pitch_of_views(make, want):
 def test_row_pitch_refuses_what_would_need_a_copy(make, what):
     with pytest.raises(ValueError, match=what):
         _lib.row_pitch(make(torch.zeros(4, 6, 8)), "t")
+
+
+@pytest.mark.parametrize("op", [0, 1, 2])
+@pytest.mark.parametrize("name", ["n", "k"])
+def test_grouped_sizes_that_the_kernels_cannot_count_are_refused(op, name):
+    """Column and contraction counters are 32 bits wide and run a tile past the end."""
+    for size in ((1 << 31) - 1, (1 << 31) - 64, _lib.GROUPED_MAX_SIZE + 1):
+        a = _lib.GroupedGemmArgs()
+        a.struct_size, a.op = C.sizeof(a), op
+        a.x = a.w = a.y = a.offsets = FAKE
+        a.x_dtype = a.y_dtype = _lib.BF16
+        a.offsets_dtype = _lib.I32
+        a.rows, a.experts, a.n, a.k, a.x_pitch, a.y_pitch, a.w_pitch = 1, 1, 1, 1, 1, 1, 1
+        setattr(a, name, size)
+        assert _lib.load().cppmega_mi355_grouped_gemm(C.byref(a), C.sizeof(a), None) == _lib.ERR_SHAPE
