@@ -888,6 +888,8 @@ def mask_sparse_indices(mask: torch.Tensor, out: torch.Tensor, *, topk: int) -> 
 # RMS norm of the residual stream
 # ---------------------------------------------------------------------------
 def _norm_weight(weight: torch.Tensor, x: torch.Tensor) -> None:
+    if x.shape[-1] > _lib.NORM_MAX_WIDTH:                  # (here: the argument block holds 32 bits of it)
+        raise ValueError(f"rows of width {x.shape[-1]}: at most {_lib.NORM_MAX_WIDTH} are served")
     _lib.require_device_tensor(weight, "weight", x)
     if tuple(weight.shape) != (x.shape[-1],):
         raise ValueError(f"weight must have shape {(x.shape[-1],)}; got {tuple(weight.shape)}")
@@ -1011,6 +1013,8 @@ def _grouped_args(op: int, x: torch.Tensor, offsets: torch.Tensor, experts: int,
     a.offsets_dtype = _dtype_or_raise(offsets, "offsets", (_lib.I32, _lib.I64))
     if tuple(offsets.shape) != (experts + 1,):
         raise ValueError(f"offsets must have shape {(experts + 1,)} for {experts} experts; got {tuple(offsets.shape)}")
+    if max(experts, n, k) > _lib.GROUPED_MAX_SIZE:         # (here: the argument block holds 32 bits of them)
+        raise ValueError(f"{experts} experts, n={n}, k={k}: at most 2^30 are served")
     a.offsets = offsets.data_ptr()
     a.x_dtype = _lib.dtype_code(x)
     a.rows, a.experts, a.n, a.k = x.shape[0], experts, n, k

@@ -543,3 +543,20 @@ def test_caller_owned_results_count_as_changed(device):
     grouped_gemm_bwd(x, x, w, off, dx=dx, dw=dw), grouped_gemm_bwd(x, x, w, off, dw=other, need_dx=False)
     grouped_fp8_gemm(x.to(torch.uint8), torch.ones(9, device=device), w.to(torch.uint8), torch.ones(2, 1, 1, device=device), off, out=out)
     assert all(t._version > v for t, v in zip((dx, dw, other, out), before))
+
+
+def test_sizes_beyond_the_kernels_counters_are_refused(device):
+    x, off = torch.zeros(1, 1, dtype=BF16, device=device), _offsets([1], device)
+    wide = torch.empty((1 << 32) + 64, dtype=BF16, device=device)
+    codes, one = wide.view(torch.uint8)[:(1 << 32) + 64], torch.ones(1, device=device)
+    for call in (lambda: grouped_gemm(x, wide.view(1, -1, 1), off), lambda: grouped_gemm(wide.view(1, -1), wide.view(1, 1, -1), off),
+                 lambda: grouped_gemm_bwd(wide.view(1, -1), x, wide.view(1, -1, 1), off), lambda: grouped_gemm_bwd(x, wide.view(1, -1), wide.view(1, 1, -1), off, need_dx=False),
+                 lambda: grouped_fp8_gemm(x.to(torch.uint8), one, codes.view(1, -1, 1), torch.ones(1, ((1 << 32) + 64) // 128 + 1, 1, device=device), off)):
+        with pytest.raises(ValueError, match="2\\^30"):
+            call()
+    n, k = (1 << 30) - 64, 8                                        # (the last size of one row that a launch has tiles for)
+    w = wide[:n].view(1, n, 1).expand(1, n, k).contiguous()
+    w[0, -200:] = _normal(device, 200, k, dtype=BF16, seed=90)
+    x = _normal(device, 1, k, dtype=BF16, seed=91)
+    y = grouped_gemm(x, w, off)
+    _assert_near(y[:, -200:], *_plain(x, w[:, -200:], off), k)

@@ -392,3 +392,10 @@ def test_caller_owned_results_count_as_changed(device):
     assert all(t._version > v for t, v in zip((a, codes, scale, dx, dw), before))
     with torch.inference_mode():
         assert rms_norm(r, w, out=torch.zeros_like(r)).shape == r.shape
+
+
+def test_widths_beyond_32_bits_are_refused(device):
+    x = torch.empty(1, (1 << 32) + 64, dtype=BF16, device=device)
+    for call in (lambda: rms_norm(x, x[0]), lambda: rms_norm_fp8(x, x[0], scale_block=128), lambda: rms_norm_bwd(x, x, x[0])):
+        with pytest.raises(ValueError, match="width"):
+            call()
