@@ -399,3 +399,33 @@ def test_widths_beyond_32_bits_are_refused(device):
     for call in (lambda: rms_norm(x, x[0]), lambda: rms_norm_fp8(x, x[0], scale_block=128), lambda: rms_norm_bwd(x, x, x[0])):
         with pytest.raises(ValueError, match="width"):
             call()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype, wdtype", [(F16, F16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("block", [0, 128])
+@pytest.mark.parametrize("pow2", [False, True])
+def test_codes_of_every_type(device, shape, dtype, wdtype, block, pow2):
+    """float16 rows, and 16-bit rows with a float32 weight: the bounds of bfloat16 and float32 rows (h is exact in the comparison, the rest is float32)."""
+    x, w, r = _inputs(device, *shape, dtype, wdtype, seed=9)
+    codes, scale, h = rms_norm_fp8(x, w, eps=1e-6, residual=r, scale_block=block, pow2_scales=pow2)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    alone = rms_norm_fp8(h, w, eps=1e-6, scale_block=block, pow2_scales=pow2)
+    assert torch.equal(alone[0], codes) and torch.equal(alone[1], scale)
+    want, n, size = _plain(h, w, 1e-6), shape[1], block or shape[1]
+    per = (scale if block else scale[:, None]).double()
+    amax = torch.stack([want[:, i:i + size].abs().amax(1) for i in range(0, n, size)], 1)
+    if pow2:
+        least = lambda a: torch.exp2(torch.ceil(torch.log2(a / 448)))
+        assert ((per >= least(amax * (1 - 40 * U))) & (per <= least(amax * (1 + 40 * U)))).all()
+    else:
+        assert ((per - amax / 448).abs() <= amax / 448 * 37 * U).all()
+    v = want / per.repeat_interleave(size, 1)[:, :n]
+    assert ((_value(codes) - v).abs() <= torch.maximum(v.abs() / 16, torch.tensor(2.0 ** -10, device=device, dtype=torch.float64)) + v.abs() * 43 * U).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES + [(513, 96), (2500, 64), (1027, 5000), (2049, 1000)])
+@pytest.mark.parametrize("dtype, wdtype", [(BF16, F32), (F16, F16)])
+@pytest.mark.parametrize("past", [False, True])
+def test_gradients_of_every_type(device, shape, dtype, wdtype, past):
+    test_gradients(device, shape, dtype, wdtype, past)
