@@ -237,8 +237,9 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = (i * THREADS + tid) * 8, valid = p.width - c;
-      // y / scale = h w s / (max |h w| s / 448) = h w / (max |h w| / 448): without s and the roundings that come with it (8192 x 7168
-      // bf16 rows: 159 codes are not those of 64 bits, 4000 with y / scale).  A scale that is rounded to a power of two or held at its least divides y itself.
+      // y / scale = h w s / (max |h w| s / 448) = 448 h w / max |h w|: without s and the roundings that come with it, and for bf16, whose products and
+      // their 448 times are exact, with one rounding in all, so that a tie stays one (8192 x 7168 bf16 rows: every code is that of 64 bits; 159 of 59
+      // million are not with the largest over 448 as the divisor, 4000 with y / scale).  A scale that is rounded to a power of two or held at its least divides y itself.
       const float top = p.scale_block ? over16<true>(am[i]) : am[0];
       float q[8], sc;
       if (p.pow2) {
@@ -249,8 +250,8 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_kernel
         for (int e = 0; e < 8; ++e) q[e] = ldexpf(v[i][e] * s, -ex);
       } else {
         sc = fmaxf(over448(top * s), 1.0e-12f);
-        const bool cancels = sc > 1.0e-12f;
-        const float d = cancels ? over448(top) : sc, r = 1.0f / d, f = cancels ? 1.0f : s;
+        const bool cancels = sc > 1.0e-12f && top < 0x1p119f;    // (448 h w is finite)
+        const float d = cancels ? top : sc, r = 1.0f / d, f = cancels ? 448.0f : s;
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = quotient(v[i][e] * f, d, r);
       }

@@ -429,3 +429,16 @@ def test_codes_of_every_type(device, shape, dtype, wdtype, block, pow2):
 @pytest.mark.parametrize("past", [False, True])
 def test_gradients_of_every_type(device, shape, dtype, wdtype, past):
     test_gradients(device, shape, dtype, wdtype, past)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("block", [0, 128])
+def test_codes_in_the_middle_between_two_go_to_the_even_one(device, dtype, block):
+    """y / scale = 448 h / max |h| whatever the row's factor: 3 / 64 of the largest are 21, between the codes 20 and 22, and 3 / 32 are 42."""
+    top = torch.arange(1, 86, 2, device=device).float()[:, None]
+    for n in (128, 640, 2048):
+        x = torch.zeros(top.shape[0], n, device=device)
+        x[:, 0::128], x[:, 1::128], x[:, 2::128] = top, top * (3 / 64), -top * (3 / 32)
+        codes, scale = rms_norm_fp8(x.to(dtype), torch.ones(n, dtype=dtype, device=device), eps=1e-6, scale_block=block)
+        v = _value(codes)
+        assert (v[:, 0::128] == 448).all() and (v[:, 1::128] == 20).all() and (v[:, 2::128] == -40).all() and (v[:, 3:128] == 0).all()
