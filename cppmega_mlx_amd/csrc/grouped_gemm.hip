@@ -88,7 +88,9 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
     // Few rows to an expert: the kernel that streams the weights, 16 rows at a time.  Measured against tiles, us, rows to an expert on average (drawn
     // at random): 64 experts of 2048 x 2048, bf16 8 96 / 129, 14 109 / 130, 20 143 / 131; of 4096 x 2048 8 184 / 185, 14 209 / 187, 20 275 / 189; e4m3 8
     // 48 / 49 and 97 / 108, 12 51 / 49 and 104 / 109, 20 77 / 50 and 151 / 121.  float16 and float32 results of e4m3
-    // operands have the general kernel instead of tiles: 20 78 / 136, 48 145 / 149.
+    // operands have the general kernel instead of tiles: 20 78 / 136, 48 145 / 149.  The offsets stay on the device, so the rule knows the mean only:
+    // with all rows in one expert of 64 its weights are read once for every 16 of them (4096 x 2048 bf16, 890 rows: 128 us, where the tiles take 30 and an
+    // even call 186), with half of them there the call takes 239.
     const bool exact = fp8 && a.y_dtype != CPPMEGA_MI355_BF16;
     if (a.op == kRows && a.rows < (exact ? 48ll : fp8 ? 12ll : 14ll) * a.experts) {
       to.kind = kStream;

@@ -2,7 +2,8 @@
 // bytes, and float16 and float32 results of e4m3 operands (as bfloat16, whose products are exact).  The aligned kernels let the load unit write to LDS,
 // which wants whole 16-byte pieces; here a piece goes through registers, by one (unaligned) load where it is whole and element by element
 // at the end of a row.  Bound by those loads: a step's wait for the one before it.  Measured, 16384 rows of 32 experts, 4096 x 2049 bf16:
-// 597 us (461 TFLOP/s; 2048: 313 by the aligned tiles), both gradients 1610; e4m3 into float32, 4096 x 2048: 642 (into bfloat16 164).
+// 597 us (461 TFLOP/s; 2048: 313 by the aligned tiles), both gradients 1610; 4097 x 2048, whose forward the tiles take (326), both gradients 1315;
+// e4m3 into float16 or float32, 4096 x 2048: 642 (into bfloat16 164).
 //
 // One workgroup of four wavefronts per 128 x 128 tile, 128 bytes of contraction a step (one scale block of e4m3), the next
 // step's pieces on their way under the products of this one.  Pieces are 16 bytes; in LDS

@@ -23,9 +23,9 @@
 // workgroups with the next tile's first stages under the stores were not faster, and tiles of few rows after all others 5 % slower (the weights are
 // read twice).  Both gradients, 8192 rows of 16 experts, 4096 x 2048 bf16, in one launch 329 (835); one after the other 375: the
 // rows' 320 tiles leave 192 of 512 places empty, and a gradient's contraction is 512 rows.
-// e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 510 (2150): the matrix cores are busy 0.41 of the time, the scaling's vector
-// instructions take 0.30 (one multiply-add per result and block: none to spare), wavefronts wait 0.28 of theirs, at 1.9 GHz; the multiply-adds spread
-// between single products changed nothing.
+// e4m3, 4096 x 7168 of 32 experts 600 (1600), 4096 x 8192 of one 510 (2150): of a SIMD's cycles the products take 0.41 and the scaling's multiply-adds
+// (one per result and block: none to spare) 0.30, at 1.9 GHz; its two wavefronts could be at the one and the other at once, but pass the same barriers and
+// do the same at the same time (a wavefront waits 0.28 of its own cycles).  The multiply-adds spread between single products changed nothing.
 
 #include <type_traits>
 

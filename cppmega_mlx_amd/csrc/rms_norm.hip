@@ -284,7 +284,8 @@ struct NormBwdParams {
 
 // Group g of THREADS threads takes rows g, g + groups, ..; its sums for the weight stay in registers until its last row and go
 // to partial[g].  TWICE: rows too wide for the registers of 1024 threads beside those sums are read again (from the caches) for
-// their second use.
+// their second use.  Above 16384 channels a thread's sums of 32 channels do not fit all the same (48 to 252 bytes a lane go to memory):
+// 2048 x 32768 bf16 139 us (2.9 TB/s), float32 383; of 16384 channels 44 and 104.
 template <int DT, bool WF32, int THREADS, int PER, bool TWICE>
 __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_norm_bwd_kernel(const NormBwdParams p) {
   typedef typename Elem<DT>::type T;
@@ -422,7 +423,8 @@ __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float* par
 }
 
 // Groups of the gradient kernel: four rows each, so that their partial sums (float32, written and read) stay below the rows' traffic, but
-// a workgroup for every CU at least, and at most 1024 threads of them to a CU (512 of narrow rows).  Measured, us with 256 / 512 / 1024 groups:
+// 256 at least (a workgroup for every CU; of rows of up to 1024 channels, four groups to a workgroup, for a quarter of them: 1024 x 1024 bf16
+// take 10 us, 4096 x 1024 14), and at most 1024 threads of them to a CU (512 of narrow rows).  Measured, us with 256 / 512 / 1024 groups:
 // 512 x 7168 14 / 17 / 17, 2048 x 4096 22 / 18 / 21, 8192 x 4096 61 / 44 / 42, 4096 x 7168 50 / 41 / 48, 2048 x 16384 54 / 59 / 71.
 int bwd_groups(long long rows, int width) {
   const long long most = width <= 1024 ? 2048 : width <= 4096 ? 1024 : width <= 8192 ? 512 : 256;

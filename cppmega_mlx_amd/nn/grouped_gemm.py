@@ -3,14 +3,14 @@
 ``x [T, K]`` holds the rows sorted by expert: rows ``offsets[e] .. offsets[e + 1] - 1`` belong to expert e.  ``offsets`` is an int32 or
 int64 device tensor ``[E + 1]`` that begins with 0, does not decrease and ends with T at most; it is read by the kernels
 on the stream (no read-back: calls can be captured into graphs, and replayed with other offsets).  ``w [E, N, K]`` is dense, the contraction
-index contiguous as in ``ops.head_gemm``; up to 512 experts.
+index contiguous as in ``ops.head_gemm``; up to 512 experts, fewer than 2^29 rows, N and K up to 2^30.
 
     grouped_gemm        y[t, n] = sum_k x[t, k] w[e(t), n, k]             float16 / bfloat16, float32 sums, rounded once
     grouped_gemm_bwd    dx[t, k] = sum_n dy[t, n] w[e(t), n, k],  dw[e, n, k] = sum_{t in e} dy[t, n] x[t, k]
     grouped_fp8_gemm    the same product of e4m3 rows and block-128 e4m3 weights, every 128-channel block scaled in float32
 
 Experts without rows cost nothing (their ``dw`` is zeros).  Rows behind the last expert's: zeros in an output made here, left as
-they were in a caller-owned one, which must not overlap the operands.  Rows may have a pitch of their own; sizes of any kind are served, rows that begin on 16 bytes
+they were in a caller-owned one, which must not overlap the operands (and makes a graph that has saved it refuse its backward pass).  Rows may have a pitch of their own; sizes of any kind are served, rows that begin on 16 bytes
 by faster kernels.  ``grouped_gemm_apply`` is the differentiable form; a backward pass that is to be captured into a graph must not share its
 leaves with an eager autograd graph that is still alive: capture ``grouped_gemm_bwd``, or drop the eager graph first.
 

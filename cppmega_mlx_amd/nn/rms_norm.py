@@ -4,12 +4,17 @@
     y = h / sqrt(mean(h^2) + eps) * weight      in float32, rounded once
 
 Rows are ``x[..., n]`` in float32 / float16 / bfloat16, n up to 32768, with a row pitch of their own; ``weight`` is ``[n]`` in the
-rows' type or float32.  Outputs may be caller-owned: ``out`` may be ``x``, ``residual_out`` may be ``x`` or ``residual``.  A row
-with NaN or infinities gives NaN, a row of zeros gives zeros for ``eps > 0``.
+rows' type or float32.  Outputs may be caller-owned: ``out`` may be ``x``, ``residual_out`` may be ``x`` or ``residual``; otherwise they
+must not overlap what the call reads.  Writing into a tensor that autograd has saved makes that graph refuse its backward pass.
+
+A row of zeros gives zeros for ``eps > 0``, a row with a NaN is NaN throughout; with an infinity it is NaN in that channel and zeros in the
+others.  Squares and their sum are float32: a row whose sum leaves its range (a root mean square beyond 1.8e19 / sqrt(n)) gives zeros, and
+``eps`` has to carry rows below 1e-19.
 
 ``rms_norm_fp8`` writes e4m3 codes and float32 scales in the layouts of ``SparseFP8KVCache`` and the FP8 projections:
 one scale a row (``scale_block=0``) or per 128 channels (``scale_block=128``, the last block may be shorter), the codes taken from
-the float32 values.  ``rms_norm_bwd`` gives the gradients of the rows and of the weight, ``rms_norm_apply`` is the
+the float32 values.  A row with a NaN has NaN codes throughout, beside scales of 1e-12
+(1 with ``pow2_scales``).  ``rms_norm_bwd`` gives the gradients of the rows and of the weight, ``rms_norm_apply`` is the
 differentiable form.  A backward pass that is to be captured into a graph must not share its leaves with an eager autograd graph
 that is still alive (torch then synchronises with the eager stream inside the capture); capture ``rms_norm_bwd``, or drop
 the eager graph first.

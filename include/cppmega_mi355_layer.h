@@ -21,8 +21,9 @@ extern "C" {
  * out_dtype E4M3: `scale` float32 per row (scale_block 0) or per 128 channels (scale_block 128, the last
  * block may be shorter): max(amax|y| / 448, 1e-12), or with pow2_scales the smallest power of two with
  * 448 * scale >= amax (1 for a block of zeros; infinite for an infinite amax); codes are y / scale rounded to
- * nearest even (a NaN gives a NaN code).  Rows may be up to CPPMEGA_MI355_NORM_MAX_WIDTH wide.  out may be x, residual_out may be x or
- * residual. */
+ * nearest even (a NaN gives a NaN code; a row with one has scales of 1e-12, or 1).  Rows may be up to
+ * CPPMEGA_MI355_NORM_MAX_WIDTH wide.  out may be x, residual_out may be x or residual; otherwise outputs must not
+ * overlap the inputs.  Squares and their sum are float32. */
 #define CPPMEGA_MI355_NORM_MAX_WIDTH 32768
 typedef struct cppmega_mi355_rms_norm_args {
   uint32_t struct_size;

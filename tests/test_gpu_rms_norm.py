@@ -296,6 +296,7 @@ def test_second_derivatives_are_refused(device):
         g.sum().backward()
 
 
+# (the workspace is the call's own, so one per stream at least)
 def test_two_streams_at_once(device):
     """The gradient's workspace is one per stream."""
     sets = [(_normal(device, 3000, 2048, dtype=BF16, seed=140 + i), _inputs(device, 3000, 2048, BF16, seed=150 + i)) for i in range(2)]
