@@ -74,6 +74,17 @@ GROUPED_MAX_SIZE = 1 << 30            # CPPMEGA_MI355_GROUPED_MAX_SIZE
 # operations of the grouped products
 GROUPED_ROWS, GROUPED_ROWS_GRAD, GROUPED_WEIGHTS_GRAD = range(3)
 
+# include/cppmega_mi355_ffn.h
+FFN_SYMBOLS = (
+    "cppmega_mi355_gated_gemm",
+    "cppmega_mi355_gated_gemm_bwd_workspace_bytes",
+    "cppmega_mi355_gated_gemm_bwd",
+    "cppmega_mi355_w4_gemm",
+)
+GATED_MAX_OUTPUTS = 1 << 29           # CPPMEGA_MI355_GATED_MAX_OUTPUTS
+# activations of the gated block
+GATE_NONE, GATE_SILU, GATE_GELU_TANH = -1, 0, 1
+
 
 class NativeLibraryError(RuntimeError):
     """The HIP library is missing, stale or unusable."""
@@ -456,6 +467,91 @@ class GroupedGemmArgs(C.Structure):
     ]
 
 
+class GatedGemmArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("activation", C.c_int32),
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("y", C.c_void_p),
+        ("pre", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("x_scale", C.c_void_p),
+        ("w_scale", C.c_void_p),
+        ("x_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("pre_dtype", C.c_int32),
+        ("offsets_dtype", C.c_int32),
+        ("rows", C.c_int64),
+        ("x_pitch", C.c_int64),
+        ("y_pitch", C.c_int64),
+        ("pre_pitch", C.c_int64),
+        ("experts", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("x_scale_block", C.c_int32),
+        ("zero_tail", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class GatedGemmBwdArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("activation", C.c_int32),
+        ("dy", C.c_void_p),
+        ("pre", C.c_void_p),
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("pre_dtype", C.c_int32),
+        ("dx_dtype", C.c_int32),
+        ("dw_dtype", C.c_int32),
+        ("offsets_dtype", C.c_int32),
+        ("zero_tail", C.c_int32),
+        ("rows", C.c_int64),
+        ("dy_pitch", C.c_int64),
+        ("pre_pitch", C.c_int64),
+        ("x_pitch", C.c_int64),
+        ("dx_pitch", C.c_int64),
+        ("experts", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("reserved", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class W4GemmArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("activation", C.c_int32),
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("y", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("x_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("scale_dtype", C.c_int32),
+        ("offsets_dtype", C.c_int32),
+        ("rows", C.c_int64),
+        ("x_pitch", C.c_int64),
+        ("y_pitch", C.c_int64),
+        ("experts", C.c_int32),
+        ("n", C.c_int32),
+        ("k", C.c_int32),
+        ("group", C.c_int32),
+        ("zero_tail", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
 _lock = threading.RLock()
 _lib: C.CDLL | None = None
 
@@ -479,7 +575,7 @@ def load() -> C.CDLL:
             lib = C.CDLL(str(LIB_PATH))
         except OSError as exc:
             raise NativeLibraryError(f"cannot load {LIB_PATH}: {exc}") from exc
-        missing = [name for name in EXPORTED_SYMBOLS + LAYER_SYMBOLS if not hasattr(lib, name)]
+        missing = [name for name in EXPORTED_SYMBOLS + LAYER_SYMBOLS + FFN_SYMBOLS if not hasattr(lib, name)]
         if missing:
             raise NativeLibraryError(f"{LIB_PATH} does not export {missing}; rebuild it")
         lib.cppmega_mi355_status.argtypes = [C.POINTER(StatusStruct), C.c_size_t]
@@ -528,13 +624,16 @@ def load() -> C.CDLL:
             fn.argtypes = [C.POINTER(struct), C.c_size_t, C.c_void_p]
             fn.restype = C.c_int
         for fn, struct in ((lib.cppmega_mi355_rms_norm, RmsNormArgs), (lib.cppmega_mi355_rms_norm_bwd, RmsNormBwdArgs),
-                           (lib.cppmega_mi355_grouped_gemm, GroupedGemmArgs)):
+                           (lib.cppmega_mi355_grouped_gemm, GroupedGemmArgs), (lib.cppmega_mi355_gated_gemm, GatedGemmArgs),
+                           (lib.cppmega_mi355_gated_gemm_bwd, GatedGemmBwdArgs), (lib.cppmega_mi355_w4_gemm, W4GemmArgs)):
             fn.argtypes = [C.POINTER(struct), C.c_size_t, C.c_void_p]
             fn.restype = C.c_int
         lib.cppmega_mi355_grouped_gemm_bwd.argtypes = [C.POINTER(GroupedGemmArgs), C.POINTER(GroupedGemmArgs), C.c_size_t, C.c_void_p]
         lib.cppmega_mi355_grouped_gemm_bwd.restype = C.c_int
         lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.argtypes = [C.POINTER(RmsNormBwdArgs), C.c_size_t, C.POINTER(C.c_size_t)]
         lib.cppmega_mi355_rms_norm_bwd_workspace_bytes.restype = C.c_int
+        lib.cppmega_mi355_gated_gemm_bwd_workspace_bytes.argtypes = [C.POINTER(GatedGemmBwdArgs), C.c_size_t, C.POINTER(C.c_size_t)]
+        lib.cppmega_mi355_gated_gemm_bwd_workspace_bytes.restype = C.c_int
         lib.cppmega_mi355_fp8_vecmat_workspace_bytes.argtypes = [
             C.POINTER(VecmatArgs), C.c_size_t, C.POINTER(C.c_size_t)]
         lib.cppmega_mi355_fp8_vecmat_workspace_bytes.restype = C.c_int

@@ -47,6 +47,10 @@ int rms_norm_bwd_launch(const cppmega_mi355_rms_norm_bwd_args_t& a, hipStream_t 
 int rms_norm_bwd_workspace_bytes(const cppmega_mi355_rms_norm_bwd_args_t& a, size_t* bytes);
 int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream);
 int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream);
+int gated_gemm_launch(const cppmega_mi355_gated_gemm_args_t& a, hipStream_t stream);
+int gated_gemm_bwd_launch(const cppmega_mi355_gated_gemm_bwd_args_t& a, hipStream_t stream);
+int gated_gemm_bwd_workspace_bytes(const cppmega_mi355_gated_gemm_bwd_args_t& a, size_t* bytes);
+int w4_gemm_launch(const cppmega_mi355_w4_gemm_args_t& a, hipStream_t stream);
 int indexer_topk_launch(const cppmega_mi355_indexer_args_t& a, hipStream_t stream);
 int indexer_topk_workspace_bytes(const cppmega_mi355_indexer_args_t& a, size_t* bytes);
 
@@ -425,6 +429,27 @@ int cppmega_mi355_grouped_gemm_bwd(const cppmega_mi355_grouped_gemm_args_t* rows
   CM_CHECK_ARGS(rows, args_size, cppmega_mi355_grouped_gemm_args_t);
   CM_CHECK_ARGS(weights, args_size, cppmega_mi355_grouped_gemm_args_t);
   return grouped_gemm_bwd_launch(*rows, *weights, (hipStream_t)stream);
+}
+
+int cppmega_mi355_gated_gemm(const cppmega_mi355_gated_gemm_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_gated_gemm_args_t);
+  return gated_gemm_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_gated_gemm_bwd_workspace_bytes(const cppmega_mi355_gated_gemm_bwd_args_t* args, size_t args_size, size_t* bytes) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_gated_gemm_bwd_args_t);
+  if (!bytes) return fail(CPPMEGA_MI355_ERR_NULL, "bytes is NULL");
+  return gated_gemm_bwd_workspace_bytes(*args, bytes);
+}
+
+int cppmega_mi355_gated_gemm_bwd(const cppmega_mi355_gated_gemm_bwd_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_gated_gemm_bwd_args_t);
+  return gated_gemm_bwd_launch(*args, (hipStream_t)stream);
+}
+
+int cppmega_mi355_w4_gemm(const cppmega_mi355_w4_gemm_args_t* args, size_t args_size, void* stream) {
+  CM_CHECK_ARGS(args, args_size, cppmega_mi355_w4_gemm_args_t);
+  return w4_gemm_launch(*args, (hipStream_t)stream);
 }
 
 }  // extern "C"

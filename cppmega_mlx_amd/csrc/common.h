@@ -4,7 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "../../include/cppmega_mi355_layer.h"
+#include "../../include/cppmega_mi355_ffn.h"
 
 namespace cm {
 

@@ -9,7 +9,7 @@
 #pragma once
 
 #include "common.h"
-#include "mfma_util.h"
+#include "gate.h"
 
 namespace cm {
 
@@ -24,12 +24,17 @@ struct GroupedParams {
   long long rows, x_pitch, w_pitch, y_pitch;
   int experts, n, k;
   int y_dtype, offsets64, x_scale_block, zero_tail;
+  // the gated block: w is [experts, 2 n, k]; a tile's columns are as many of the gate's as of the up projection's
+  int activation, pre_dtype;
+  void* pre;
+  long long pre_pitch;
 };
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // Rows of expert e.  Offsets are what the device holds: they are brought into [0, rows], so that no kernel reads or writes outside.
 __device__ __forceinline__ long long offset_of(const GroupedParams& p, int e) {
+  if (!p.offsets) return e == 0 ? 0 : p.rows;                   // (one expert has all rows)
   const long long o = p.offsets64 ? ((const long long*)p.offsets)[e] : (long long)((const int*)p.offsets)[e];
   return o < 0 ? 0 : (o > p.rows ? p.rows : o);
 }
@@ -71,14 +76,43 @@ __device__ __forceinline__ int expert_of_tile(const GroupedParams& p, const int*
   return __builtin_amdgcn_readfirstlane(found - 1);
 }
 
+// Tiles of BM rows of all experts in a row, found by every wavefront for itself (a scan over the counts in registers): which expert tile mt
+// belongs to (p.experts: the rows behind them, to be zeroed), its first row and how many rows are there from it on.  false: no such tile.
+template <int BM>
+__device__ __forceinline__ bool rows_of_tile(const GroupedParams& p, int mt, int& e, int& first, int& rows) {
+  const int lane = lane_id();
+  e = -1; first = 0; rows = 0;
+  for (int e0 = 0, before = 0; e0 <= p.experts; e0 += 64) {
+    const int x = e0 + lane;
+    int lo = 0, count = 0;
+    if (x <= p.experts) {                                        // (the last entry: rows behind the experts)
+      lo = (int)offset_of(p, x);
+      const int hi = x < p.experts ? (int)offset_of(p, x + 1) : (p.zero_tail ? (int)p.rows : lo);
+      count = hi > lo ? hi - lo : 0;
+    }
+    const int tiles = (count + BM - 1) / BM, through = before + (int)wave_inclusive_sum_dpp((unsigned)tiles);
+    const unsigned long long behind = __ballot(through > mt);
+    if (behind) {
+      const int at = (int)__builtin_ctzll(behind);
+      const int m0 = (mt - (__builtin_amdgcn_readlane(through, at) - __builtin_amdgcn_readlane(tiles, at))) * BM;
+      e = e0 + at;
+      first = __builtin_amdgcn_readlane(lo, at) + m0;
+      rows = __builtin_amdgcn_readlane(count, at) - m0;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(through, 63);
+  }
+  return false;
+}
+
 // A launch has fewer than 2^32 threads.
 inline int check_tiles(long long tiles, int threads) {
   return tiles * threads > 0xffffffffll ? fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles) : 0;
 }
 
-int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream);
-int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream);
+int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream);
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bool gated, hipStream_t stream);
 int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream);
-int grouped_stream_launch(const GroupedParams& p, int dtype, hipStream_t stream);
+int grouped_stream_launch(const GroupedParams& p, int dtype, bool gated, hipStream_t stream);
 
 }  // namespace cm

@@ -1,5 +1,7 @@
 // Products grouped by expert: checks and the choice of a kernel (gfx950).
 
+#include <string.h>
+
 #include "grouped_gemm.h"
 
 namespace cm {
@@ -52,11 +54,12 @@ enum Kind { kNothing, kGeneral, kStream, kTile };
 struct Plan {
   GroupedParams p;
   Kind kind;
-  bool high;
+  bool high, gated;
 };
 
 int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   to.kind = kNothing;
+  to.gated = false;
   if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: unknown op %d", a.op);
   if (a.rows < 0 || a.rows > 0x1fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
     return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
@@ -76,9 +79,10 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   if (fp8 && a.x_scale_block != 0 && a.x_scale_block != 128)
     return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: x_scale_block must be 0 (per row) or 128, got %d", a.x_scale_block);
   if (a.rows == 0 && a.op != kWeightsGrad) return 0;
-  if (!a.y || !a.offsets || (a.rows > 0 && (!a.x || !a.w)) || (fp8 && (!a.x_scale || !a.w_scale)))
+  if (!a.y || (!a.offsets && a.experts != 1) || (a.rows > 0 && (!a.x || !a.w)) || (fp8 && (!a.x_scale || !a.w_scale)))
     return fail(CPPMEGA_MI355_ERR_NULL, "grouped_gemm: x / w / y / offsets / scales is NULL");
   GroupedParams& p = to.p;
+  memset(&p, 0, sizeof(p));
   p.x = a.x; p.w = a.w; p.y = a.y; p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale;
   p.rows = a.rows; p.x_pitch = a.x_pitch; p.w_pitch = a.w_pitch; p.y_pitch = a.y_pitch;
   p.experts = a.experts; p.n = a.n; p.k = a.k;
@@ -103,9 +107,9 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
 }
 
 int launch(const Plan& plan, int op, int dtype, hipStream_t stream) {
-  if (plan.kind == kTile) return grouped_tile_launch(plan.p, op, dtype, plan.high, stream);
-  if (plan.kind == kStream) return grouped_stream_launch(plan.p, dtype, stream);
-  return plan.kind == kGeneral ? grouped_general_launch(plan.p, op, dtype, stream) : 0;
+  if (plan.kind == kTile) return grouped_tile_launch(plan.p, op, dtype, plan.high, plan.gated, stream);
+  if (plan.kind == kStream) return grouped_stream_launch(plan.p, dtype, plan.gated, stream);
+  return plan.kind == kGeneral ? grouped_general_launch(plan.p, op, dtype, plan.gated, stream) : 0;
 }
 
 }  // namespace
@@ -127,6 +131,38 @@ int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const
     return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, high_grads(r.p, w.p), stream);
   rc = launch(r, kRowsGrad, rows.x_dtype, stream);
   return rc ? rc : launch(w, kWeightsGrad, weights.x_dtype, stream);
+}
+
+// Whether the gradients that are wanted would be launched, with the reason if not.
+int grouped_gemm_check(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights) {
+  Plan plan;
+  int rc = need_rows ? plan_of(rows, plan) : 0;
+  if (!rc && need_weights) rc = plan_of(weights, plan);
+  return rc;
+}
+
+// The gated block is a product of rows with 2 n rows of a weight, whose kernels pair them off; the same rules choose among them.
+int gated_gemm_launch(const cppmega_mi355_gated_gemm_args_t& a, hipStream_t stream) {
+  if (a.activation != CPPMEGA_MI355_GATE_SILU && a.activation != CPPMEGA_MI355_GATE_GELU_TANH)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "gated_gemm: unknown activation %d", a.activation);
+  if (a.n < 1 || a.n > CPPMEGA_MI355_GATED_MAX_OUTPUTS) return fail(CPPMEGA_MI355_ERR_SHAPE, "gated_gemm: n=%d, 1 to 2^29 are served", a.n);
+  if (a.pre && a.x_dtype == CPPMEGA_MI355_E4M3) return fail(CPPMEGA_MI355_ERR_DTYPE, "gated_gemm: the products of e4m3 operands are not kept");
+  if (a.pre && a.pre_dtype != a.x_dtype && a.pre_dtype != CPPMEGA_MI355_F32)
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "gated_gemm: pre of dtype %d from operands of dtype %d", a.pre_dtype, a.x_dtype);
+  cppmega_mi355_grouped_gemm_args_t g;
+  memset(&g, 0, sizeof(g));
+  g.op = kRows;
+  g.x = a.x; g.w = a.w; g.y = a.y; g.offsets = a.offsets; g.x_scale = a.x_scale; g.w_scale = a.w_scale;
+  g.x_dtype = a.x_dtype; g.y_dtype = a.y_dtype; g.offsets_dtype = a.offsets_dtype; g.x_scale_block = a.x_scale_block;
+  g.rows = a.rows; g.x_pitch = a.x_pitch; g.y_pitch = a.y_pitch;
+  g.experts = a.experts; g.n = 2 * a.n; g.k = a.k; g.zero_tail = a.zero_tail;
+  Plan plan;
+  if (int rc = plan_of(g, plan)) return rc;
+  plan.gated = true;
+  plan.p.n = a.n;
+  plan.p.activation = a.activation;
+  plan.p.pre = a.pre; plan.p.pre_dtype = a.pre_dtype; plan.p.pre_pitch = a.pre_pitch;
+  return launch(plan, kRows, a.x_dtype, stream);
 }
 
 }  // namespace cm

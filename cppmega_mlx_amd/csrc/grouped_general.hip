@@ -39,7 +39,8 @@ __device__ __forceinline__ u32x4 piece(const char* at, long long valid) {     //
   return r;
 }
 
-template <int OP, int DT>
+// GATED: of every wavefront's 64 columns the first 32 are rows of the gate, the others those of the up projection for the same outputs.
+template <int OP, int DT, bool GATED>
 __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParams p) {
   constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
   constexpr int BYTES = FP8 ? 1 : 2, STEP = 128 / BYTES;            // elements of contraction in a step
@@ -51,7 +52,8 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
 
   // ---- which tile ----
   const int rows_c = OP == kWeightsGrad ? p.n : 0, cols_c = OP == kRows ? p.n : p.k;
-  const int tiles_n = (cols_c + BN - 1) / BN;
+  constexpr int BO = GATED ? BN / 2 : BN;                          // columns of the result in a tile
+  const int tiles_n = (cols_c + BO - 1) / BO;
   int e, m0, n0;
   long long lo, hi;
   if (OP == kWeightsGrad) {
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
     e = (int)blockIdx.x / per;
     const int t = (int)blockIdx.x - e * per;
     m0 = t / tiles_n * BM;
-    n0 = t % tiles_n * BN;
+    n0 = t % tiles_n * BO;
     lo = offset_of(p, e);
     hi = offset_of(p, e + 1);
   } else {
@@ -70,13 +72,13 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
     lo = offset_of(p, e);
     hi = e < p.experts ? offset_of(p, e + 1) : p.rows;
     m0 = (mt - starts[e]) * BM;
-    n0 = (int)(blockIdx.x % (unsigned)tiles_n) * BN;
+    n0 = (int)(blockIdx.x % (unsigned)tiles_n) * BO;
   }
   const long long tokens = hi > lo ? hi - lo : 0;
   const long long contraction = OP == kWeightsGrad ? tokens : (e == p.experts ? 0 : (OP == kRows ? p.k : p.n));
   const long long rows_here = (OP == kWeightsGrad ? rows_c : tokens) - m0;          // rows of C from m0 on
   const long long cols_here = cols_c - n0;
-  const size_t weight = (size_t)e * p.n * p.k;
+  const size_t weight = (size_t)e * (GATED ? 2 : 1) * p.n * p.k;
   const char* const xb = (const char*)p.x + (size_t)lo * p.x_pitch * BYTES;
   const char* const wb = (const char*)p.w + (OP == kWeightsGrad ? (size_t)lo * p.w_pitch : e < p.experts ? weight : 0) * BYTES;
   const long long w_pitch = OP == kWeightsGrad ? p.w_pitch : p.k;
@@ -95,6 +97,15 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
         const int step = u >> 4, c = u & 15;
         to[i] = piece<BYTES>(base + ((k0 + step) * pitch + first + c * 8) * BYTES, k0 + step < contraction ? here - c * 8 : 0);
       }
+    }
+  };
+  // (gated: the rows of the weight that are the tile's columns)
+  auto fetch_gated = [&](long long k0, u32x4 (&to)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int u = i * 256 + tid, row = u >> 3, c = u & 7, out = (row >> 6) * 32 + (row & 31);
+      const long long k = k0 + c * (16 / BYTES);
+      to[i] = piece<BYTES>(wb + (((row & 32 ? (long long)p.n : 0) + n0 + out) * w_pitch + k) * BYTES, out < cols_here ? contraction - k : 0);
     }
   };
   auto keep = [&](bool transposed, u32x4* lds, const u32x4 (&from)[4]) {
@@ -137,7 +148,8 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
   const long long steps = (contraction + STEP - 1) / STEP;
   if (steps > 0) {
     fetch(TR, xb, p.x_pitch, m0, rows_here, 0, pr);
-    fetch(TQ, wb, w_pitch, n0, cols_here, 0, pq);
+    if constexpr (GATED) fetch_gated(0, pq);
+    else fetch(TQ, wb, w_pitch, n0, cols_here, 0, pq);
   }
   for (long long s = 0; s < steps; ++s) {
     __syncthreads();
@@ -146,16 +158,20 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
     __syncthreads();
     if (s + 1 < steps) {
       fetch(TR, xb, p.x_pitch, m0, rows_here, (s + 1) * STEP, pr);
-      fetch(TQ, wb, w_pitch, n0, cols_here, (s + 1) * STEP, pq);
+      if constexpr (GATED) fetch_gated((s + 1) * STEP, pq);
+      else fetch(TQ, wb, w_pitch, n0, cols_here, (s + 1) * STEP, pq);
     }
     if constexpr (FP8) {
-      float sx[2], sw;
+      float sx[2], sw[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const long long row = m0 + wm + i * 32 + l32;
         sx[i] = row < tokens ? p.x_scale[p.x_scale_block ? (size_t)(lo + row) * blocks_k + s : (size_t)(lo + row)] : 0.0f;
       }
-      sw = n0 < p.n ? p.w_scale[((size_t)e * ((p.n + 127) / 128) + n0 / 128) * blocks_k + s] : 0.0f;
+      const int blocks_n = (p.n + 127) / 128;
+      const float* const ws = p.w_scale + ((size_t)e * (GATED ? 2 : 1) * blocks_n + n0 / 128) * blocks_k + s;
+      sw[0] = n0 < p.n ? *ws : 0.0f;
+      sw[1] = !GATED ? sw[0] : n0 < p.n ? ws[(size_t)blocks_n * blocks_k] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -171,7 +187,7 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
             t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cvt8(q[0], q[1]), cvt8(r[0], r[1]), t, 0, 0, 0);
             t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cvt8(q[2], q[3]), cvt8(r[2], r[3]), t, 0, 0, 0);
           }
-          const float f = sx[i] * sw;
+          const float f = sx[i] * sw[j];
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[i][j][v] = fmaf(f, t[v], acc[i][j][v]);
         }
@@ -200,6 +216,21 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
   for (int i = 0; i < 2; ++i) {
     const int row = wm + i * 32 + l32;
     if (row >= rows_here) continue;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int col = wn / 2 + (v >> 2) * 8 + half * 4 + (v & 3);
+        if (col >= cols_here) continue;
+        const float g = acc[i][0][v], u = acc[i][1][v];
+        if (p.pre && e < p.experts) {
+          const size_t at = (row0 + row) * p.pre_pitch + n0 + col;
+          store_as(p.pre, at, p.pre_dtype, g);
+          store_as(p.pre, at + p.n, p.pre_dtype, u);
+        }
+        store_as(p.y, (row0 + row) * y_pitch + n0 + col, p.y_dtype, gated(g, u, p.activation));
+      }
+      continue;
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -212,21 +243,30 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
 
 }  // namespace
 
-int grouped_general_launch(const GroupedParams& p, int op, int dtype, hipStream_t stream) {
-  const long long tiles_n = ((op == kRows ? p.n : p.k) + BN - 1) / BN;
+int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream) {
+  const int across = gated ? BN / 2 : BN;
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + across - 1) / across;
   const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + BM - 1) / BM) : p.rows / BM + p.experts + 1;
   if (int rc = check_tiles(tiles_m * tiles_n, 256)) return rc;
   const dim3 grid((unsigned)(tiles_m * tiles_n)), block(256);
-#define CM_GENERAL(op_, dt) hipLaunchKernelGGL((grouped_general_kernel<op_, dt>), grid, block, 0, stream, p)
-#define CM_GENERAL_OP(op_)                                           \
-  do {                                                               \
-    if (dtype == CPPMEGA_MI355_F16) CM_GENERAL(op_, CPPMEGA_MI355_F16); \
-    else CM_GENERAL(op_, CPPMEGA_MI355_BF16);                        \
+#define CM_GENERAL(op_, dt, gated_) hipLaunchKernelGGL((grouped_general_kernel<op_, dt, gated_>), grid, block, 0, stream, p)
+#define CM_GENERAL_OP(op_, gated_)                                              \
+  do {                                                                          \
+    if (dtype == CPPMEGA_MI355_F16) CM_GENERAL(op_, CPPMEGA_MI355_F16, gated_); \
+    else CM_GENERAL(op_, CPPMEGA_MI355_BF16, gated_);                           \
   } while (0)
-  if (dtype == CPPMEGA_MI355_E4M3) CM_GENERAL(kRows, CPPMEGA_MI355_E4M3);
-  else if (op == kRows) CM_GENERAL_OP(kRows);
-  else if (op == kRowsGrad) CM_GENERAL_OP(kRowsGrad);
-  else CM_GENERAL_OP(kWeightsGrad);
+  if (dtype == CPPMEGA_MI355_E4M3) {
+    if (gated) CM_GENERAL(kRows, CPPMEGA_MI355_E4M3, true);
+    else CM_GENERAL(kRows, CPPMEGA_MI355_E4M3, false);
+  } else if (gated) {
+    CM_GENERAL_OP(kRows, true);
+  } else if (op == kRows) {
+    CM_GENERAL_OP(kRows, false);
+  } else if (op == kRowsGrad) {
+    CM_GENERAL_OP(kRowsGrad, false);
+  } else {
+    CM_GENERAL_OP(kWeightsGrad, false);
+  }
 #undef CM_GENERAL_OP
 #undef CM_GENERAL
   CM_HIP_CHECK(hipGetLastError());

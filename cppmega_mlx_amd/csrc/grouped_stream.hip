@@ -19,10 +19,11 @@ namespace {
 
 constexpr int kWaves = 4;
 
-template <int DT, int TN>
+// GATED: half of a workgroup's weight rows are the gate's, half the up projection's for the same outputs.
+template <int DT, int TN, bool GATED>
 __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const GroupedParams p) {
   constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
-  constexpr int BYTES = FP8 ? 1 : 2, STEP = 128 / BYTES, BM = 16, BN = 16 * TN;
+  constexpr int BYTES = FP8 ? 1 : 2, STEP = 128 / BYTES, BM = 16, TO = GATED ? TN / 2 : TN, BN = 16 * TO;
   __shared__ f32x4 sums[kWaves][TN][64];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15, quad = lane >> 4;
@@ -30,28 +31,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
   // ---- which tile ----
   const int tiles_n = (p.n + BN - 1) / BN;
   const int mt = (int)(blockIdx.x / (unsigned)tiles_n), n0 = (int)(blockIdx.x % (unsigned)tiles_n) * BN;
-  int e = -1, first = 0, rows = 0;
-  for (int e0 = 0, before = 0; e0 <= p.experts; e0 += 64) {
-    const int x = e0 + lane;
-    int lo = 0, count = 0;
-    if (x <= p.experts) {                                        // (the last entry: rows behind the experts, to be zeroed)
-      lo = (int)offset_of(p, x);
-      const int hi = x < p.experts ? (int)offset_of(p, x + 1) : (p.zero_tail ? (int)p.rows : lo);
-      count = hi > lo ? hi - lo : 0;
-    }
-    const int tiles = (count + BM - 1) / BM, through = before + (int)wave_inclusive_sum_dpp((unsigned)tiles);
-    const unsigned long long behind = __ballot(through > mt);
-    if (behind) {
-      const int at = (int)__builtin_ctzll(behind);
-      const int m0 = (mt - (__builtin_amdgcn_readlane(through, at) - __builtin_amdgcn_readlane(tiles, at))) * BM;
-      e = e0 + at;
-      first = __builtin_amdgcn_readlane(lo, at) + m0;
-      rows = __builtin_amdgcn_readlane(count, at) - m0;
-      break;
-    }
-    before = __builtin_amdgcn_readlane(through, 63);
-  }
-  if (e < 0) return;
+  int e, first, rows;
+  if (!rows_of_tile<BM>(p, mt, e, first, rows)) return;
 
   // ---- this wavefront's steps ----
   const int steps = e < p.experts ? (p.k + STEP - 1) / STEP : 0;
@@ -61,19 +42,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
   const float *sxat = nullptr, *swat = nullptr;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int n = n0 + j * 16 + l16;
-    wat[j] = (const char*)p.w + ((size_t)(e < p.experts ? e : 0) * p.n + (n < p.n ? n : p.n - 1)) * p.k * BYTES + quad * 16;
+    const int n = n0 + j % TO * 16 + l16;
+    wat[j] = (const char*)p.w + ((size_t)(e < p.experts ? e : 0) * (GATED ? 2 : 1) * p.n + (n < p.n ? n : p.n - 1) + (j < TO ? 0 : p.n)) * p.k * BYTES + quad * 16;
   }
   const size_t x_row = (size_t)(first + (l16 < rows ? l16 : rows - 1));      // (rows past the end repeat the last one and are not stored)
   const char* const xat = (const char*)p.x + x_row * p.x_pitch * BYTES + quad * 16;
   if (FP8) sxat = p.x_scale + x_row * (p.x_scale_block ? blocks_k : 1);
-  if (FP8) swat = p.w_scale + ((size_t)(e < p.experts ? e : 0) * ((p.n + 127) / 128) + n0 / 128) * blocks_k;
+  const int blocks_n = (p.n + 127) / 128;
+  if (FP8) swat = p.w_scale + ((size_t)(e < p.experts ? e : 0) * (GATED ? 2 : 1) * blocks_n + n0 / 128) * blocks_k;
+  const size_t up_scale = (size_t)blocks_n * blocks_k;
 
   f32x4 acc[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   u32x4 w[2][TN][2], x[2][2];
-  float sx[2], sw[2];
+  float sx[2], sw[2], sw_up[2];
   // PART: the last step, of which a part may not be there (a condition on every load costs 15 %: its select waits for the data)
   auto load = [&](int s, int to, auto part) {
     constexpr bool PART = decltype(part)::value;
@@ -89,6 +72,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
     if (FP8) {
       sx[to] = sxat[p.x_scale_block ? s : 0];
       sw[to] = swat[s];
+      if (GATED) sw_up[to] = swat[up_scale + s];
     }
   };
   auto multiply = [&](int b) {
@@ -96,14 +80,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
       bf16x8 xv[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) xv[c] = cvt8(x[b][c >> 1][2 * (c & 1)], x[b][c >> 1][2 * (c & 1) + 1]);
-      const float f = sx[b] * sw[b];
+      const float f = sx[b] * sw[b], f_up = GATED ? sx[b] * sw_up[b] : f;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < 4; ++c) t = mm<false>(cvt8(w[b][j][c >> 1][2 * (c & 1)], w[b][j][c >> 1][2 * (c & 1) + 1]), xv[c], t);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[j][v] = fmaf(f, t[v], acc[j][v]);
+        for (int v = 0; v < 4; ++v) acc[j][v] = fmaf(j < TO ? f : f_up, t[v], acc[j][v]);
       }
     } else {
 #pragma unroll
@@ -131,43 +115,60 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
 #pragma unroll
   for (int j = 0; j < TN; ++j) sums[wave][j][lane] = acc[j];
   __syncthreads();
-  if (wave >= TN) return;
-  f32x4 v = sums[0][wave][lane];
+  if (wave >= TO) return;
+  auto sum_of = [&](int j) {
+    f32x4 v = sums[0][j][lane];
 #pragma unroll
-  for (int k = 1; k < kWaves; ++k) v += sums[k][wave][lane];
+    for (int k = 1; k < kWaves; ++k) v += sums[k][j][lane];
+    return v;
+  };
   const int n = n0 + wave * 16 + quad * 4;
   if (l16 >= rows || n >= p.n) return;
-  const size_t at = (size_t)(first + l16) * p.y_pitch + n;
-  if (n + 4 <= p.n && p.y_dtype != CPPMEGA_MI355_F32) {
-    const uint2 r = p.y_dtype == CPPMEGA_MI355_F16 ? make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3])) : make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-    __builtin_memcpy((unsigned short*)p.y + at, &r, 8);
-  } else {
+  auto store = [&](void* y, int dtype, size_t at, const f32x4 v) {
+    if (n + 4 <= p.n && dtype != CPPMEGA_MI355_F32) {
+      const uint2 r = dtype == CPPMEGA_MI355_F16 ? make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3])) : make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+      __builtin_memcpy((unsigned short*)y + at, &r, 8);
+    } else {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (n + c < p.n) store_as(p.y, at + c, p.y_dtype, v[c]);
+      for (int c = 0; c < 4; ++c)
+        if (n + c < p.n) store_as(y, at + c, dtype, v[c]);
+    }
+  };
+  f32x4 v = sum_of(wave);
+  if constexpr (GATED) {
+    const f32x4 u = sum_of(TO + wave);
+    if (p.pre && e < p.experts) {
+      const size_t at = (size_t)(first + l16) * p.pre_pitch + n;
+      store(p.pre, p.pre_dtype, at, v);
+      store(p.pre, p.pre_dtype, at + p.n, u);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = gated(v[c], u[c], p.activation);
   }
+  store(p.y, p.y_dtype, (size_t)(first + l16) * p.y_pitch + n, v);
 }
 
-template <int DT>
+template <int DT, bool GATED>
 int launch(const GroupedParams& p, hipStream_t stream) {
   const long long tails = p.experts + 1 < p.rows ? p.experts + 1 : p.rows;       // tiles of rows that are not full, at most
   const long long tiles_m = p.rows / 16 + tails < p.rows ? p.rows / 16 + tails : p.rows;
-  const bool wide = tiles_m * ((p.n + 63) / 64) >= 512;                          // (two workgroups to a CU at least)
-  const long long tiles = tiles_m * (wide ? (p.n + 63) / 64 : (p.n + 15) / 16);
+  constexpr int kWide = GATED ? 32 : 64;                                         // outputs of a workgroup
+  const bool wide = tiles_m * ((p.n + kWide - 1) / kWide) >= 512;                // (two workgroups to a CU at least)
+  const long long tiles = tiles_m * (wide ? (p.n + kWide - 1) / kWide : (p.n + 15) / 16);
   if (int rc = check_tiles(tiles, 64 * kWaves)) return rc;
   const dim3 grid((unsigned)tiles), block(64 * kWaves);
-  if (wide) hipLaunchKernelGGL((grouped_stream_kernel<DT, 4>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((grouped_stream_kernel<DT, 1>), grid, block, 0, stream, p);
+  if (wide) hipLaunchKernelGGL((grouped_stream_kernel<DT, 4, GATED>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((grouped_stream_kernel<DT, GATED ? 2 : 1, GATED>), grid, block, 0, stream, p);
   CM_HIP_CHECK(hipGetLastError());
   return 0;
 }
 
 }  // namespace
 
-int grouped_stream_launch(const GroupedParams& p, int dtype, hipStream_t stream) {
-  if (dtype == CPPMEGA_MI355_E4M3) return launch<CPPMEGA_MI355_E4M3>(p, stream);
-  if (dtype == CPPMEGA_MI355_F16) return launch<CPPMEGA_MI355_F16>(p, stream);
-  return launch<CPPMEGA_MI355_BF16>(p, stream);
+int grouped_stream_launch(const GroupedParams& p, int dtype, bool gated, hipStream_t stream) {
+  if (dtype == CPPMEGA_MI355_E4M3) return gated ? launch<CPPMEGA_MI355_E4M3, true>(p, stream) : launch<CPPMEGA_MI355_E4M3, false>(p, stream);
+  if (dtype == CPPMEGA_MI355_F16) return gated ? launch<CPPMEGA_MI355_F16, true>(p, stream) : launch<CPPMEGA_MI355_F16, false>(p, stream);
+  return gated ? launch<CPPMEGA_MI355_BF16, true>(p, stream) : launch<CPPMEGA_MI355_BF16, false>(p, stream);
 }
 
 }  // namespace cm

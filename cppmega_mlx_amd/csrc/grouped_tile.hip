@@ -61,11 +61,15 @@ using Count = std::integral_constant<int, N>;
 
 // Tile `block` of a product (of the launch's order, or none: every XCD's blocks are counted up to the same number), in S::kLds bytes of LDS.
 // `cut`: the last round's tiles in parts.
-template <int OP, int DT, bool HIGH>
+template <int OP, int DT, bool HIGH, bool GATED>
 __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block, u32x4* const smem, const bool cut) {
   typedef Shape<OP, DT, HIGH> S;                                 // (inlined throughout: a call would put the sums into memory)
   constexpr bool FP8 = S::FP8, F16 = S::F16, TR = S::TR, TQ = S::TQ;
   constexpr int BYTES = S::BYTES, STEP = S::STEP, BM = S::BM, BN = S::BN, RS = S::RS, QS = S::QS, RL = S::RL, QL = S::QL, L = S::L, KB = S::KB;
+  // Columns of the result in a tile.  GATED: of every wavefront's columns the first half are rows of the gate, the others those of the up
+  // projection for the same outputs: a lane has both sums.
+  constexpr int BO = GATED ? BN / 2 : BN, kHalf = S::kWidth / 2;
+  static_assert(!GATED || OP == kRows, "the gated block is a product of rows");
   static_assert(S::kLds >= (kMaxExperts + 2) * (int)sizeof(int), "the tiles' table lies where the stages are later");
   int* const starts = reinterpret_cast<int*>(smem);
   char* const lds = reinterpret_cast<char*>(smem);
@@ -75,7 +79,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
   // ---- which tile: every XCD takes one run of the order, which goes through the experts; of each, up to four row tiles share the
   // columns that pass, so that an expert's weight leaves memory once (groups of four rows of tiles whatever their experts: 5 % slower) ----
   const int cols_c = OP == kRows ? p.n : p.k;
-  const int tiles_n = (cols_c + BN - 1) / BN;
+  const int tiles_n = (cols_c + BO - 1) / BO;
   const int per_expert = OP == kWeightsGrad ? (p.n + BM - 1) / BM : 0;
   int e, m0, n0, part_rows = BM;
   {
@@ -111,7 +115,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
     const int group = local / (step * tiles_n), in = local - group * step * tiles_n;
     const int height = high - group * step < step ? high - group * step : step;
     const int nt = in / height;
-    n0 = nt * BN;
+    n0 = nt * BO;
     m0 = (group * step + in - nt * height) * BM + part * part_rows;
   }
   const int lo = __builtin_amdgcn_readfirstlane((int)offset_of(p, e));
@@ -127,7 +131,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
 
   // ---- loads ----
   const char* xb = (const char*)p.x + ((size_t)lo * p.x_pitch + (TR ? (size_t)m0 : (size_t)m0 * p.x_pitch)) * BYTES;
-  const char* wb = (const char*)p.w + ((OP == kWeightsGrad ? (size_t)lo * p.w_pitch : (size_t)(e < p.experts ? e : 0) * p.n * p.k) + (TQ ? (size_t)n0 : (size_t)n0 * p.k)) * BYTES;
+  const char* wb = (const char*)p.w + ((OP == kWeightsGrad ? (size_t)lo * p.w_pitch : (size_t)(e < p.experts ? e : 0) * (GATED ? 2 : 1) * p.n * p.k) + (TQ ? (size_t)n0 : (size_t)n0 * p.k)) * BYTES;
   const long long x_step = TR ? p.x_pitch * STEP * BYTES : KB, w_step = TQ ? w_pitch * STEP * BYTES : KB;
   unsigned xoff[RL], woff[QL], soff = 0;
   // where a lane's piece of load instruction u of an operand lies, and how far along the contraction that is
@@ -140,13 +144,20 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
     const int step = u * (512 / BM) + lane / (BM / 8), c = (lane % (BM / 8)) ^ ((step & 3) << 2);
     return (unsigned)(step * pitch * BYTES) + (unsigned)(c * 8 < limit ? c : (limit - 1) >> 3) * 16u;
   };
+  // (gated: the row of the weight's half, in which the outputs of a wavefront's columns follow each other)
+  auto gated_piece = [&](int u) -> unsigned {
+    const int row = u * (64 / PIECES) + lane / PIECES, c = (lane % PIECES) ^ S::fold(row), out = row / S::kWidth * kHalf + row % kHalf;
+    return (unsigned)((out < cols_here ? out : cols_here - 1) * w_pitch * BYTES) + (unsigned)c * 16u;
+  };
+  const size_t up_at = GATED ? (size_t)p.n * p.k * BYTES : 0;     // from the gate's rows to the up projection's
+  auto half_of = [&](int u) -> size_t { return GATED && (u * (64 / PIECES) / kHalf & 1) ? up_at : 0; };   // (eight rows of one load instruction are of one half)
   auto along = [&](bool transposed, int u) {
     return transposed ? u * (512 / BM) + lane / (BM / 8) : ((lane % PIECES) ^ S::fold(u * (64 / PIECES) + lane / PIECES)) * (16 / BYTES);
   };
 #pragma unroll
   for (int i = 0; i < RL; ++i) xoff[i] = piece_of(TR, wave * RL + i, rows_here, p.x_pitch);
 #pragma unroll
-  for (int i = 0; i < QL; ++i) woff[i] = piece_of(TQ, wave * QL + i, cols_here, w_pitch);
+  for (int i = 0; i < QL; ++i) woff[i] = GATED ? gated_piece(wave * QL + i) : piece_of(TQ, wave * QL + i, cols_here, w_pitch);
   const char* sb = nullptr;
   unsigned s_step = 0;
   if constexpr (FP8) {
@@ -158,9 +169,9 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
       soff = (unsigned)(row < rows_here ? row : rows_here - 1) * (p.x_scale_block ? (unsigned)blocks_k * 4u : 4u);
       s_step = p.x_scale_block ? 4u : 0u;
     } else {
-      const int b = n0 / 128 + (BN > 128 ? lane & 1 : 0);
-      sb = (const char*)(p.w_scale + (size_t)(e < p.experts ? e : 0) * blocks_n * blocks_k);
-      soff = (unsigned)(b < blocks_n ? b : blocks_n - 1) * (unsigned)blocks_k * 4u;
+      const int b = n0 / 128 + (BO > 128 ? lane & 1 : 0), half = GATED ? lane & 1 : 0;
+      sb = (const char*)(p.w_scale + (size_t)(e < p.experts ? e : 0) * (GATED ? 2 : 1) * blocks_n * blocks_k);
+      soff = ((unsigned)(b < blocks_n ? b : blocks_n - 1) + (unsigned)half * (unsigned)blocks_n) * (unsigned)blocks_k * 4u;
       s_step = 4u;
     }
   }
@@ -189,10 +200,10 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
           const int u = wave * QL + i;
           unsigned off = woff[i < QL ? i : 0];
           if (MORE) {
-            load16(wb, off, q_slot + (unsigned)(u * 1024));
+            load16(wb + half_of(u), off, q_slot + (unsigned)(u * 1024));
           } else {
             asm("" : "+v"(off));                                // (the address is made here, not kept in registers throughout)
-            load16_at(next_q * STEP + along(TQ, u) < contraction ? wb + off : (const char*)zeros, q_slot + (unsigned)(u * 1024));
+            load16_at(next_q * STEP + along(TQ, u) < contraction ? wb + half_of(u) + off : (const char*)zeros, q_slot + (unsigned)(u * 1024));
           }
         } else {
           const bool there = MORE || next_q < stages;
@@ -254,24 +265,39 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
   const size_t row0 = OP == kWeightsGrad ? (size_t)e * p.n + m0 : (size_t)lo + m0;
   const long long y_pitch = OP == kWeightsGrad ? p.k : p.y_pitch;
   // 8 (16-bit) or 4 (float32) values of a row, as far as the columns go
-  auto store = [&](int row, int col, const float* v, int count) __attribute__((always_inline)) {
-    if (row >= rows_here || col >= cols_here) return;
-    const size_t at = (row0 + row) * y_pitch + n0 + col;
+  auto store_to = [&](void* y, int dtype, size_t at, int col, const float* v, int count) __attribute__((always_inline)) {
     if (col + count <= cols_here) {
-      if (p.y_dtype == CPPMEGA_MI355_F32) {
-        __builtin_memcpy((float*)p.y + at, v, 4 * count);
+      if (dtype == CPPMEGA_MI355_F32) {
+        __builtin_memcpy((float*)y + at, v, 4 * count);
       } else {
         unsigned r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (2 * i < count) r[i] = p.y_dtype == CPPMEGA_MI355_F16 ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
-        __builtin_memcpy((unsigned short*)p.y + at, r, 2 * count);
+          if (2 * i < count) r[i] = dtype == CPPMEGA_MI355_F16 ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
+        __builtin_memcpy((unsigned short*)y + at, r, 2 * count);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < count && col + i < cols_here) store_as(p.y, at + i, p.y_dtype, v[i]);
+        if (i < count && col + i < cols_here) store_as(y, at + i, dtype, v[i]);
     }
+  };
+  auto store = [&](int row, int col, const float* v, int count) __attribute__((always_inline)) {
+    if (row >= rows_here || col >= cols_here) return;
+    store_to(p.y, p.y_dtype, (row0 + row) * y_pitch + n0 + col, col, v, count);
+  };
+  // gated: 8 values of the gate and of the up projection
+  auto store_gated = [&](int row, int col, const float* g, const float* u) __attribute__((always_inline)) {
+    if (row >= rows_here || col >= cols_here) return;
+    if (p.pre && e < p.experts) {
+      const size_t at = (row0 + row) * p.pre_pitch + n0 + col;
+      store_to(p.pre, p.pre_dtype, at, col, g, 8);
+      store_to(p.pre, p.pre_dtype, at + p.n, col, u, 8);
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gated(g[i], u[i], p.activation);
+    store_to(p.y, p.y_dtype, (row0 + row) * y_pitch + n0 + col, col, v, 8);
   };
 
   if constexpr (!FP8) {
@@ -372,21 +398,30 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // (what was requested behind the end still writes to LDS)
     // lane: row l % 32, columns 8 q + 4 (l / 32) + 0..3; the halves change places so that a lane has 8 columns in a run
+    auto run_of = [&](int i, int j, int h, float (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][h * 8 + c]), __float_as_uint(acc[i][j][h * 8 + 4 + c]), false, false);
+        v[c] = __uint_as_float(x[0]);
+        v[4 + c] = __uint_as_float(x[1]);
+      }
+    };
     if (runs > 0) {
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
-        for (int j = 0; j < TJ; ++j)
+        for (int j = 0; j < TJ; j += GATED ? 2 : 1)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float v[8];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][j][h * 8 + c]), __float_as_uint(acc[i][j][h * 8 + 4 + c]), false, false);
-              v[c] = __uint_as_float(x[0]);
-              v[4 + c] = __uint_as_float(x[1]);
+            float v[8], u[8];
+            run_of(i, j, h, v);
+            if constexpr (GATED) {
+              static_assert(TJ == 2, "a wavefront has 32 outputs");
+              run_of(i, j + 1, h, u);
+              store_gated(i * 64 + upper * 32 + l32, wn / 2 + h * 16 + half * 8, v, u);
+            } else {
+              store(i * 64 + upper * 32 + l32, wn + j * 32 + h * 16 + half * 8, v, 8);
             }
-            store(i * 64 + upper * 32 + l32, wn + j * 32 + h * 16 + half * 8, v, 8);
           }
     }
   } else {
@@ -394,7 +429,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
     const int l16 = lane & 15, quad = lane >> 4, f = (l16 >> 1) & 7;
     const int rat[2] = {(upper * 32 + l16) * 128 + (quad ^ f) * 16, (upper * 32 + l16) * 128 + ((quad + 4) ^ f) * 16};
     const int qat[2] = {(wn + l16) * 128 + (quad ^ f) * 16, (wn + l16) * 128 + ((quad + 4) ^ f) * 16};
-    const int xsat = (upper * 32 + l16) * 4, wsat = BM / 64 * 256 + (wn >> 7) * 4;
+    const int xsat = (upper * 32 + l16) * 4, wsat = BM / 64 * 256 + (GATED ? 0 : (wn >> 7) * 4);
     auto operand = [&](int a, int b) -> i32x8 {
       const u32x4 x = *reinterpret_cast<const u32x4*>(lds + a), y = *reinterpret_cast<const u32x4*>(lds + b);
       i32x8 o;
@@ -411,7 +446,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
 #pragma unroll
       for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     i32x8 q[TJ], r[2];
-    float sx[TI], sw;
+    float sx[TI], sw, sw_up = 0.0f;
     auto read_q = [&](int from, int j) { q[j] = operand(from + qat[0] + j * 2048, from + qat[1] + j * 2048); };
     auto row_of = [](int i) { return (i >> 1) * 64 + (i & 1) * 16; };   // where the rows' tile i begins
     auto read_r = [&](int from, int i) { r[i & 1] = operand(from + rat[0] + row_of(i) * 128, from + rat[1] + row_of(i) * 128); };
@@ -419,6 +454,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
 #pragma unroll
       for (int i = 0; i < decltype(n)::value; ++i) sx[i] = *reinterpret_cast<const float*>(lds + from + xsat + row_of(i) * 4);
       sw = *reinterpret_cast<const float*>(lds + from + wsat);
+      if (GATED) sw_up = *reinterpret_cast<const float*>(lds + from + wsat + 4);
     };
     // a block's products are scaled and added while the matrix unit is at the next ones
     f32x4 t[2][TJ];
@@ -427,11 +463,11 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
       t[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q[j], r[i & 1], zero, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
     };
     auto add = [&](int i) {
-      const float s = sx[i] * sw;
+      const float s = sx[i] * sw, s_up = GATED ? sx[i] * sw_up : s;
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(s, t[i & 1][j][v], acc[i][j][v]);
+        for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(GATED && j >= TJ / 2 ? s_up : s, t[i & 1][j][v], acc[i][j][v]);
     };
     // the first n of the rows' tiles (an even number) but the last; load instructions from .. between them, a share to a group of products
     auto products = [&](auto n, auto more, int from) __attribute__((always_inline)) {
@@ -500,28 +536,37 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // lane: row l % 16, columns 4 (l / 16) + 0..3; two tiles' quarters change places so that a lane has 8 columns in a run
+    auto run_of = [&](int i, int j, float (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const u32x2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][c]), __float_as_uint(acc[i][j + 1][c]), false, false);
+        v[c] = __uint_as_float(x[0]);
+        v[4 + c] = __uint_as_float(x[1]);
+      }
+    };
     if (runs > 0) {
 #pragma unroll
       for (int i = 0; i < TI; ++i)
 #pragma unroll
-        for (int j = 0; j < TJ; j += 2) {
-          float v[8];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const u32x2 x = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][j][c]), __float_as_uint(acc[i][j + 1][c]), false, false);
-            v[c] = __uint_as_float(x[0]);
-            v[4 + c] = __uint_as_float(x[1]);
+        for (int j = 0; j < (GATED ? TJ / 2 : TJ); j += 2) {
+          float v[8], u[8];
+          run_of(i, j, v);
+          if constexpr (GATED) {
+            static_assert(TJ == 4, "a wavefront has 32 outputs");
+            run_of(i, TJ / 2 + j, u);
+            store_gated(row_of(i) + upper * 32 + l16, wn / 2 + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, u);
+          } else {
+            store(row_of(i) + upper * 32 + l16, wn + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, 8);
           }
-          store(row_of(i) + upper * 32 + l16, wn + (j + (quad & 1)) * 16 + (quad >> 1) * 8, v, 8);
         }
     }
   }
 }
 
-template <int OP, int DT, bool HIGH>
+template <int OP, int DT, bool HIGH, bool GATED>
 __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
   __shared__ u32x4 smem[Shape<OP, DT, HIGH>::kLds / 16];
-  tile_of<OP, DT, HIGH>(p, (int)blockIdx.x, smem, true);
+  tile_of<OP, DT, HIGH, GATED>(p, (int)blockIdx.x, smem, true);
 }
 
 // Both gradients: the weights' tiles fill the CUs that the rows' last round leaves idle.
@@ -529,38 +574,46 @@ template <int DT, bool HIGH>
 __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_grads_kernel(const GroupedParams rows, const GroupedParams weights, const int first) {
   constexpr int kLds = Shape<kRowsGrad, DT, HIGH>::kLds, kLdsW = Shape<kWeightsGrad, DT, HIGH>::kLds;
   __shared__ u32x4 smem[(kLds > kLdsW ? kLds : kLdsW) / 16];
-  if ((int)blockIdx.x < first) tile_of<kRowsGrad, DT, HIGH>(rows, (int)blockIdx.x, smem, false);
-  else tile_of<kWeightsGrad, DT, HIGH>(weights, (int)blockIdx.x - first, smem, false);
+  if ((int)blockIdx.x < first) tile_of<kRowsGrad, DT, HIGH, false>(rows, (int)blockIdx.x, smem, false);
+  else tile_of<kWeightsGrad, DT, HIGH, false>(weights, (int)blockIdx.x - first, smem, false);
 }
 
 // Blocks of a product, a multiple of eight.
-long long blocks_of(const GroupedParams& p, int op, bool high, bool cut) {
-  const int b = high ? 256 : 128;
-  const long long tiles_n = ((op == kRows ? p.n : p.k) + b - 1) / b, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
+long long blocks_of(const GroupedParams& p, int op, bool high, bool cut, bool gated) {
+  const int b = high ? 256 : 128, across = gated ? b / 2 : b;
+  const long long tiles_n = ((op == kRows ? p.n : p.k) + across - 1) / across, tiles_w = ((long long)p.n + b - 1) / b * tiles_n;   // (of a weight)
   if (op == kWeightsGrad) return p.experts * ((tiles_w + 7) / 8) * 8;
   return (((p.rows / b + p.experts + 1) * tiles_n + 7) / 8 + (!cut ? 0 : high ? 24 : 32)) * 8;   // (parts of the last tiles)
 }
 
 }  // namespace
 
-int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hipStream_t stream) {
-  const long long blocks = blocks_of(p, op, high, true);
+int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bool gated, hipStream_t stream) {
+  const long long blocks = blocks_of(p, op, high, true, gated);
   if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
-#define CM_TILE(op_, dt)                                                                              \
-  do {                                                                                                \
-    if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true>), grid, block, 0, stream, p);    \
-    else hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, false>), grid, block, 0, stream, p);        \
+#define CM_TILE(op_, dt, gated_)                                                                              \
+  do {                                                                                                        \
+    if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true, gated_>), grid, block, 0, stream, p);    \
+    else hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, false, gated_>), grid, block, 0, stream, p);        \
   } while (0)
-#define CM_TILE_OP(op_)                                              \
-  do {                                                               \
-    if (dtype == CPPMEGA_MI355_F16) CM_TILE(op_, CPPMEGA_MI355_F16); \
-    else CM_TILE(op_, CPPMEGA_MI355_BF16);                           \
+#define CM_TILE_OP(op_, gated_)                                              \
+  do {                                                                       \
+    if (dtype == CPPMEGA_MI355_F16) CM_TILE(op_, CPPMEGA_MI355_F16, gated_); \
+    else CM_TILE(op_, CPPMEGA_MI355_BF16, gated_);                           \
   } while (0)
-  if (dtype == CPPMEGA_MI355_E4M3) CM_TILE(kRows, CPPMEGA_MI355_E4M3);
-  else if (op == kRows) CM_TILE_OP(kRows);
-  else if (op == kRowsGrad) CM_TILE_OP(kRowsGrad);
-  else CM_TILE_OP(kWeightsGrad);
+  if (dtype == CPPMEGA_MI355_E4M3) {
+    if (gated) CM_TILE(kRows, CPPMEGA_MI355_E4M3, true);
+    else CM_TILE(kRows, CPPMEGA_MI355_E4M3, false);
+  } else if (gated) {
+    CM_TILE_OP(kRows, true);
+  } else if (op == kRows) {
+    CM_TILE_OP(kRows, false);
+  } else if (op == kRowsGrad) {
+    CM_TILE_OP(kRowsGrad, false);
+  } else {
+    CM_TILE_OP(kWeightsGrad, false);
+  }
 #undef CM_TILE_OP
 #undef CM_TILE
   CM_HIP_CHECK(hipGetLastError());
@@ -568,7 +621,7 @@ int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, hi
 }
 
 int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream) {
-  const long long first = blocks_of(rows, kRowsGrad, high, false), blocks = first + blocks_of(weights, kWeightsGrad, high, false);
+  const long long first = blocks_of(rows, kRowsGrad, high, false, false), blocks = first + blocks_of(weights, kWeightsGrad, high, false, false);
   if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
 #define CM_GRADS(dt)                                                                                                              \

@@ -22,7 +22,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "../../include/cppmega_mi355_layer.h"
+#include "../../include/cppmega_mi355_ffn.h"
 
 namespace {
 
@@ -828,6 +828,138 @@ PyObject* grouped_fp8_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   return wrap(y);
 }
 
+// ---- gated block, products with 4-bit weights -----------------------------------------------------
+// Sizes, experts and offsets of a feed-forward call over weights [E, rows, channels] or (no offsets) [rows, channels]; false: not the plain case.
+template <class Args>
+bool ffn_operands(const Place& at, const Tensor& x, const Tensor& w, PyObject* offsets, Args& a) {
+  const bool dense = offsets == Py_None;
+  const Tensor* o = tensor(offsets);
+  if ((!dense && !o) || x.dim() != 2 || w.dim() != (dense ? 2 : 3) || !at.dense(x) || !at.dense(w) || x.size(0) < 1) return false;
+  const int64_t experts = dense ? 1 : w.size(0);
+  if (!dense && (!at.dense(*o) || !is_index(o->scalar_type()) || !has_shape(*o, {experts + 1}))) return false;
+  for (int64_t size : {x.size(0), x.size(1), experts, w.size(-2), w.size(-1)})
+    if (!fits_int(size) || size < 1) return false;
+  memset(&a, 0, sizeof(a));
+  a.struct_size = sizeof(a);
+  a.offsets = dense ? nullptr : o->data_ptr();
+  a.offsets_dtype = dense ? CPPMEGA_MI355_I32 : code(o->scalar_type());
+  a.rows = x.size(0);
+  a.experts = (int32_t)experts;
+  a.k = (int32_t)x.size(1);
+  a.x = x.data_ptr(); a.w = w.data_ptr();
+  a.x_pitch = a.k;
+  a.zero_tail = 1;
+  return true;
+}
+
+// gated_gemm(x, w, offsets or None, activation, pre or None) -> y or None
+PyObject* gated_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 5 || !PyLong_CheckExact(arg[3])) DECLINE;
+  const Tensor *x = tensor(arg[0]), *w = tensor(arg[1]), *pre = tensor(arg[4]);
+  Place at;
+  cppmega_mi355_gated_gemm_args_t a;
+  if (!x || !w || (!pre && arg[4] != Py_None) || !at.take(*x) || !is_half(*x) || w->scalar_type() != x->scalar_type()) DECLINE;
+  if (!ffn_operands(at, *x, *w, arg[2], a) || w->size(-1) != a.k || w->size(-2) % 2) DECLINE;
+  a.n = (int32_t)(w->size(-2) / 2);
+  a.activation = (int32_t)as_int(arg[3]);
+  a.x_dtype = a.y_dtype = code(x->scalar_type());
+  if (pre) {
+    if (!at.dense(*pre) || pre->scalar_type() != x->scalar_type() || !has_shape(*pre, {a.rows, 2ll * a.n})) DECLINE;
+    a.pre = pre->data_ptr();
+    a.pre_dtype = a.x_dtype;
+    a.pre_pitch = 2ll * a.n;
+  }
+  Tensor y = at::empty({a.rows, a.n}, x->options());
+  a.y = y.data_ptr();
+  a.y_pitch = a.n;
+  if (unlocked([&] { return cppmega_mi355_gated_gemm(&a, sizeof(a), at.stream); })) DECLINE;
+  if (pre && !pre->is_inference()) pre->unsafeGetTensorImpl()->bump_version();
+  return wrap(y);
+}
+
+// gated_gemm_bwd(dy, pre, x, w, offsets or None, activation) -> (dx, dw) or None
+PyObject* gated_gemm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 6 || !PyLong_CheckExact(arg[5])) DECLINE;
+  const Tensor *dy = tensor(arg[0]), *pre = tensor(arg[1]), *x = tensor(arg[2]), *w = tensor(arg[3]);
+  Place at;
+  cppmega_mi355_gated_gemm_bwd_args_t a;
+  if (!dy || !pre || !x || !w || !at.take(*x) || !is_half(*x)) DECLINE;
+  for (const Tensor* t : {dy, pre, w})
+    if (t->scalar_type() != x->scalar_type() || !at.dense(*t)) DECLINE;
+  if (!ffn_operands(at, *x, *w, arg[4], a) || w->size(-1) != a.k || w->size(-2) % 2) DECLINE;
+  a.n = (int32_t)(w->size(-2) / 2);
+  if (!has_shape(*dy, {a.rows, a.n}) || !has_shape(*pre, {a.rows, 2ll * a.n})) DECLINE;
+  a.activation = (int32_t)as_int(arg[5]);
+  a.dtype = a.pre_dtype = a.dx_dtype = a.dw_dtype = code(x->scalar_type());
+  a.dy = dy->data_ptr(); a.pre = pre->data_ptr();
+  a.dy_pitch = a.n; a.pre_pitch = 2ll * a.n; a.dx_pitch = a.k;
+  size_t bytes = 0;
+  if (cppmega_mi355_gated_gemm_bwd_workspace_bytes(&a, sizeof(a), &bytes)) DECLINE;
+  Tensor scratch = at::empty({(int64_t)bytes}, x->options().dtype(at::kByte));   // (the call's own, as the norm's)
+  a.workspace = scratch.data_ptr();
+  a.workspace_bytes = bytes;
+  Tensor dx = at::empty({a.rows, a.k}, x->options()), dw = at::empty(w->sizes(), w->options());
+  a.dx = dx.data_ptr(); a.dw = dw.data_ptr();
+  if (unlocked([&] { return cppmega_mi355_gated_gemm_bwd(&a, sizeof(a), at.stream); })) DECLINE;
+  return tuple_of({dx, dw});
+}
+
+// fp8_gated_gemm(x, x_scale, w, w_scale, offsets or None, activation) -> y (bfloat16) or None
+PyObject* fp8_gated_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 6 || !PyLong_CheckExact(arg[5])) DECLINE;
+  const Tensor *x = tensor(arg[0]), *xs = tensor(arg[1]), *w = tensor(arg[2]), *ws = tensor(arg[3]);
+  Place at;
+  cppmega_mi355_gated_gemm_args_t a;
+  if (!x || !xs || !w || !ws || !at.take(*x) || x->scalar_type() != ScalarType::Byte || w->scalar_type() != ScalarType::Byte) DECLINE;
+  if (!ffn_operands(at, *x, *w, arg[4], a) || w->size(-1) != a.k || w->size(-2) % 2) DECLINE;
+  a.n = (int32_t)(w->size(-2) / 2);
+  a.activation = (int32_t)as_int(arg[5]);
+  const int64_t blocks_n = ((int64_t)a.n + 127) / 128, blocks_k = ((int64_t)a.k + 127) / 128;
+  for (const Tensor* t : {xs, ws})
+    if (!at.dense(*t) || t->scalar_type() != ScalarType::Float) DECLINE;
+  if (has_shape(*xs, {a.rows, blocks_k})) a.x_scale_block = 128;
+  else if (!has_shape(*xs, {a.rows})) DECLINE;
+  if (!(a.offsets ? has_shape(*ws, {a.experts, 2, blocks_n, blocks_k}) : has_shape(*ws, {2, blocks_n, blocks_k}))) DECLINE;
+  Tensor y = at::empty({a.rows, a.n}, x->options().dtype(at::kBFloat16));
+  a.x_dtype = CPPMEGA_MI355_E4M3;
+  a.y_dtype = CPPMEGA_MI355_BF16;
+  a.x_scale = (const float*)xs->data_ptr(); a.w_scale = (const float*)ws->data_ptr();
+  a.y = y.data_ptr();
+  a.y_pitch = a.n;
+  if (unlocked([&] { return cppmega_mi355_gated_gemm(&a, sizeof(a), at.stream); })) DECLINE;
+  return wrap(y);
+}
+
+// w4_gemm(x, w, scale, bias or None, offsets or None, activation or -1) -> y or None
+PyObject* w4_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+  if (n != 6 || !PyLong_CheckExact(arg[5])) DECLINE;
+  const Tensor *x = tensor(arg[0]), *w = tensor(arg[1]), *scale = tensor(arg[2]), *bias = tensor(arg[3]);
+  Place at;
+  cppmega_mi355_w4_gemm_args_t a;
+  if (!x || !w || !scale || (!bias && arg[3] != Py_None) || !at.take(*x) || !is_half(*x) || w->scalar_type() != ScalarType::Byte) DECLINE;
+  if (!ffn_operands(at, *x, *w, arg[4], a) || 2 * w->size(-1) != a.k || !at.dense(*scale) || scale->dim() != w->dim()) DECLINE;
+  for (int64_t d = 0; d + 1 < w->dim(); ++d)
+    if (scale->size(d) != w->size(d)) DECLINE;
+  const int64_t groups = scale->size(-1);
+  const auto type = scale->scalar_type();
+  if (groups < 1 || a.k % groups || (type != ScalarType::Float && type != x->scalar_type())) DECLINE;
+  if (bias && (!at.dense(*bias) || bias->scalar_type() != type || bias->sizes() != scale->sizes())) DECLINE;
+  a.activation = (int32_t)as_int(arg[5]);
+  const bool gated = a.activation != CPPMEGA_MI355_GATE_NONE;
+  if (gated && w->size(-2) % 2) DECLINE;
+  a.n = (int32_t)(gated ? w->size(-2) / 2 : w->size(-2));
+  a.group = (int32_t)(a.k / groups);
+  a.x_dtype = a.y_dtype = code(x->scalar_type());
+  a.scale_dtype = code(type);
+  a.scale = scale->data_ptr();
+  if (bias) a.bias = bias->data_ptr();
+  Tensor y = at::empty({a.rows, a.n}, x->options());
+  a.y = y.data_ptr();
+  a.y_pitch = a.n;
+  if (unlocked([&] { return cppmega_mi355_w4_gemm(&a, sizeof(a), at.stream); })) DECLINE;
+  return wrap(y);
+}
+
 // ---- workspace of the Python launch helpers, release ---------------------------------------------
 // workspace(device, bytes, stream) -> tensor
 PyObject* workspace_of(PyObject*, PyObject* const* arg, Py_ssize_t n) {
@@ -861,6 +993,8 @@ PyMethodDef methods[] = {
     CALL("mla_backward", mla_backward), CALL("indexer_loss", indexer_loss),
     CALL("rms_norm", rms_norm),         CALL("rms_norm_bwd", rms_norm_bwd), CALL("grouped_gemm", grouped_gemm),
     CALL("grouped_gemm_bwd", grouped_gemm_bwd), CALL("grouped_fp8_gemm", grouped_fp8_gemm),
+    CALL("gated_gemm", gated_gemm),     CALL("gated_gemm_bwd", gated_gemm_bwd), CALL("fp8_gated_gemm", fp8_gated_gemm),
+    CALL("w4_gemm", w4_gemm),
     {"release_workspaces", release_workspaces, METH_NOARGS, "Give the kept scratch tensors back to torch's allocator."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Launch path of the per-step calls.", -1, methods};

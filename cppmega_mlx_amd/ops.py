@@ -1135,3 +1135,196 @@ def grouped_fp8_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_
     a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
     a.x_scale, a.w_scale = x_scale.data_ptr(), w_scale.data_ptr()
     return _grouped_call(a, out)
+
+
+# ---------------------------------------------------------------------------
+# feed-forward layer: the gated block, products with 4-bit weights
+# ---------------------------------------------------------------------------
+_GATES = {"silu": _lib.GATE_SILU, "gelu_tanh": _lib.GATE_GELU_TANH}
+
+
+def gate_code(activation: str) -> int:
+    if activation not in _GATES:
+        raise ValueError(f"activation must be one of {sorted(_GATES)}; got {activation!r}")
+    return _GATES[activation]
+
+
+def _ffn_rows(a, x: torch.Tensor, offsets: torch.Tensor | None, experts: int, n: int, k: int, most: int) -> None:
+    """Sizes and the rows' experts; without offsets one expert has all rows."""
+    if n < 1 or k < 1 or n > most or k > _lib.GROUPED_MAX_SIZE or experts > _lib.GROUPED_MAX_SIZE:   # (here: the argument block holds 32 bits of them)
+        raise ValueError(f"{experts} experts, {n} outputs, {k} channels: 1 to {most} outputs and 2^30 channels are served")
+    a.struct_size = C.sizeof(a)
+    if offsets is None:
+        if experts != 1:
+            raise ValueError(f"offsets are needed for {experts} experts")
+        a.offsets_dtype = _lib.I32
+    else:
+        _lib.require_device_tensor(offsets, "offsets", x)
+        a.offsets_dtype = _dtype_or_raise(offsets, "offsets", (_lib.I32, _lib.I64))
+        if tuple(offsets.shape) != (experts + 1,):
+            raise ValueError(f"offsets must have shape {(experts + 1,)} for {experts} experts; got {tuple(offsets.shape)}")
+        a.offsets = offsets.data_ptr()
+    a.rows, a.experts, a.n, a.k = x.shape[0], experts, n, k
+
+
+def _stacked(w: torch.Tensor, name: str, offsets: torch.Tensor | None, ref: torch.Tensor) -> tuple[int, int, int]:
+    """(experts, rows, bytes or channels) of weights [E, R, C], or [R, C] without offsets."""
+    _lib.require_device_tensor(w, name, ref)
+    if w.ndim != (2 if offsets is None else 3):
+        raise ValueError(f"{name} must be {'[rows, channels] without offsets' if offsets is None else '[experts, rows, channels]'}; got {tuple(w.shape)}")
+    return (1, *w.shape) if offsets is None else tuple(w.shape)
+
+
+def _half_rows(x: torch.Tensor) -> None:
+    _lib.require_rows(x, "x")
+    if x.ndim != 2 or x.dtype not in _HALF:
+        raise TypeError(f"x must be a 2D float16 or bfloat16 tensor of rows; got {x.dtype} {tuple(x.shape)}")
+
+
+def _gated_weights(w: torch.Tensor, offsets: torch.Tensor | None, x: torch.Tensor) -> tuple[int, int, int]:
+    """(experts, outputs, channels) of the gate's and the up projection's rows."""
+    experts, both, k = _stacked(w, "w", offsets, x)
+    if both % 2:
+        raise ValueError(f"w must hold as many rows of the gate as of the up projection; got {tuple(w.shape)}")
+    return experts, both // 2, k
+
+
+def gated_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *, activation: str, out: torch.Tensor,
+               pre: torch.Tensor | None = None, x_scale: torch.Tensor | None = None, w_scale: torch.Tensor | None = None,
+               zero_tail: bool = False) -> torch.Tensor:
+    """out[t, j] = act(x[t] . w[e(t), j]) (x[t] . w[e(t), n + j]) into caller-owned ``out`` [T, n]; ``pre`` [T, 2 n] takes the two products.
+
+    uint8 ``x`` and ``w`` are e4m3 codes with float32 ``x_scale`` [T] or [T, ceil(K / 128)] and ``w_scale`` [E, 2, ceil(n / 128), ceil(K / 128)]."""
+    fp8 = isinstance(x, torch.Tensor) and x.dtype == torch.uint8
+    a = _lib.GatedGemmArgs()
+    a.activation = gate_code(activation)
+    if fp8:
+        _lib.require_rows(x, "x")
+        if x.ndim != 2:
+            raise ValueError(f"x must be [T, K]; got {tuple(x.shape)}")
+    else:
+        _half_rows(x)
+    experts, n, k = _gated_weights(w, offsets, x)
+    if w.dtype != x.dtype:
+        raise TypeError(f"w must be {x.dtype} like x; got {w.dtype}")
+    T = int(x.shape[0])
+    _ffn_rows(a, x, offsets, experts, n, k, _lib.GATED_MAX_OUTPUTS)
+    a.x_dtype = _lib.dtype_code(x)
+    a.x_pitch = _rows2d(x, "x", (T, k))
+    a.y_pitch = _rows2d(out, "out", (T, n), x)
+    _own_rows(out, "out", T, a.y_pitch)
+    a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, _lib.F16, _lib.BF16) if fp8 else (_lib.F32, a.x_dtype))
+    if pre is not None:
+        if fp8:
+            raise TypeError("the products of e4m3 operands are not kept")
+        a.pre_pitch = _rows2d(pre, "pre", (T, 2 * n), x)
+        _own_rows(pre, "pre", T, a.pre_pitch)
+        a.pre_dtype = _dtype_or_raise(pre, "pre", (_lib.F32, a.x_dtype))
+        a.pre = pre.data_ptr()
+    if fp8:
+        blocks_n, blocks_k = (n + 127) // 128, (k + 127) // 128
+        want = (2, blocks_n, blocks_k) if offsets is None else (experts, 2, blocks_n, blocks_k)
+        for name, t in (("x_scale", x_scale), ("w_scale", w_scale)):
+            _lib.require_device_tensor(t, name, x)
+            if t.dtype != torch.float32:
+                raise TypeError(f"{name} must be float32; got {t.dtype}")
+        if tuple(x_scale.shape) == (T, blocks_k):
+            a.x_scale_block = 128
+        elif tuple(x_scale.shape) != (T,):
+            raise ValueError(f"x_scale must have shape {(T,)} or {(T, blocks_k)}; got {tuple(x_scale.shape)}")
+        if tuple(w_scale.shape) != want:
+            raise ValueError(f"w_scale must have shape {want}; got {tuple(w_scale.shape)}")
+        a.x_scale, a.w_scale = x_scale.data_ptr(), w_scale.data_ptr()
+    elif x_scale is not None or w_scale is not None:
+        raise ValueError("scales go with e4m3 codes only")
+    a.x, a.w, a.y, a.zero_tail = x.data_ptr(), w.data_ptr(), out.data_ptr(), int(bool(zero_tail))
+    with torch.cuda.device(x.device):
+        rc = _lib.load().cppmega_mi355_gated_gemm(C.byref(a), C.sizeof(a), _lib.current_stream(x.device))
+    _lib.check(rc, "gated_gemm")
+    _written(out, pre)
+    return out
+
+
+def gated_gemm_backward(dy: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *, activation: str,
+                        dx: torch.Tensor | None, dw: torch.Tensor | None, zero_tail: bool = False, workspace: torch.Tensor | None = None) -> None:
+    """Gradients of :func:`gated_gemm` from the products it kept, into caller-owned ``dx`` [T, K] and ``dw`` (like w); None: not wanted.
+    Scratch belongs to the call (to the graph, within a capture)."""
+    a = _lib.GatedGemmBwdArgs()
+    a.activation = gate_code(activation)
+    _half_rows(x)
+    experts, n, k = _gated_weights(w, offsets, x)
+    T = int(x.shape[0])
+    for name, t in (("w", w), ("dy", dy)):
+        if t.dtype != x.dtype:
+            raise TypeError(f"{name} must be {x.dtype} like x; got {t.dtype}")
+    _ffn_rows(a, x, offsets, experts, n, k, _lib.GATED_MAX_OUTPUTS)
+    a.dtype = _lib.dtype_code(x)
+    a.x_pitch = _rows2d(x, "x", (T, k))
+    a.dy_pitch = _rows2d(dy, "dy", (T, n), x)
+    a.pre_pitch = _rows2d(pre, "pre", (T, 2 * n), x)
+    a.pre_dtype = _dtype_or_raise(pre, "pre", (_lib.F32, a.dtype))
+    if dx is not None:
+        a.dx_pitch = _rows2d(dx, "dx", (T, k), x)
+        _own_rows(dx, "dx", T, a.dx_pitch)
+        a.dx_dtype = _dtype_or_raise(dx, "dx", (_lib.F32, a.dtype))
+    if dw is not None:
+        _lib.require_device_tensor(dw, "dw", x)
+        if tuple(dw.shape) != tuple(w.shape):
+            raise ValueError(f"dw must have shape {tuple(w.shape)}; got {tuple(dw.shape)}")
+        a.dw_dtype = _dtype_or_raise(dw, "dw", (_lib.F32, a.dtype))
+    a.dy, a.pre, a.x, a.w, a.dx, a.dw = dy.data_ptr(), pre.data_ptr(), x.data_ptr(), w.data_ptr(), _lib.ptr(dx), _lib.ptr(dw)
+    a.zero_tail = int(bool(zero_tail))
+    lib = _lib.load()
+    need = C.c_size_t(0)
+    _lib.check(lib.cppmega_mi355_gated_gemm_bwd_workspace_bytes(C.byref(a), C.sizeof(a), C.byref(need)), "gated_gemm_bwd")
+    if need.value:
+        if workspace is None:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        else:
+            _lib.require_device_tensor(workspace, "workspace", x)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    with torch.cuda.device(x.device):
+        rc = lib.cppmega_mi355_gated_gemm_bwd(C.byref(a), C.sizeof(a), _lib.current_stream(x.device))
+    _lib.check(rc, "gated_gemm_bwd")
+    _written(dx, dw)
+
+
+def w4_gemm(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None, offsets: torch.Tensor | None, *, out: torch.Tensor,
+            activation: str | None = None, zero_tail: bool = False) -> torch.Tensor:
+    """out[t, j] = sum_k x[t, k] (scale q + bias)[e(t), j, k] into caller-owned ``out``; with an activation the gated block over weights of
+    2 n rows.  ``w`` uint8 [E, n, K / 2], ``scale`` (and ``bias``) [E, n, K / G]; without offsets no leading axis."""
+    a = _lib.W4GemmArgs()
+    a.activation = _lib.GATE_NONE if activation is None else gate_code(activation)
+    _half_rows(x)
+    experts, n, half = _stacked(w, "w", offsets, x)
+    if w.dtype != torch.uint8:
+        raise TypeError(f"w must be uint8 (two 4-bit codes a byte); got {w.dtype}")
+    k = 2 * half
+    T = int(x.shape[0])
+    _lib.require_device_tensor(scale, "scale", x)
+    groups = int(scale.shape[-1]) if scale.ndim else 0
+    if tuple(scale.shape[:-1]) != tuple(w.shape[:-1]) or groups < 1 or k % groups or k // groups not in (32, 64, 128):
+        raise ValueError(f"scale must have shape {tuple(w.shape[:-1])} + (K / G,) with groups of G = 32, 64 or 128 of {k} channels; got {tuple(scale.shape)}")
+    if activation is not None:
+        if n % 2:
+            raise ValueError(f"w must hold as many rows of the gate as of the up projection; got {tuple(w.shape)}")
+        n //= 2
+    _ffn_rows(a, x, offsets, experts, n, k, _lib.GROUPED_MAX_SIZE if activation is None else _lib.GATED_MAX_OUTPUTS)
+    a.group = k // groups
+    a.x_dtype = _lib.dtype_code(x)
+    a.scale_dtype = _dtype_or_raise(scale, "scale", (_lib.F32, a.x_dtype))
+    if bias is not None:
+        _lib.require_device_tensor(bias, "bias", x)
+        if bias.dtype != scale.dtype or tuple(bias.shape) != tuple(scale.shape):
+            raise ValueError(f"bias must be {scale.dtype} with shape {tuple(scale.shape)} like scale; got {bias.dtype} {tuple(bias.shape)}")
+    a.x_pitch = _rows2d(x, "x", (T, k))
+    a.y_pitch = _rows2d(out, "out", (T, n), x)
+    _own_rows(out, "out", T, a.y_pitch)
+    a.y_dtype = _dtype_or_raise(out, "out", (_lib.F32, a.x_dtype))
+    a.x, a.w, a.scale, a.bias, a.y = x.data_ptr(), w.data_ptr(), scale.data_ptr(), _lib.ptr(bias), out.data_ptr()
+    a.zero_tail = int(bool(zero_tail))
+    with torch.cuda.device(x.device):
+        rc = _lib.load().cppmega_mi355_w4_gemm(C.byref(a), C.sizeof(a), _lib.current_stream(x.device))
+    _lib.check(rc, "w4_gemm")
+    _written(out)
+    return out

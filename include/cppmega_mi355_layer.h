@@ -96,7 +96,7 @@ typedef struct cppmega_mi355_grouped_gemm_args {
   const void* x;
   const void* w;              /* [experts, n, k] dense; WEIGHTS_GRAD: [rows, k]              */
   void* y;                    /* WEIGHTS_GRAD: [experts, n, k] dense                         */
-  const void* offsets;        /* [experts + 1]                                               */
+  const void* offsets;        /* [experts + 1], or NULL: one expert (experts = 1) has all rows */
   const float* x_scale;       /* E4M3                                                        */
   const float* w_scale;       /* E4M3                                                        */
   int32_t x_dtype;            /* BF16 / F16 / E4M3; w alike                                  */

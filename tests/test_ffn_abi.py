@@ -1,0 +1,129 @@
+"""The third header of the C ABI (feed-forward layer): symbols, struct layouts, and the refusals that come before any launch, at the C
+boundary and in the Python entry points.  No GPU is touched."""
+
+import ctypes as C
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from cppmega_mlx_amd import _lib
+from cppmega_mlx_amd.nn import gated_ffn as gf, w4_gemm as w4
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "cppmega_mi355_ffn.h"
+STRUCTS = {
+    "cppmega_mi355_gated_gemm_args_t": _lib.GatedGemmArgs,
+    "cppmega_mi355_gated_gemm_bwd_args_t": _lib.GatedGemmBwdArgs,
+    "cppmega_mi355_w4_gemm_args_t": _lib.W4GemmArgs,
+}
+FAKE = 0x1000     # never dereferenced: validation fails first
+
+
+def test_library_exports_every_declared_symbol():
+    text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
+    declared = set(re.findall(r"\b(cppmega_mi355_[a-z0-9_]+)\s*\(", text))
+    assert declared == set(_lib.FFN_SYMBOLS)
+    lib = _lib.load()
+    for name in declared:
+        assert hasattr(lib, name), name
+    assert f"GATED_MAX_OUTPUTS {_lib.GATED_MAX_OUTPUTS}" in text
+    assert f"GATE_NONE = {_lib.GATE_NONE}" in text and f"GATE_SILU = {_lib.GATE_SILU}" in text and f"GATE_GELU_TANH = {_lib.GATE_GELU_TANH}" in text
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+def test_struct_layouts_match_the_header(tmp_path):
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void){"]
+    for ctype, struct in STRUCTS.items():
+        lines.append(f'printf("{ctype} size %zu\\n", sizeof({ctype}));')
+        lines += [f'printf("{ctype} {n} %zu\\n", offsetof({ctype}, {n}));' for n, _ in struct._fields_]
+    lines.append("return 0;}")
+    (tmp_path / "layout.c").write_text("\n".join(lines))
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", str(tmp_path / "layout.c"), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split("\n")
+    seen = 0
+    for line in filter(None, out):
+        ctype, name, value = line.split()
+        struct = STRUCTS[ctype]
+        assert (C.sizeof(struct) if name == "size" else getattr(struct, name).offset) == int(value), line
+        seen += 1
+    assert seen == sum(len(s._fields_) + 1 for s in STRUCTS.values())
+
+
+def _call(a, fn, over):
+    a.struct_size = C.sizeof(a)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return getattr(_lib.load(), fn)(C.byref(a), C.sizeof(a), None)
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(activation=2), _lib.ERR_SHAPE), (dict(activation=-1), _lib.ERR_SHAPE), (dict(n=0), _lib.ERR_SHAPE), (dict(n=_lib.GATED_MAX_OUTPUTS + 1), _lib.ERR_SHAPE),
+    (dict(n=(1 << 31) - 1), _lib.ERR_SHAPE), (dict(k=0), _lib.ERR_SHAPE), (dict(k=_lib.GROUPED_MAX_SIZE + 1), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(rows=1 << 29), _lib.ERR_SHAPE),
+    (dict(experts=0), _lib.ERR_SHAPE), (dict(experts=513), _lib.ERR_UNSUPPORTED), (dict(x_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(y_dtype=_lib.F16), _lib.ERR_DTYPE),
+    (dict(pre=FAKE, pre_dtype=_lib.F16), _lib.ERR_DTYPE), (dict(offsets_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(offsets=None), _lib.ERR_NULL), (dict(x=None), _lib.ERR_NULL), (dict(y=None), _lib.ERR_NULL),
+    (dict(w=None), _lib.ERR_NULL), (dict(x_dtype=_lib.E4M3), _lib.ERR_NULL), (dict(x_dtype=_lib.E4M3, pre=FAKE), _lib.ERR_DTYPE), (dict(x_dtype=_lib.E4M3, x_scale_block=64), _lib.ERR_SHAPE),
+    (dict(struct_size=16), _lib.ERR_STRUCT_SIZE), (dict(rows=0), _lib.OK), (dict(rows=0, experts=1, offsets=None), _lib.OK)])
+def test_gated_refusals(over, code):
+    a = _lib.GatedGemmArgs()
+    a.x = a.w = a.y = a.offsets = FAKE
+    a.x_dtype = a.y_dtype = a.pre_dtype = _lib.BF16
+    a.offsets_dtype = _lib.I32
+    a.rows, a.experts, a.n, a.k, a.x_pitch, a.y_pitch, a.pre_pitch = 4, 2, 64, 64, 64, 64, 128
+    assert _call(a, "cppmega_mi355_gated_gemm", over) == code
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(activation=2), _lib.ERR_SHAPE), (dict(n=0), _lib.ERR_SHAPE), (dict(n=_lib.GATED_MAX_OUTPUTS + 1), _lib.ERR_SHAPE), (dict(k=0), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE),
+    (dict(dtype=_lib.F32), _lib.ERR_DTYPE), (dict(pre_dtype=_lib.F16), _lib.ERR_DTYPE), (dict(dx_dtype=_lib.F16), _lib.ERR_DTYPE), (dict(dw_dtype=_lib.F16), _lib.ERR_DTYPE),
+    (dict(offsets_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(dy=None), _lib.ERR_NULL), (dict(pre=None), _lib.ERR_NULL), (dict(x=None), _lib.ERR_NULL), (dict(w=None), _lib.ERR_NULL),
+    (dict(offsets=None), _lib.ERR_NULL), (dict(workspace=None), _lib.ERR_WORKSPACE), (dict(workspace_bytes=16), _lib.ERR_WORKSPACE), (dict(workspace=FAKE + 2), _lib.ERR_ALIGNMENT),
+    (dict(experts=513), _lib.ERR_UNSUPPORTED), (dict(dx=None, dw=None), _lib.OK), (dict(rows=0, dw=None), _lib.OK)])
+def test_gated_gradient_refusals(over, code):
+    a = _lib.GatedGemmBwdArgs()
+    a.dy = a.pre = a.x = a.w = a.dx = a.dw = a.offsets = a.workspace = FAKE
+    a.dtype = a.pre_dtype = a.dx_dtype = a.dw_dtype = _lib.BF16
+    a.offsets_dtype = _lib.I32
+    a.rows, a.experts, a.n, a.k, a.dy_pitch, a.pre_pitch, a.x_pitch, a.dx_pitch, a.workspace_bytes = 4, 2, 63, 64, 63, 126, 64, 64, 1 << 20
+    a.struct_size = C.sizeof(a)
+    need = C.c_size_t(0)
+    lib = _lib.load()
+    assert lib.cppmega_mi355_gated_gemm_bwd_workspace_bytes(C.byref(a), C.sizeof(a), C.byref(need)) == _lib.OK and need.value == 4 * 128 * 2
+    assert lib.cppmega_mi355_gated_gemm_bwd_workspace_bytes(C.byref(a), C.sizeof(a), None) == _lib.ERR_NULL
+    assert _call(a, "cppmega_mi355_gated_gemm_bwd", over) == code
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(activation=2), _lib.ERR_SHAPE), (dict(activation=-2), _lib.ERR_SHAPE), (dict(n=0), _lib.ERR_SHAPE), (dict(n=_lib.GROUPED_MAX_SIZE + 1), _lib.ERR_SHAPE), (dict(activation=0, n=_lib.GATED_MAX_OUTPUTS + 1), _lib.ERR_SHAPE),
+    (dict(k=0), _lib.ERR_SHAPE), (dict(k=96), _lib.ERR_SHAPE), (dict(k=(1 << 31) - 64), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(rows=1 << 29), _lib.ERR_SHAPE), (dict(group=16), _lib.ERR_SHAPE),
+    (dict(group=256), _lib.ERR_SHAPE), (dict(experts=0), _lib.ERR_SHAPE), (dict(experts=513), _lib.ERR_UNSUPPORTED), (dict(x_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(y_dtype=_lib.F16), _lib.ERR_DTYPE),
+    (dict(scale_dtype=_lib.F16), _lib.ERR_DTYPE), (dict(offsets_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(x=None), _lib.ERR_NULL), (dict(w=None), _lib.ERR_NULL), (dict(scale=None), _lib.ERR_NULL),
+    (dict(y=None), _lib.ERR_NULL), (dict(offsets=None), _lib.ERR_NULL), (dict(struct_size=16), _lib.ERR_STRUCT_SIZE), (dict(rows=0), _lib.OK)])
+def test_w4_refusals(over, code):
+    a = _lib.W4GemmArgs()
+    a.x = a.w = a.scale = a.y = a.offsets = FAKE
+    a.x_dtype = a.y_dtype = a.scale_dtype = _lib.BF16
+    a.activation, a.offsets_dtype = _lib.GATE_NONE, _lib.I32
+    a.rows, a.experts, a.n, a.k, a.group, a.x_pitch, a.y_pitch = 4, 2, 64, 128, 64, 128, 64
+    assert _call(a, "cppmega_mi355_w4_gemm", over) == code
+
+
+def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
+    x, w, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    pre, dy, codes, scale = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=torch.bfloat16)
+    for call in (lambda: gf.gated_gemm(x, w), lambda: gf.gated_gemm(x, w[None], off), lambda: gf.gated_gemm_bwd(dy, pre, x, w), lambda: gf.gated_gemm_apply(x, w),
+                 lambda: gf.fp8_gated_gemm(x.to(torch.uint8), torch.ones(4), w.to(torch.uint8), torch.ones(2, 1, 1)), lambda: w4.w4_gemm(x, codes, scale),
+                 lambda: w4.w4_gated_gemm(x, codes, scale), lambda: w4.w4_gemm(x, codes[None], scale[None], None, off)):
+        with pytest.raises(_lib.NativeCallError, match="no CPU path"):
+            call()
+    for call in (lambda: gf.gated_gemm(x, w, activation="relu"), lambda: gf.gated_gemm_bwd(dy, pre, x, w, activation="relu"), lambda: w4.w4_gated_gemm(x, codes, scale, activation="relu")):
+        with pytest.raises(ValueError, match="activation must be one of"):
+            call()
+    with pytest.raises(ValueError, match=r"w must be \[E, 2 F, K\]"):
+        gf.gated_gemm(x, w, off)
+    with pytest.raises(ValueError, match="w must be"):
+        gf.gated_gemm(x, w[:7])
+    with pytest.raises(ValueError, match="w must be"):
+        w4.w4_gemm(x, codes, scale, None, off)
