@@ -82,6 +82,7 @@ FFN_SYMBOLS = (
     "cppmega_mi355_w4_gemm",
 )
 GATED_MAX_OUTPUTS = 1 << 29           # CPPMEGA_MI355_GATED_MAX_OUTPUTS
+W4_MAX_CHANNELS = 1 << 24             # CPPMEGA_MI355_W4_MAX_CHANNELS
 # activations of the gated block
 GATE_NONE, GATE_SILU, GATE_GELU_TANH = -1, 0, 1
 

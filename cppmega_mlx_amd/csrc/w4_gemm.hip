@@ -2,12 +2,16 @@
 //
 //   y[t, n] = sum_k x[t, k] (s[n, g] q[n, k] + b[n, g]),  g = k / G;  without biases b = -8 s
 //
-// Bound by memory: the weights pass once.  A workgroup has 16 TM rows of one expert and 16 TN rows of its weight (gated: half of them
-// the gate's); its wavefronts divide the contraction, and their sums meet in LDS once at the end, added in order.
+// Bound by memory and by the vector instructions that widen the codes: the weights pass once.  A workgroup has 16 rows of x of one expert and one or
+// more runs of 16 TN rows of its weight (gated: 16 of the gate's and 16 of the up projection's), a run to a wavefront; the others divide the
+// contraction, and their sums meet in LDS once at the end, added in order.  A wavefront has 8 KiB of weights on their way and nothing else: loads
+// return in the order in which they were asked for, and rows of x, from the cache but behind weights, waited for memory.  x passes through LDS
+// instead, as much of it at a time as there is room, in the codes' order.
+//
 // Four bits become 16 + q in 16 bits by a shift and an and-or, two at a time: q lies where float16 and bfloat16 between 16 and 32 have their
 // next four bits.  Products are exact; 16 times a group's sum of x comes off again in float32 with the bias,
-//   sum over a group = s (sum x (16 + q)) + (b - 16 s) (sum x),
-// where sum x comes from the matrix cores too (times ones), once for all of a workgroup's weights.
+//   y = sum over groups of s (sum x (16 + q)) + (b - 16 s) (sum x),
+// the second part a product of its own with float32 operands, four steps to a matrix instruction.
 // x is the first operand: a lane has one row of the weight in every sum, and with it one scale and one bias.
 // A step is 128 channels, 16 bytes (32 codes) a lane; a word of it is eight channels, of which the low and the high half of a register
 // take those four apart, so the pieces of x are put in that order.  With groups below 128 the four words of the four lanes of a row change
@@ -16,24 +20,26 @@
 #include <string.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "grouped_gemm.h"
 
 namespace cm {
 namespace {
 
-constexpr int kMostWaves = 8;
+constexpr int kMostWaves = 8, kRoom = 8192;                      // wavefronts of a workgroup; bytes of LDS that each of them brings for x
 
 struct W4Params {
   GroupedParams g;                                               // (w, scales: of 2 n rows when gated)
   const void *scale, *bias;
-  int gated;
+  int gated, log_split;                                          // wavefronts that divide the contraction
+  int tile0;                                                     // the launch's first 16 rows
 };
 
 // Eight codes as 16 + q in 16 bits, in the order 0 4 1 5 2 6 3 7.
 template <bool F16>
-__device__ __forceinline__ bf16x8 widen(unsigned w) {
-  constexpr unsigned mask = F16 ? 0x03c003c0u : 0x00780078u, one = F16 ? 0x4c004c00u : 0x41804180u;
+__device__ __forceinline__ bf16x8 widen(unsigned w, unsigned one) {        // (one: 16 twice, from a vector register, so that and-or is one instruction)
+  constexpr unsigned mask = F16 ? 0x03c003c0u : 0x00780078u;
   u32x4 r;
   if (F16) r = u32x4{w << 6, w << 2, w >> 2, w >> 6};
   else r = u32x4{w << 3, w >> 1, w >> 5, w >> 9};
@@ -53,204 +59,289 @@ __device__ __forceinline__ void transpose4(u32x4& w) {
   w = u32x4{c[0], c[1], d[0], d[1]};
 }
 
+// A value of quad Q's lanes in the lanes of all quads (of the same place).
+template <int Q>
+__device__ __forceinline__ unsigned of_quad(unsigned v) {
+  const u32x2 a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_permlane16_swap(a[Q >> 1], a[Q >> 1], false, false)[Q & 1];
+}
+
+template <int N>
+using Count = std::integral_constant<int, N>;
+template <int... I, class F>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) { (f(Count<I>()), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F f) { each(std::make_integer_sequence<int, N>(), f); }
+
 // The scales (or biases) of N consecutive groups as they are stored, S bytes each.
 template <int N, int S>
 struct Groups {
-  unsigned v[(N * S + 3) / 4];
-  __device__ __forceinline__ void load(const void* base, size_t at) { __builtin_memcpy(v, (const char*)base + at * S, N * S); }
-  __device__ __forceinline__ void load_part(const void* base, size_t at, int left) {       // zeros for groups that are not there
+  static constexpr int kWords = (N * S + 3) / 4;
+  unsigned v[kWords];
+  __device__ __forceinline__ void load(const char* at) { __builtin_memcpy(v, at, N * S); }
+  __device__ __forceinline__ void load_part(const char* at, int left) {         // zeros for groups that are not there
 #pragma unroll
-    for (int i = 0; i < (N * S + 3) / 4; ++i) v[i] = 0u;
+    for (int i = 0; i < kWords; ++i) v[i] = 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i >= left) continue;
-      if (S == 4) v[i] = ((const unsigned*)base)[at + i];
-      else v[i / 2] |= (unsigned)((const unsigned short*)base)[at + i] << (16 * (i & 1));
+      if (S == 4) v[i] = *(const unsigned*)(at + 4 * i);
+      else v[i / 2] |= (unsigned)*(const unsigned short*)(at + 2 * i) << (16 * (i & 1));
     }
   }
+  // the second half in the first one's place
+  __device__ __forceinline__ void drop_half(bool yes) {
+    constexpr int kHalf = N * S / 8;
+    if constexpr (kHalf == 0) v[0] = yes ? v[0] >> 16 : v[0];
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) v[i] = yes ? v[i + kHalf] : v[i];
+  }
   template <bool F16>
-  __device__ __forceinline__ float get(int i) const {
-    if (S == 4) return __uint_as_float(v[i]);
-    const unsigned short b = (unsigned short)(v[i / 2] >> (16 * (i & 1)));
+  static __device__ __forceinline__ float value(unsigned word, int i) {
+    if (S == 4) return __uint_as_float(word);
+    const unsigned short b = (unsigned short)(word >> (16 * (i & 1)));
     return F16 ? f16_bits_to_f32(b) : bf16_bits_to_f32(b);
   }
 };
 
 // S: bytes of a scale.
-template <int G, int TN, int TM, bool F16, int S>
-__global__ __launch_bounds__(64 * kMostWaves, 2) void w4_kernel(const W4Params p) {
-  constexpr int kSteps = TM == 1 && G > 32 ? 2 : 1;                        // (two rounds of operands are in registers)
-  constexpr int kRound = 128 * kSteps, kGroups = kRound / G;     // channels and groups of a round
-  constexpr int kIn = G / 32;                                    // matrix instructions to a group
+template <int G, bool F16, int S>
+__global__ __launch_bounds__(64 * kMostWaves, 4) void w4_kernel(const W4Params p) {
+  constexpr int kIn = G / 32, kPer = 4 / kIn;                    // 32s of channels in a group, groups in a step
   constexpr bool SWAP = G < 128;
-  extern __shared__ f32x4 sums[];                                // [wavefronts][TM][TN][64]
+  extern __shared__ u32x4 smem[];                                // x, afterwards the sums
   const GroupedParams& q = p.g;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = (int)blockDim.x >> 6;
   const int l16 = lane & 15, quad = lane >> 4;
-  const int to = p.gated ? TN / 2 : TN;                          // outputs of a workgroup, in 16s
-  const int tiles_n = (q.n + 16 * to - 1) / (16 * to);
-  const int mt = (int)(blockIdx.x / (unsigned)tiles_n), n0 = (int)(blockIdx.x % (unsigned)tiles_n) * 16 * to;
-  int e, first, rows;
-  if (!rows_of_tile<16 * TM>(q, mt, e, first, rows)) return;
-  const int expert = e < q.experts ? e : 0;
-  const int groups = q.k / G;
-  const int rounds = e < q.experts ? (q.k + kRound - 1) / kRound : 0, whole = q.k / kRound;
-  const int r0 = (int)((long long)rounds * wave / waves), r1 = (int)((long long)rounds * (wave + 1) / waves);
+  const int split = 1 << p.log_split, tiles = waves >> p.log_split, tile = wave >> p.log_split, slice = wave & (split - 1);
+  const int to = p.gated ? tiles >> 1 : tiles;                   // outputs of a workgroup, in 16s
+  const int up = tile >= to ? 1 : 0, n0 = ((int)blockIdx.x * to + tile - up * to) * 16;
+  const int mt = p.tile0 + (int)blockIdx.y;
+  int e = 0, first = mt * 16, rows = (int)(q.rows - first);
+  if (q.offsets && !rows_of_tile<16>(q, mt, e, first, rows)) return;
+  e = __builtin_amdgcn_readfirstlane(e);
+  first = __builtin_amdgcn_readfirstlane(first);
+  rows = __builtin_amdgcn_readfirstlane(rows < 16 ? rows : 16);
+  const bool there = e < q.experts;
+  const int groups = q.k / G, pitch = q.k >> 1, steps = there ? q.k / 128 : 0;
 
-  const char* wat[TN];
-  size_t sat[TN];
+  // ---- passes of x through LDS: rows of it, as a power of two, and steps of a wavefront (whole blocks of eight where there is room) ----
+  const int log_rows = rows > 1 ? 32 - __builtin_clz(rows - 1) : 0, row_mask = (1 << log_rows) - 1;
+  const int room = waves * kRoom >> (log_rows + 8 + p.log_split), most = room >= 8 ? room & ~7 : room;
+  const int per_pass = most << p.log_split;
+  const char* const xb = (const char*)q.x + (size_t)first * q.x_pitch * 2;
+  // piece o (eight channels) of row r of a pass: a row's pieces lie in different banks, and so do the rows' of one piece
+  auto place = [&](int o, int r) { return (o << log_rows) + ((r ^ o) & row_mask); };
+  unsigned xo[4];                                                // a lane's pieces of a step
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int up = j >= to ? 1 : 0, n = n0 + (j - (up ? to : 0)) * 16 + l16;
-    const size_t row = (size_t)expert * (p.gated ? 2 : 1) * q.n + (n < q.n ? n : q.n - 1) + (up ? q.n : 0);
-    wat[j] = (const char*)q.w + row * (q.k >> 1) + quad * 16;
-    sat[j] = row * groups;
-  }
-  const char* xat[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = i * 16 + l16;                                // (rows past the end repeat the last one and are not stored)
-    xat[i] = (const char*)q.x + ((size_t)(first + (row < rows ? row : rows - 1)) * q.x_pitch + quad * (SWAP ? 8 : 32)) * 2;
-  }
+  for (int c = 0; c < 4; ++c) xo[c] = (unsigned)place(SWAP ? c * 4 + quad : quad * 4 + c, l16) * 16u;
 
-  f32x4 acc[TM][TN];
+  // ---- where operands lie: a place that the wavefront shares, and 32 bits of the lane ----
+  const int n1 = n0 < q.n ? n0 : q.n - 1, row = n0 + l16 < q.n ? l16 : q.n - 1 - n1;
+  const size_t weight = (size_t)(there ? e : 0) * (p.gated ? 2 : 1) * q.n + (up ? q.n : 0) + n1;
+  const char* const wt = (const char*)q.w + weight * pitch;
+  const char* const st = (const char*)p.scale + weight * groups * S;
+  const char* const bt = (const char*)p.bias + weight * groups * S;
+  const unsigned wo = (unsigned)row * (unsigned)pitch + (unsigned)quad * 16u, go = (unsigned)row * (unsigned)groups * S;
+
+  const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc = zero;
+  typedef Groups<2 * kPer, S> Pair;                              // of two steps: quad i has steps 2 i and 2 i + 1 of a block
+  u32x4 w[8];
+  Pair scale, bias;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  u32x4 w[2][TN][kSteps], x[2][TM][4 * kSteps];
-  Groups<kGroups, S> s[2][TN], b[2][TN];
-  // Round r into buffer `at`.  PART: the last one, of which a part may not be there: zeros for x, of which nothing is added.
-  auto load = [&](int r, int at, auto part) __attribute__((always_inline)) {
-    constexpr bool PART = decltype(part)::value;
-    const int left = q.k - r * kRound;                           // channels from this round on
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-#pragma unroll
-      for (int h = 0; h < kSteps; ++h) {
-        if (!PART || h * 128 + quad * 32 < left) __builtin_memcpy(&w[at][j][h], wat[j] + (size_t)r * (kRound / 2) + h * 64, 16);
-        else w[at][j][h] = u32x4{0u, 0u, 0u, 0u};
-      }
-      const size_t group = sat[j] + (size_t)r * kGroups;
-      if (PART) s[at][j].load_part(p.scale, group, left / G);
-      else s[at][j].load(p.scale, group);
-      if (p.bias) {
-        if (PART) b[at][j].load_part(p.bias, group, left / G);
-        else b[at][j].load(p.bias, group);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int c = 0; c < 4 * kSteps; ++c) {
-        // channels of this lane's piece: of 32 in a run (SWAP), or of its 32 of a step
-        const int in = (c >> 2) * 128 + (SWAP ? (c & 3) * 32 : (c & 3) * 8), first_k = in + quad * (SWAP ? 8 : 32);
-        if (!PART || first_k < left) __builtin_memcpy(&x[at][i][c], xat[i] + ((size_t)r * kRound + in) * 2, 16);
-        else x[at][i][c] = u32x4{0u, 0u, 0u, 0u};
-      }
-  };
+  for (int i = 0; i < Pair::kWords; ++i) bias.v[i] = 0u;
+  const float shift = p.bias ? -16.0f : -24.0f;
+  unsigned sixteen = F16 ? 0x4c004c00u : 0x41804180u;
+  asm("" : "+v"(sixteen));
   const bf16x8 ones = __builtin_bit_cast(bf16x8, F16 ? u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  auto multiply = [&](int at) __attribute__((always_inline)) {
-    if (SWAP)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int h = 0; h < kSteps; ++h) transpose4(w[at][j][h]);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      f32x4 t[TM][TN], sum[TM];
-#pragma unroll
-      for (int c = g * kIn; c < (g + 1) * kIn; ++c) {
-        bf16x8 xv[TM];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          xv[i] = reorder(x[at][i][c]);
-          sum[i] = mm<F16>(xv[i], ones, c == g * kIn ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : sum[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const bf16x8 wv = widen<F16>(w[at][j][c >> 2][c & 3]);
-#pragma unroll
-          for (int i = 0; i < TM; ++i) t[i][j] = mm<F16>(xv[i], wv, c == g * kIn ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : t[i][j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const float f = s[at][j].template get<F16>(g), off = p.bias ? fmaf(-16.0f, f, b[at][j].template get<F16>(g)) : -24.0f * f;
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[i][j][v] = fmaf(f, t[i][j][v], fmaf(off, sum[i][v], acc[i][j][v]));
-      }
+
+  // A wavefront's steps of a pass: the first one's place in the row, how many there are from there on.
+  auto share = [&](int base, int& from, int& left) {
+    const int count = steps - base < per_pass ? steps - base : per_pass, s0 = (count * slice) >> p.log_split;
+    from = base + s0;
+    left = ((count * (slice + 1)) >> p.log_split) - s0;
+  };
+  auto load_w = [&](u32x4& to_w, int s) __attribute__((always_inline)) { __builtin_memcpy(&to_w, wt + (size_t)s * 64 + wo, 16); };
+  // Groups of a block's steps.  The row's last step may be the first of a pair: then it is read as the second one of the pair before.
+  auto load_groups = [&](int from, int here) __attribute__((always_inline)) {
+    const int i = 2 * quad < here ? 2 * quad : here - 1;
+    if (steps > 1) {
+      const bool end = from + i + 1 == steps;
+      const unsigned at = (unsigned)(from + i - (end ? 1 : 0)) * (kPer * S) + go;
+      scale.load(st + at);
+      if (p.bias) bias.load(bt + at);
+      scale.drop_half(end);
+      if (p.bias) bias.drop_half(end);
+    } else {
+      scale.load_part(st + go, kPer);
+      if (p.bias) bias.load_part(bt + go, kPer);
     }
   };
-  const std::integral_constant<bool, false> all;
-  const int end = whole < r1 ? whole : r1;
-  if (r0 < end) load(r0, 0, all);
-  for (int r = r0; r < end; r += 2) {
-    if (r + 1 < end) load(r + 1, 1, all);
-    multiply(0);
-    if (r + 1 < end) {
-      if (r + 2 < end) load(r + 2, 0, all);
-      multiply(1);
+  float sum[2 * kPer];                                           // of a block's groups of x, in the scales' order
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 2 * kPer; ++g) sum[g] = 0.0f;
+  };
+  // step I of a block, x's pieces given by `piece`
+  auto multiply = [&](auto step, auto piece) __attribute__((always_inline)) {
+    constexpr int I = decltype(step)::value;
+    if (SWAP) transpose4(w[I]);
+    f32x4 t, one;
+    each<4>([&](auto c_) __attribute__((always_inline)) {
+      constexpr int c = decltype(c_)::value, g = (I & 1) * kPer + c / kIn;
+      constexpr bool fresh = c % kIn == 0;
+      const bf16x8 xv = piece(c);
+      one = mm<F16>(ones, xv, fresh ? zero : one);
+      t = mm<F16>(xv, widen<F16>(w[I][c], sixteen), fresh ? zero : t);
+      if constexpr (c % kIn == kIn - 1) {
+        sum[g] = quad == I >> 1 ? one[0] : sum[g];
+        const float f = Pair::template value<F16>(of_quad<(I >> 1)>(scale.v[g * S / 4]), g);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[v] = fmaf(f, t[v], acc[v]);
+      }
+    });
+  };
+  // the part of a block that goes by the sums of x, as far as its steps go
+  auto shifts = [&](int here) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 2 * kPer; ++g) {
+      const bool mine = 2 * quad + (g >= kPer ? 1 : 0) < here;
+      const float off = mine ? fmaf(shift, Pair::template value<F16>(scale.v[g * S / 4], g), Pair::template value<F16>(bias.v[g * S / 4], g)) : 0.0f;
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[g], off, acc, 0, 0, 0);
+    }
+  };
+
+  // A thread brings up to eight pieces of a pass, of one row or (16 rows, eight wavefronts or fewer) of several; those past the end repeat the last one.
+  const int beside = waves * 64 >> log_rows > 64 ? waves * 64 >> log_rows : 64, log_each = waves * 64 >> log_rows >= 64 ? 3 : 31 - __builtin_clz(waves * 512 >> (log_rows + 6));
+  const int row0 = wave & row_mask, piece0 = (wave >> log_rows) * 64 + lane;
+  int from = 0, left = 0;
+  for (int base = 0; base < steps; base += per_pass) {
+    const int count = steps - base < per_pass ? steps - base : per_pass, last = count * 16 - 1;
+    if (base > 0) __syncthreads();
+    u32x4 v[4];
+    int o[4], r[4];
+    auto fetch = [&](int h) __attribute__((always_inline)) {      // four pieces
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = piece0 + ((4 * h + u) & ((1 << log_each) - 1)) * beside, x_row = row0 + ((4 * h + u) >> log_each) * waves;
+        o[u] = at < last ? at : last;
+        r[u] = x_row < rows ? x_row : rows - 1;
+        __builtin_memcpy(&v[u], xb + ((size_t)r[u] * q.x_pitch + (size_t)base * 128) * 2 + (unsigned)o[u] * 16u, 16);
+      }
+    };
+    auto put = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) smem[place(o[u], r[u])] = __builtin_bit_cast(u32x4, reorder(v[u]));
+    };
+    fetch(0);
+    if (log_each < 3 || last >= 4 * beside) {
+      put();
+      fetch(1);
+    }
+    if (base == 0) {                                             // (x is asked for before the first weights: it is needed first)
+      share(0, from, left);
+      if (left > 0) {
+        const int here = left < 8 ? left : 8;
+        load_groups(from, here);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_w(w[i], from + (i < here ? i : here - 1));
+      }
+    }
+    put();
+    __syncthreads();
+    // ---- this wavefront's blocks of it ----
+    while (left > 0) {
+      const int here = left < 8 ? left : 8;
+      int next = from + here, next_left = left - here;
+      if (next_left == 0 && base + per_pass < steps) share(base + per_pass, next, next_left);
+      const bool more = next_left > 0;
+      if (!more) next = from;                                    // (what is requested then is not used)
+      const int next_here = !more ? here : next_left < 8 ? next_left : 8;
+      const char* const at = (const char*)smem + ((unsigned)(from - base) << (log_rows + 8));
+      clear();
+      each<8>([&](auto i_) __attribute__((always_inline)) {
+        constexpr int i = decltype(i_)::value;
+        if (i < here) {
+          const char* const to_x = at + ((unsigned)i << (log_rows + 8));
+          multiply(i_, [&](int c) __attribute__((always_inline)) { return *reinterpret_cast<const bf16x8*>(to_x + xo[c]); });
+        }
+        load_w(w[i], next + (i < next_here ? i : next_here - 1));
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      shifts(here);
+      load_groups(next, next_here);
+      left -= here;
+      from = next;
+      if (left == 0) {                                           // (the next pass's, if there is one)
+        left = next_left;
+        break;
+      }
     }
   }
-  if (r0 <= whole && whole < r1) {
-    load(whole, 0, std::integral_constant<bool, true>());
-    multiply(0);
+  // channels behind the last whole step: the last slice's; zeros for those that are not there
+  const int rest = q.k & 127;
+  if (rest && there && slice == split - 1) {
+    const char* const at = xb + (size_t)(l16 < rows ? l16 : rows - 1) * q.x_pitch * 2 + (size_t)steps * 256 + quad * 16;
+    const unsigned group = (unsigned)steps * (kPer * S) + go;
+    scale.load_part(st + group, groups - steps * kPer);
+    if (p.bias) bias.load_part(bt + group, groups - steps * kPer);
+    w[0] = u32x4{0u, 0u, 0u, 0u};
+    if (quad * 32 < rest) load_w(w[0], steps);
+    clear();
+    multiply(Count<0>(), [&](int c) __attribute__((always_inline)) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (c * 32 < rest) __builtin_memcpy(&v, at + c * 64, 16);
+      return reorder(v);
+    });
+    shifts(1);
   }
 
-  // ---- the wavefronts' sums, in order; lane: weight row l % 16, rows 4 (l / 16) + 0..3 of a tile ----
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) sums[((wave * TM + i) * TN + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  auto sum_of = [&](int i, int j) {
-    f32x4 v = sums[(i * TN + j) * 64 + lane];
-    for (int k = 1; k < waves; ++k) v += sums[((k * TM + i) * TN + j) * 64 + lane];
+  // ---- the slices' sums, in order; lane: weight row l % 16, rows 4 (l / 16) + 0..3 ----
+  f32x4* const sums = reinterpret_cast<f32x4*>(smem);            // [tiles][slices][64]
+  if (split > 1 || p.gated) {
+    __syncthreads();
+    sums[wave * 64 + lane] = acc;
+    __syncthreads();
+  }
+  if (slice != 0 || up) return;
+  auto sum_of = [&](int t) {
+    f32x4 v = sums[(t << p.log_split) * 64 + lane];
+    for (int k = 1; k < split; ++k) v += sums[((t << p.log_split) + k) * 64 + lane];
     return v;
   };
-  for (int u = wave; u < TM * to; u += waves) {
-    const int i = u / to, j = u - i * to, n = n0 + j * 16 + l16;
-    f32x4 v = sum_of(i, j);
-    if (p.gated) {
-      const f32x4 up = sum_of(i, to + j);
+  f32x4 v = split > 1 || p.gated ? sum_of(tile) : acc;
+  if (p.gated) {
+    const f32x4 u = sum_of(to + tile);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = gated(v[c], up[c], q.activation);
-    }
-    if (n >= q.n) continue;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int row = i * 16 + quad * 4 + c;
-      if (row < rows) store_as(q.y, (size_t)(first + row) * q.y_pitch + n, q.y_dtype, v[c]);
-    }
+    for (int c = 0; c < 4; ++c) v[c] = gated(v[c], u[c], q.activation);
   }
+  const int n = n0 + l16;
+  if (n >= q.n) return;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (quad * 4 + c < rows) store_as(q.y, (size_t)(first + quad * 4 + c) * q.y_pitch + n, q.y_dtype, v[c]);
 }
 
 template <int G, bool F16, int S>
-int launch(const W4Params& p, hipStream_t stream) {
+int launch(W4Params p, hipStream_t stream) {
   const GroupedParams& q = p.g;
-  // rows to a workgroup: as many as an expert has on average, up to 32
-  const long long mean = (q.rows + q.experts - 1) / q.experts;
-  const int tm = mean <= 16 ? 1 : 2;
-  const long long bm = 16 * tm, tails = q.experts + 1 < q.rows ? q.experts + 1 : q.rows;
-  const long long tiles_m = !q.offsets ? (q.rows + bm - 1) / bm : q.rows / bm + tails < q.rows ? q.rows / bm + tails : q.rows;
-  auto tiles = [&](int tn) { return tiles_m * ((q.n + 16 * tn / (p.gated ? 2 : 1) - 1) / (16 * tn / (p.gated ? 2 : 1))); };
-  const int least = p.gated || tm > 1 ? 2 : 1;
-  const int tn = least < 2 && tiles(2) < 512 ? 1 : 2;
-  const long long count = tiles(tn);
-  const int rounds = tm == 1 && G > 32 ? (q.k + 255) / 256 : (q.k + 127) / 128;
-  int waves = 4;
-  while (waves < kMostWaves && waves < rounds && count * waves < 2048) waves *= 2;
-  if (int rc = check_tiles(count, 64 * waves)) return rc;
-  const dim3 grid((unsigned)count), block(64 * waves);
-  const size_t lds = (size_t)waves * tm * tn * 64 * sizeof(f32x4);
-#define CM_W4(tn_, tm_) hipLaunchKernelGGL((w4_kernel<G, tn_, tm_, F16, S>), grid, block, lds, stream, p)
-  if (tm == 2) CM_W4(2, 2);
-  else if (tn == 2) CM_W4(2, 1);
-  else CM_W4(1, 1);
-#undef CM_W4
+  const long long tails = q.experts + 1 < q.rows ? q.experts + 1 : q.rows;        // tiles of rows that are not full, at most
+  const long long tiles_m = !q.offsets ? (q.rows + 15) / 16 : q.rows / 16 + tails < q.rows ? q.rows / 16 + tails : q.rows;
+  const long long work = tiles_m * ((q.n + 15) / 16) * (p.gated ? 2 : 1);         // tiles of rows of x and of the weight
+  const int steps = q.k / 128;
+  const bool thin = q.rows <= 4 && q.experts == 1;
+  const int tiles = work >= 1024 && !thin ? 4 : work >= 512 || p.gated ? 2 : 1;
+  const int waves = work >= 4096 || steps * tiles < 32 ? 4 : 8;
+  p.log_split = __builtin_ctz(waves / tiles);
+  const int out = 16 * (p.gated ? tiles / 2 : tiles), parts = (q.n + out - 1) / out;
+  if (int rc = check_tiles(parts, 64 * waves)) return rc;
+  constexpr long long kMostY = 65535;                            // (of a grid)
+  for (long long t = 0; t < tiles_m; t += kMostY) {
+    p.tile0 = (int)t;
+    const dim3 grid((unsigned)parts, (unsigned)(tiles_m - t < kMostY ? tiles_m - t : kMostY));
+    hipLaunchKernelGGL((w4_kernel<G, F16, S>), grid, dim3(64 * waves), (size_t)waves * kRoom, stream, p);
+  }
   CM_HIP_CHECK(hipGetLastError());
   return 0;
 }
@@ -269,8 +360,11 @@ int w4_gemm_launch(const cppmega_mi355_w4_gemm_args_t& a, hipStream_t stream) {
     return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: unknown activation %d", a.activation);
   if (a.rows < 0 || a.rows > 0x1fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
     return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
-  if (a.n > (is_gated ? CPPMEGA_MI355_GATED_MAX_OUTPUTS : CPPMEGA_MI355_GROUPED_MAX_SIZE) || a.k > CPPMEGA_MI355_GROUPED_MAX_SIZE)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: n=%d k=%d, at most 2^30 weight rows and channels are served", a.n, a.k);
+  if (a.n > (is_gated ? CPPMEGA_MI355_GATED_MAX_OUTPUTS : CPPMEGA_MI355_GROUPED_MAX_SIZE))
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: n=%d, at most 2^30 weight rows are served", a.n);
+  // (a lane's place in a tile's rows is kept in 32 bits)
+  if (a.k > CPPMEGA_MI355_W4_MAX_CHANNELS || a.x_pitch < 0 || a.x_pitch > CPPMEGA_MI355_W4_MAX_CHANNELS)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: k=%d and rows of x %lld apart, at most 2^24 are served", a.k, (long long)a.x_pitch);
   if (a.experts > kMaxExperts) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "w4_gemm: %d experts, at most %d are served", a.experts, kMaxExperts);
   if (a.group != 32 && a.group != 64 && a.group != 128) return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: groups of %d, 32, 64 and 128 are served", a.group);
   if (a.k % a.group != 0) return fail(CPPMEGA_MI355_ERR_SHAPE, "w4_gemm: k=%d is no multiple of the group, %d", a.k, a.group);

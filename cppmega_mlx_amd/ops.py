@@ -1152,7 +1152,7 @@ def gate_code(activation: str) -> int:
 def _ffn_rows(a, x: torch.Tensor, offsets: torch.Tensor | None, experts: int, n: int, k: int, most: int) -> None:
     """Sizes and the rows' experts; without offsets one expert has all rows."""
     if n < 1 or k < 1 or n > most or k > _lib.GROUPED_MAX_SIZE or experts > _lib.GROUPED_MAX_SIZE:   # (here: the argument block holds 32 bits of them)
-        raise ValueError(f"{experts} experts, {n} outputs, {k} channels: 1 to {most} outputs and 2^30 channels are served")
+        raise ValueError(f"{experts} experts, {n} outputs, {k} channels: 1 to {most} outputs and up to 2^30 channels are served")
     a.struct_size = C.sizeof(a)
     if offsets is None:
         if experts != 1:

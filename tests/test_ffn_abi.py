@@ -29,7 +29,7 @@ def test_library_exports_every_declared_symbol():
     lib = _lib.load()
     for name in declared:
         assert hasattr(lib, name), name
-    assert f"GATED_MAX_OUTPUTS {_lib.GATED_MAX_OUTPUTS}" in text
+    assert f"GATED_MAX_OUTPUTS {_lib.GATED_MAX_OUTPUTS}" in text and f"W4_MAX_CHANNELS {_lib.W4_MAX_CHANNELS}" in text
     assert f"GATE_NONE = {_lib.GATE_NONE}" in text and f"GATE_SILU = {_lib.GATE_SILU}" in text and f"GATE_GELU_TANH = {_lib.GATE_GELU_TANH}" in text
 
 
@@ -97,7 +97,7 @@ def test_gated_gradient_refusals(over, code):
 
 @pytest.mark.parametrize("over, code", [
     (dict(activation=2), _lib.ERR_SHAPE), (dict(activation=-2), _lib.ERR_SHAPE), (dict(n=0), _lib.ERR_SHAPE), (dict(n=_lib.GROUPED_MAX_SIZE + 1), _lib.ERR_SHAPE), (dict(activation=0, n=_lib.GATED_MAX_OUTPUTS + 1), _lib.ERR_SHAPE),
-    (dict(k=0), _lib.ERR_SHAPE), (dict(k=96), _lib.ERR_SHAPE), (dict(k=(1 << 31) - 64), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(rows=1 << 29), _lib.ERR_SHAPE), (dict(group=16), _lib.ERR_SHAPE),
+    (dict(k=0), _lib.ERR_SHAPE), (dict(k=96), _lib.ERR_SHAPE), (dict(k=_lib.W4_MAX_CHANNELS + 64), _lib.ERR_SHAPE), (dict(x_pitch=_lib.W4_MAX_CHANNELS + 1), _lib.ERR_SHAPE), (dict(x_pitch=-128), _lib.ERR_SHAPE), (dict(rows=-1), _lib.ERR_SHAPE), (dict(rows=1 << 29), _lib.ERR_SHAPE), (dict(group=16), _lib.ERR_SHAPE),
     (dict(group=256), _lib.ERR_SHAPE), (dict(experts=0), _lib.ERR_SHAPE), (dict(experts=513), _lib.ERR_UNSUPPORTED), (dict(x_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(y_dtype=_lib.F16), _lib.ERR_DTYPE),
     (dict(scale_dtype=_lib.F16), _lib.ERR_DTYPE), (dict(offsets_dtype=_lib.F32), _lib.ERR_DTYPE), (dict(x=None), _lib.ERR_NULL), (dict(w=None), _lib.ERR_NULL), (dict(scale=None), _lib.ERR_NULL),
     (dict(y=None), _lib.ERR_NULL), (dict(offsets=None), _lib.ERR_NULL), (dict(struct_size=16), _lib.ERR_STRUCT_SIZE), (dict(rows=0), _lib.OK)])
