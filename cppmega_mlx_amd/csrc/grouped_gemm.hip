@@ -162,6 +162,12 @@ int gated_gemm_launch(const cppmega_mi355_gated_gemm_args_t& a, hipStream_t stre
   plan.p.n = a.n;
   plan.p.activation = a.activation;
   plan.p.pre = a.pre; plan.p.pre_dtype = a.pre_dtype; plan.p.pre_pitch = a.pre_pitch;
+  // Few tiles leave most CUs without work, and each goes through the whole contraction: the kernel that streams the weights has more
+  // workgroups, and passes them once for 16 rows.  Measured, us stream / tiles, rows x n x k of one expert: bf16 64 x 2048 x 4096 25 / 33, 128 x 2048 x 4096
+  // 39 / 33, 16 x 8192 x 2048 15 / 22, 32 x 8192 x 2048 24 / 22, 64 x 1024 x 7168 22 / 59, 128 x 1024 x 1024 8.5 / 11, 200 x 512 x 2048 14 / 16; e4m3 64 x 2048 x
+  // 4096 16 / 19, 128 x 2048 x 4096 24 / 19; 512 x 8 experts x 512 x 2048 31 / 21.
+  const double passes = a.experts > 1 ? a.rows / 16.0 + 0.5 * a.experts : (double)((a.rows + 15) / 16);
+  if (plan.kind == kTile && passes * a.n <= 8192.0) plan.kind = kStream;
   return launch(plan, kRows, a.x_dtype, stream);
 }
 

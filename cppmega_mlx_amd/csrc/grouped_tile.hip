@@ -36,8 +36,9 @@ namespace {
 
 __device__ __align__(64) const unsigned char zeros[64] = {};
 
-// HIGH: 256 x 256 tiles, eight wavefronts of 128 x 64, one workgroup to a CU.  Otherwise 128 x 128, four of 64 x 64, two to a CU.
-template <int OP, int DT, bool HIGH>
+// HIGH: 256 x 256 tiles, eight wavefronts of 128 x 64, one workgroup to a CU.  Otherwise 128 x 128, four of 64 x 64, two to a CU, or one
+// with twice the stages (DEEP).
+template <int OP, int DT, bool HIGH, bool DEEP = false>
 struct Shape {
   static constexpr bool FP8 = DT == CPPMEGA_MI355_E4M3, F16 = DT == CPPMEGA_MI355_F16;
   static constexpr bool TR = OP == kWeightsGrad, TQ = OP != kRows;      // the contraction is the operand's slow axis
@@ -47,7 +48,7 @@ struct Shape {
   // rate of whole lines (5 % of a large product); of the slow axis a stage has whole rows of the tile either way, and more of them on
   // their way are worth 7 %.
   static constexpr int KB = FP8 || !TQ ? 128 : 64;
-  static constexpr int RS = KB == 64 ? (HIGH ? 5 : 4) : FP8 || !HIGH ? 2 : 3, QS = KB == 64 ? RS : 2;
+  static constexpr int RS = DEEP ? 4 : KB == 64 ? (HIGH ? 5 : 4) : FP8 || !HIGH ? 2 : 3, QS = DEEP ? 4 : KB == 64 ? RS : 2;
   static constexpr int BYTES = FP8 ? 1 : 2, STEP = KB / BYTES;
   static constexpr int RL = BM * KB / 1024 / kWaves, QL = BN * KB / 1024 / kWaves, L = RL + QL + (FP8 ? 1 : 0);   // load instructions per wavefront and stage
   static constexpr int kR = BM * KB, kQ = BN * KB, kS = FP8 ? kWaves * 256 : 0;
@@ -61,9 +62,9 @@ using Count = std::integral_constant<int, N>;
 
 // Tile `block` of a product (of the launch's order, or none: every XCD's blocks are counted up to the same number), in S::kLds bytes of LDS.
 // `cut`: the last round's tiles in parts.
-template <int OP, int DT, bool HIGH, bool GATED>
+template <int OP, int DT, bool HIGH, bool GATED, bool DEEP = false>
 __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block, u32x4* const smem, const bool cut) {
-  typedef Shape<OP, DT, HIGH> S;                                 // (inlined throughout: a call would put the sums into memory)
+  typedef Shape<OP, DT, HIGH, DEEP> S;                           // (inlined throughout: a call would put the sums into memory)
   constexpr bool FP8 = S::FP8, F16 = S::F16, TR = S::TR, TQ = S::TQ;
   constexpr int BYTES = S::BYTES, STEP = S::STEP, BM = S::BM, BN = S::BN, RS = S::RS, QS = S::QS, RL = S::RL, QL = S::QL, L = S::L, KB = S::KB;
   // Columns of the result in a tile.  GATED: of every wavefront's columns the first half are rows of the gate, the others those of the up
@@ -97,7 +98,7 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
       const int total = fill_tiles<BM>(p, starts) * tiles_n, q = total >> 3, r = total & 7;
       // A last round that leaves half of the XCD's CUs idle or more is made of halves or quarters of its tiles (128 or 64 rows: 0.67 and
       // 0.5 of a tile's time).
-      constexpr int kSlots = HIGH ? 32 : 64, kParts = BM / 64;
+      constexpr int kSlots = HIGH || DEEP ? 32 : 64, kParts = BM / 64;
       const int mine = q + (xcd < r ? 1 : 0), last = mine % kSlots, from = mine - last;
       const int parts = !cut ? 1 : last * 4 <= kSlots && kParts >= 4 ? 4 : last * 2 <= kSlots ? 2 : 1;
       if (at >= from + last * parts) return;
@@ -563,10 +564,10 @@ __device__ __forceinline__ void tile_of(const GroupedParams& p, const int block,
   }
 }
 
-template <int OP, int DT, bool HIGH, bool GATED>
+template <int OP, int DT, bool HIGH, bool GATED, bool DEEP = false>
 __global__ __launch_bounds__(HIGH ? 512 : 256, 2) void grouped_tile_kernel(const GroupedParams p) {
-  __shared__ u32x4 smem[Shape<OP, DT, HIGH>::kLds / 16];
-  tile_of<OP, DT, HIGH, GATED>(p, (int)blockIdx.x, smem, true);
+  __shared__ u32x4 smem[Shape<OP, DT, HIGH, DEEP>::kLds / 16];
+  tile_of<OP, DT, HIGH, GATED, DEEP>(p, (int)blockIdx.x, smem, true);
 }
 
 // Both gradients: the weights' tiles fill the CUs that the rows' last round leaves idle.
@@ -592,6 +593,20 @@ int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bo
   const long long blocks = blocks_of(p, op, high, true, gated);
   if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
+  // The gated block in no more low tiles than there are CUs: no second workgroup covers a CU's waits, so its rings are twice as deep (and a
+  // tile's parts are counted for one workgroup to a CU).  Measured, us deep / not, rows x n x k: bf16 512 x 4096 x 4096 46 / 66, 256 x 4096 x 4096 36 / 60,
+  // 640 x 2048 x 512 9.9 / 11.1, 777 x 500 x 1544 17 / 22, 512 x 2 experts x 2048 x 4096 42 / 63; e4m3 1024 x 1024 x 4096 20 / 28.  The rings take longer to
+  // fill, so not for a few stages: bf16 1000 x 1000 x 384 8.9 / 8.9, e4m3 1000 x 1024 x 512 8.5 / 8.1.
+  const double tiles = (p.experts > 1 ? p.rows / 128.0 + 0.5 * p.experts : (double)((p.rows + 127) / 128)) * ((p.n + 63) / 64);
+  if (gated && !high && tiles <= 256.0 && (long long)p.k * (dtype == CPPMEGA_MI355_E4M3 ? 1 : 2) >= 768) {
+#define CM_DEEP(dt) hipLaunchKernelGGL((grouped_tile_kernel<kRows, dt, false, true, true>), grid, block, 0, stream, p)
+    if (dtype == CPPMEGA_MI355_E4M3) CM_DEEP(CPPMEGA_MI355_E4M3);
+    else if (dtype == CPPMEGA_MI355_F16) CM_DEEP(CPPMEGA_MI355_F16);
+    else CM_DEEP(CPPMEGA_MI355_BF16);
+#undef CM_DEEP
+    CM_HIP_CHECK(hipGetLastError());
+    return 0;
+  }
 #define CM_TILE(op_, dt, gated_)                                                                              \
   do {                                                                                                        \
     if (high) hipLaunchKernelGGL((grouped_tile_kernel<op_, dt, true, gated_>), grid, block, 0, stream, p);    \

@@ -125,6 +125,10 @@ def _rows(counts):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("name", ACTIVATIONS)
 def test_block_and_gradients(device, case, dtype, name):
+    _check_block(device, case, dtype, name)
+
+
+def _check_block(device, case, dtype, name):
     counts, n, k = case
     rows = _rows(counts)
     offsets = None if counts is None else _offsets(counts, device)
@@ -160,13 +164,34 @@ def test_block_and_gradients(device, case, dtype, name):
     assert torch.equal(gated_gemm_bwd(dy, kept, x, w, offsets, activation=name, need_dx=False)[1], dw)
 
 
+# outputs in more than one block of the gradients' kernel, one expert's weights in several passes, few tiles with a long contraction
+MORE_CASES = [([5, 0, 30], 2100, 64), ([3], 4099, 24), ([200], 512, 2048), ([700, 0, 300], 520, 1544), ([129], 1000, 776), ([1, 640], 1111, 512)]
+
+
+@pytest.mark.parametrize("case", MORE_CASES, ids=lambda c: f"{_rows(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_wide_blocks_and_few_tiles(device, case, dtype):
+    _check_block(device, case, dtype, "silu" if dtype == BF16 else "gelu_tanh")
+
+
 FP8_CASES = [([1], 5, 16), ([1] * 8, 256, 128), ([3, 0, 2], 100, 384), ([17, 128, 1, 129], 200, 272), ([300, 3, 0, 511], 192, 640), (None, 130, 200), (None, 257, 129),
              ([40] * 3 + [0] * 90 + [33] * 5, 68, 144), ([600, 1, 257], 384, 1024), ([700, 260], 129, 2048), ([2600, 0, 900, 37], 1300, 256)]
+MORE_FP8_CASES = [([1000], 1000, 1040), ([100], 1100, 784), ([60], 500, 2048), ([333, 0, 64], 300, 1552)]
 
 
 @pytest.mark.parametrize("case", FP8_CASES, ids=lambda c: f"{_rows(c[0])}x{len(c[0]) if c[0] else 0}x{c[1]}x{c[2]}")
 @pytest.mark.parametrize("block", [0, 128])
 def test_fp8_block(device, case, block):
+    _check_fp8_block(device, case, block)
+
+
+@pytest.mark.parametrize("case", MORE_FP8_CASES, ids=lambda c: f"{_rows(c[0])}x{len(c[0])}x{c[1]}x{c[2]}")
+@pytest.mark.parametrize("block", [0, 128])
+def test_fp8_few_tiles(device, case, block):
+    _check_fp8_block(device, case, block)
+
+
+def _check_fp8_block(device, case, block):
     counts, n, k = case
     rows = _rows(counts)
     offsets = None if counts is None else _offsets(counts, device)
