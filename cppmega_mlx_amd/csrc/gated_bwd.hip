@@ -2,8 +2,8 @@
 // dx and dw as one grouped product's two gradients over the 2 n rows of the weight.
 //
 // dg and du are rounded to the rows' type, as any gradient between two 16-bit products is: the matrix cores take nothing wider.
-// Their kernel is bound by memory: of a row and output dy, g and u read and dg, du written once; of 8192 rows x 2048 outputs, 168 MB in 35 us.
-// A thread has a run of one row, found by shifts: a division by the runs of a row cost more than the arithmetic.
+// Their kernel is bound by memory: of a row and output dy, g and u read and dg, du written once; of 8192 rows x 2048 outputs, 168 MB in 35 us (float32 g, u:
+// 235 MB).
 
 #include <string.h>
 

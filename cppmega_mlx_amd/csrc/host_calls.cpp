@@ -864,9 +864,9 @@ PyObject* gated_gemm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   a.activation = (int32_t)as_int(arg[3]);
   a.x_dtype = a.y_dtype = code(x->scalar_type());
   if (pre) {
-    if (!at.dense(*pre) || pre->scalar_type() != x->scalar_type() || !has_shape(*pre, {a.rows, 2ll * a.n})) DECLINE;
+    if (!at.dense(*pre) || (pre->scalar_type() != x->scalar_type() && pre->scalar_type() != ScalarType::Float) || !has_shape(*pre, {a.rows, 2ll * a.n})) DECLINE;
     a.pre = pre->data_ptr();
-    a.pre_dtype = a.x_dtype;
+    a.pre_dtype = code(pre->scalar_type());
     a.pre_pitch = 2ll * a.n;
   }
   Tensor y = at::empty({a.rows, a.n}, x->options());
@@ -885,12 +885,13 @@ PyObject* gated_gemm_bwd(PyObject*, PyObject* const* arg, Py_ssize_t n) {
   cppmega_mi355_gated_gemm_bwd_args_t a;
   if (!dy || !pre || !x || !w || !at.take(*x) || !is_half(*x)) DECLINE;
   for (const Tensor* t : {dy, pre, w})
-    if (t->scalar_type() != x->scalar_type() || !at.dense(*t)) DECLINE;
+    if ((t->scalar_type() != x->scalar_type() && (t != pre || t->scalar_type() != ScalarType::Float)) || !at.dense(*t)) DECLINE;
   if (!ffn_operands(at, *x, *w, arg[4], a) || w->size(-1) != a.k || w->size(-2) % 2) DECLINE;
   a.n = (int32_t)(w->size(-2) / 2);
   if (!has_shape(*dy, {a.rows, a.n}) || !has_shape(*pre, {a.rows, 2ll * a.n})) DECLINE;
   a.activation = (int32_t)as_int(arg[5]);
-  a.dtype = a.pre_dtype = a.dx_dtype = a.dw_dtype = code(x->scalar_type());
+  a.dtype = a.dx_dtype = a.dw_dtype = code(x->scalar_type());
+  a.pre_dtype = code(pre->scalar_type());
   a.dy = dy->data_ptr(); a.pre = pre->data_ptr();
   a.dy_pitch = a.n; a.pre_pitch = 2ll * a.n; a.dx_pitch = a.k;
   size_t bytes = 0;

@@ -94,8 +94,8 @@ def fp8_gated_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_sc
 
 class _GatedGemmFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets, activation):
-        pre = torch.empty((x.shape[0], w.shape[-2]), dtype=x.dtype, device=x.device)
+    def forward(ctx, x, w, offsets, activation, pre_dtype):
+        pre = torch.empty((x.shape[0], w.shape[-2]), dtype=pre_dtype, device=x.device)
         y = gated_gemm(x, w, offsets, activation=activation, pre=pre)
         ctx.save_for_backward(x, w, offsets, pre)
         ctx.activation = activation
@@ -107,9 +107,13 @@ class _GatedGemmFunction(torch.autograd.Function):
         x, w, offsets, pre = ctx.saved_tensors
         dy = dy if dy.is_contiguous() else dy.contiguous()
         dx, dw = gated_gemm_bwd(dy, pre, x, w, offsets, activation=ctx.activation, need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
-        return dx, dw, None, None
+        return dx, dw, None, None, None
 
 
-def gated_gemm_apply(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None = None, *, activation: str = "silu") -> torch.Tensor:
-    """Differentiable ``gated_gemm``."""
-    return _GatedGemmFunction.apply(x, w, offsets, activation)
+def gated_gemm_apply(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None = None, *, activation: str = "silu",
+                     pre_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Differentiable ``gated_gemm``.
+
+    ``pre_dtype``: what the two products are kept in for the backward pass, float32 (unrounded) or x's type (half the memory; the
+    gradients' error grows by a fifth, as one more rounding of theirs)."""
+    return _GatedGemmFunction.apply(x, w, offsets, activation, pre_dtype)

@@ -309,22 +309,27 @@ def test_gradients_are_those_of_differences(device):
         assert abs(slope - float(grad[at])) <= 8 * 2 * n * 2.0 ** -11 * 0.25 + 1e-6
 
 
+def _check_autograd(device, y, x, w, offsets, act, kept):
+    assert torch.equal(y, gated_gemm(x.detach(), w.detach(), offsets, activation=act)) and (y[42:] == 0).all()
+    g = _normal(device, *y.shape, dtype=BF16, seed=3)
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    pre = torch.empty(y.shape[0], 2 * y.shape[1], dtype=kept, device=device)
+    gated_gemm(x.detach(), w.detach(), offsets, activation=act, pre=pre)
+    want = gated_gemm_bwd(g, pre, x.detach(), w.detach(), offsets, activation=act)
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+
+
 def test_autograd(device):
     rows, n, k = 50, 40, 48
     offsets = _offsets([20, 0, 22], device)
     x, w = _normal(device, rows, k, dtype=BF16, seed=1).requires_grad_(), (_normal(device, 3, 2 * n, k, seed=2) * 0.2).to(BF16).requires_grad_()
     for act in ACTIVATIONS:
-        y = gated_gemm_apply(x, w, offsets, activation=act)
-        assert torch.equal(y, gated_gemm(x.detach(), w.detach(), offsets, activation=act)) and (y[42:] == 0).all()
-        g = _normal(device, rows, n, dtype=BF16, seed=3)
-        dx, dw = torch.autograd.grad(y, (x, w), g)
-        pre = torch.empty(rows, 2 * n, dtype=BF16, device=device)
-        gated_gemm(x.detach(), w.detach(), offsets, activation=act, pre=pre)
-        want = gated_gemm_bwd(g, pre, x.detach(), w.detach(), offsets, activation=act)
-        assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+        for kept in (F32, BF16):
+            y = gated_gemm_apply(x, w, offsets, activation=act, pre_dtype=kept)
+            _check_autograd(device, y, x, w, offsets, act, kept)
     d = w.detach()[0].contiguous()
     gated_gemm_apply(x, d).sum().backward()                        # (a broadcast cotangent, one matrix, no gradient of the weight)
-    pre = torch.empty(rows, 2 * n, dtype=BF16, device=device)
+    pre = torch.empty(rows, 2 * n, device=device)
     gated_gemm(x.detach(), d, pre=pre)
     assert torch.equal(x.grad, gated_gemm_bwd(torch.ones(rows, n, dtype=BF16, device=device), pre, x.detach(), d, need_dw=False)[0])
     (g,) = torch.autograd.grad(gated_gemm_apply(x, d).float().square().sum(), x, create_graph=True)
@@ -422,11 +427,16 @@ def test_the_native_path_and_the_helpers_agree(device, monkeypatch):
     def call():
         pre = torch.empty(60, 192, dtype=F16, device=device)
         y = gated_gemm(x, w, off, activation="gelu_tanh", pre=pre)
-        return (y, pre, *gated_gemm_bwd(dy, pre, x, w, off, activation="gelu_tanh"), fp8_gated_gemm(x8, xs, w8, ws, off), fp8_gated_gemm(x8, xs[:, 0].contiguous(), w8[0], ws[0]))
+        wide = torch.empty(60, 192, device=device)
+        kept = (gated_gemm(x, w, off, activation="gelu_tanh", pre=wide), wide, *gated_gemm_bwd(dy, wide, x, w, off, activation="gelu_tanh"))
+        return (y, pre, *gated_gemm_bwd(dy, pre, x, w, off, activation="gelu_tanh"), fp8_gated_gemm(x8, xs, w8, ws, off), fp8_gated_gemm(x8, xs[:, 0].contiguous(), w8[0], ws[0]), *kept)
 
     native = call()
     host = ops.host
     assert host.gated_gemm(x[:, ::2], w, off, 0, None) is None and host.gated_gemm(x, w.bfloat16(), off, 0, None) is None and host.gated_gemm(x, w, None, 0, None) is None
+    wide = native[7]
+    assert wide.dtype == F32 and host.gated_gemm(x, w, off, 0, wide) is not None and host.gated_gemm_bwd(dy, wide, x, w, off, 0) is not None
+    assert host.gated_gemm(x, w, off, 0, wide.double()) is None and host.gated_gemm_bwd(dy.float(), wide, x, w, off, 0) is None
     assert host.gated_gemm(x, w, off, 5, None) is None and host.gated_gemm_bwd(dy[:9], native[1], x, w, off, 0) is None and host.fp8_gated_gemm(x8, xs, w8, ws[:1], off, 0) is None
     monkeypatch.setattr(ops, "host", type("Declines", (), {"__getattr__": lambda self, name: lambda *a: None})())
     for a, b in zip(native, call()):
