@@ -187,7 +187,7 @@ def _framework(s):
         return gated_gemm(s["x"], s["w"], s["offsets"], activation=case["activation"])
     if kind == "gated_fp8":
         return fp8_gated_gemm(s["x"], s["x_scale"], s["w"], s["w_scale"], s["offsets"], activation=case["activation"])
-    pre = torch.empty((case["rows"], 2 * case["n"]), dtype=s["x"].dtype, device=s["x"].device)
+    pre = torch.empty((case["rows"], 2 * case["n"]), dtype=torch.float32, device=s["x"].device)
     y = gated_gemm(s["x"], s["w"], s["offsets"], activation=case["activation"], pre=pre)
     return (y,) + tuple(gated_gemm_bwd(s["dy"], pre, s["x"], s["w"], s["offsets"], activation=case["activation"]))
 
