@@ -2,76 +2,25 @@
 //
 //   y[t, n] = sum_k x[t, k] (s[n, g] q[n, k] + b[n, g]),  g = k / G;  without biases b = -8 s
 //
-// Bound by memory and by the vector instructions that widen the codes: the weights pass once.  A workgroup has 16 rows of x of one expert and one or
-// more runs of 16 TN rows of its weight (gated: 16 of the gate's and 16 of the up projection's), a run to a wavefront; the others divide the
-// contraction, and their sums meet in LDS once at the end, added in order.  A wavefront has 8 KiB of weights on their way and nothing else: loads
-// return in the order in which they were asked for, and rows of x, from the cache but behind weights, waited for memory.  x passes through LDS
-// instead, as much of it at a time as there is room, in the codes' order.
+// Widened once for 16 rows of x.  A workgroup has 16 rows of x of one expert and up to four tiles of 16 rows of its weight (gated: as many of the
+// gate's as of the up projection's), a tile to a wavefront; the others divide the contraction, and their sums meet in LDS once at the
+// end, added in order.  A wavefront has 8 KiB of weights on their way and nothing else: loads return in the order in which they were asked for, and
+// rows of x, from the cache but behind weights, waited for memory.  x passes through LDS instead, as much of it at a time as there is room,
+// in the codes' order.
 //
-// Four bits become 16 + q in 16 bits by a shift and an and-or, two at a time: q lies where float16 and bfloat16 between 16 and 32 have their
-// next four bits.  Products are exact; 16 times a group's sum of x comes off again in float32 with the bias,
-//   y = sum over groups of s (sum x (16 + q)) + (b - 16 s) (sum x),
-// the second part a product of its own with float32 operands, four steps to a matrix instruction.
-// x is the first operand: a lane has one row of the weight in every sum, and with it one scale and one bias.
-// A step is 128 channels, 16 bytes (32 codes) a lane; a word of it is eight channels, of which the low and the high half of a register
-// take those four apart, so the pieces of x are put in that order.  With groups below 128 the four words of the four lanes of a row change
-// places, so that one instruction has 32 channels in a run.
+// Many experts are bound by memory: 61 experts of 4096 x 7168 codes, groups of 64, in 241 us, 4.2 TB/s.  One matrix is bound by the vector
+// instructions that widen its codes, by the start (arguments, x into LDS, the first weights: 4 to 5 us) and by the sums' way at the end: 16 x 16384 x
+// 7168 in 21 us, 2.9 TB/s; 1 x 2048 x 7168 in 9.  Tried at 1 x 16384 x 7168 with nothing gained (18 to 21 us): two or four tiles to a wavefront, x kept
+// in registers, 16 steps of weights on their way, 16 wavefronts, x read past LDS (as much of the first-level cache's time as the weights).
 
 #include <string.h>
 
-#include <type_traits>
-#include <utility>
-
-#include "grouped_gemm.h"
+#include "w4.h"
 
 namespace cm {
 namespace {
 
 constexpr int kMostWaves = 8, kRoom = 8192;                      // wavefronts of a workgroup; bytes of LDS that each of them brings for x
-
-struct W4Params {
-  GroupedParams g;                                               // (w, scales: of 2 n rows when gated)
-  const void *scale, *bias;
-  int gated, log_split;                                          // wavefronts that divide the contraction
-  int tile0;                                                     // the launch's first 16 rows
-};
-
-// Eight codes as 16 + q in 16 bits, in the order 0 4 1 5 2 6 3 7.
-template <bool F16>
-__device__ __forceinline__ bf16x8 widen(unsigned w, unsigned one) {        // (one: 16 twice, from a vector register, so that and-or is one instruction)
-  constexpr unsigned mask = F16 ? 0x03c003c0u : 0x00780078u;
-  u32x4 r;
-  if (F16) r = u32x4{w << 6, w << 2, w >> 2, w >> 6};
-  else r = u32x4{w << 3, w >> 1, w >> 5, w >> 9};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = (r[i] & mask) | one;
-  return __builtin_bit_cast(bf16x8, r);
-}
-// Eight values of x in the same order.
-__device__ __forceinline__ bf16x8 reorder(const u32x4 x) {
-  return __builtin_bit_cast(bf16x8, u32x4{__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
-                                          __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)});
-}
-// Words of four quads of lanes: word i of quad j becomes word j of quad i.
-__device__ __forceinline__ void transpose4(u32x4& w) {
-  u32x2 a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-  const u32x2 c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-  w = u32x4{c[0], c[1], d[0], d[1]};
-}
-
-// A value of quad Q's lanes in the lanes of all quads (of the same place).
-template <int Q>
-__device__ __forceinline__ unsigned of_quad(unsigned v) {
-  const u32x2 a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-  return __builtin_amdgcn_permlane16_swap(a[Q >> 1], a[Q >> 1], false, false)[Q & 1];
-}
-
-template <int N>
-using Count = std::integral_constant<int, N>;
-template <int... I, class F>
-__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) { (f(Count<I>()), ...); }
-template <int N, class F>
-__device__ __forceinline__ void each(F f) { each(std::make_integer_sequence<int, N>(), f); }
 
 // The scales (or biases) of N consecutive groups as they are stored, S bytes each.
 template <int N, int S>
@@ -330,6 +279,10 @@ int launch(W4Params p, hipStream_t stream) {
   const long long tiles_m = !q.offsets ? (q.rows + 15) / 16 : q.rows / 16 + tails < q.rows ? q.rows / 16 + tails : q.rows;
   const long long work = tiles_m * ((q.n + 15) / 16) * (p.gated ? 2 : 1);         // tiles of rows of x and of the weight
   const int steps = q.k / 128;
+  // Tiles of a workgroup share x's way through LDS; few of them, so that all CUs have some.  Four wavefronts where there is plenty of work or
+  // little to divide.  Measured, us 1 / 2 / 4 tiles with 4 wavefronts, then with 8, rows x n x k, bfloat16: 1 x 2048 x 7168 10 / 15 / 25, 9.5 / 12 / 19; 4 x 16384 x 7168
+  // 24 / 22 / 26, 29 / 22 / 22; 8 x 2048 x 2048 7.8 / 8.4 / 11, 9.2 / 9.3 / 9.7; 16 x 8192 x 2048 13 / 11 / 12, 14 / 10 / 11; 16 x 16384 x 7168 50 / 31 / 31, 61 / 34 / 25;
+  // 64 x 8192 x 8192 105 / 58 / 41, 117 / 63 / 36; 1024 x 1024 x 512 41 / 23 / 14, 62 / 45 / 24; 256 x 61 experts gated, 2 and 4 tiles: 270 / 243, 312 / 263.
   const bool thin = q.rows <= 4 && q.experts == 1;
   const int tiles = work >= 1024 && !thin ? 4 : work >= 512 || p.gated ? 2 : 1;
   const int waves = work >= 4096 || steps * tiles < 32 ? 4 : 8;
@@ -385,6 +338,12 @@ int w4_gemm_launch(const cppmega_mi355_w4_gemm_args_t& a, hipStream_t stream) {
   q.y_dtype = a.y_dtype; q.offsets64 = a.offsets_dtype == CPPMEGA_MI355_I64; q.zero_tail = a.zero_tail; q.activation = a.activation;
   p.scale = a.scale; p.bias = a.bias; p.gated = is_gated;
   const bool f16 = a.x_dtype == CPPMEGA_MI355_F16, wide = a.scale_dtype == CPPMEGA_MI355_F32;
+  // Weights widened once for 64 rows, or once for 16 with eight times the wavefronts: the former from 32 rows to an expert on, where there is as much
+  // work as makes up for its start, in tiles of 16 x 16 results.  Measured, us 64 / 16 rows, rows x n x k, bfloat16: 64 x 8192 x 8192 43 / 42, 64 x 16384 x
+  // 4096 24 / 37, 64 x 4096 x 4096 42 / 18, 128 x 4096 x 4096 22 / 21, 256 x 4096 x 4096 23 / 35, 32 x 32768 x 2048 21 / 23, 512 x 8192 x 8192 109 / 215, 1024 x 1024 x 512
+  // 18 / 14; gated 512 x 16 experts x 1024 x 2048 25 / 33, 256 x 16 experts x 1024 x 7168 62 / 60.
+  const double tiles = ((a.rows + 15) / 16 + (a.experts > 1 ? a.experts / 2 : 0)) * (((double)a.n * (is_gated ? 2 : 1) + 15) / 16);
+  if (a.rows >= 32ll * a.experts && a.k >= 1024 && tiles >= 2560.0) return w4_tile_launch(p, a.group, f16, wide, stream);
   return a.group == 32 ? launch_group<32>(p, f16, wide, stream) : a.group == 64 ? launch_group<64>(p, f16, wide, stream) : launch_group<128>(p, f16, wide, stream);
 }
 

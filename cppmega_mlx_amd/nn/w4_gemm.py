@@ -10,7 +10,8 @@ These are the bytes that an affine 4-bit quantiser packs into little-endian 32-b
 float16 or bfloat16, rows of any pitch; products are exact, sums float32, rounded once.  The codes enter as 16 + q, and 16 times a
 group's sum of x comes off again: rows with infinities give NaN, and 32 times a group's sum of magnitudes must be finite in float32.
 
-Made for the rows of a decode step: up to 64 rows of an expert pass its weights once.  By expert: a leading axis ``[E, ..]`` and ``offsets [E + 1]`` as
+Made for the rows of a decode step: the codes are widened once for every 16 rows of an expert (64 where there are many), so long prompts
+cost as many passes.  By expert: a leading axis ``[E, ..]`` and ``offsets [E + 1]`` as
 in ``grouped_gemm``.  Rows behind the last expert's: zeros in an output made here, left as they were in a caller-owned one, which must not overlap
 the operands.  Fewer than 2^29 rows, up to 2^24 elements apart, N up to 2^30, K up to 2^24, up to 512 experts.
 

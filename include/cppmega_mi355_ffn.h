@@ -88,7 +88,8 @@ int cppmega_mi355_gated_gemm_bwd(const cppmega_mi355_gated_gemm_bwd_args_t* args
  *   y[t, j] = sum_k x[t, k] (scale[j, k / group] q[j, k] + bias[j, k / group]);  without biases scale (q - 8)
  * q is 0 .. 15, two to a byte, the even channel in the low four bits.  Products with 16 + q are exact, sums float32: what is
  * added and taken away again is 16 times the rows' sums, so rows with infinities give NaN.  `activation` NONE: the product;
- * otherwise the gated block over weights [experts, 2 n, ..] as above.  Made for few rows (16 to 64 an expert pass its weights once). */
+ * otherwise the gated block over weights [experts, 2 n, ..] as above.  Made for few rows: the codes are widened once for
+ * every 16 rows of an expert, or for 64 where there are many. */
 #define CPPMEGA_MI355_W4_MAX_CHANNELS 16777216   /* of k, and of x_pitch */
 typedef struct cppmega_mi355_w4_gemm_args {
   uint32_t struct_size;

@@ -55,6 +55,20 @@ CASES = [(1, 1, 1), (1, 16, 4), (2, 17, 8), (16, 40, 36), (5, 1001, 33), (17, 10
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("bias", [True, False])
 def test_products(device, case, group, dtype, bias):
+    _check_products(device, case, group, dtype, bias)
+
+
+# many rows: 64 at a time, the contraction in 4 and 2 parts, passes and groups that end inside, experts of fewer rows and of none
+MANY = [(64, 10300, 33), (51, 10250, 36), (130, 4600, 35), (300, 2200, 68), (500, 4100, 32), ([200, 0, 33, 300, 1], 1500, 37), ([64, 65, 0, 190], 1901, 100)]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0] if isinstance(c[0], int) else f'{sum(c[0])}of{len(c[0])}'}x{c[1]}x{c[2] * 32}")
+@pytest.mark.parametrize("group, dtype, bias", [(32, BF16, True), (64, F16, False), (64, BF16, True), (128, BF16, False), (128, F16, True)])
+def test_products_of_many_rows(device, case, group, dtype, bias):
+    _check_products(device, case, group, dtype, bias)
+
+
+def _check_products(device, case, group, dtype, bias):
     rows, n, k = case[0], case[1], case[2] * 32
     k = (k + group - 1) // group * group
     offsets = None if isinstance(rows, int) else _offsets(rows, device)
@@ -93,7 +107,7 @@ def test_every_code_in_every_place(device):
         assert torch.equal(w4_gemm(x, w, scale, out=got).double(), (s * (q - 8)).T)
 
 
-@pytest.mark.parametrize("shape", [(7, 40, 320), (37, 33, 96)], ids=str)
+@pytest.mark.parametrize("shape", [(7, 40, 320), (37, 33, 96), (380, 1700, 1056)], ids=str)
 def test_views_and_tails(device, shape):
     rows, n, k = shape
     tail, counts = 9, [rows // 3, 0, rows - rows // 3]
@@ -124,8 +138,8 @@ def test_views_and_tails(device, shape):
 
 
 @pytest.mark.parametrize("values", [[0, 9, 4, 60], [0, 3, 2 ** 30, 5], [5, -7, 40, 40], [40, 40, 40, 40], [0, 0, 0, -1]], ids=str)
-def test_offsets_that_break_the_rules_stay_inside(device, values):
-    rows, n, k = 40, 48, 64
+@pytest.mark.parametrize("rows, n, k", [(40, 48, 64), (200, 1500, 1024)])
+def test_offsets_that_break_the_rules_stay_inside(device, values, rows, n, k):
     w, scale, bias = _weights(device, (3,), 2 * n, k, 32, True, BF16, seed=1)
     x = _normal(device, rows, k, dtype=BF16, seed=2)
     off = torch.tensor(values, dtype=torch.int64, device=device)
@@ -146,9 +160,10 @@ def test_large_magnitudes_and_nan(device):
     assert torch.isfinite(y[0]).all() and y[1:].isnan().all()
 
 
-def test_graphs_streams_and_repeats(device):
-    w, scale, bias = _weights(device, (4,), 128, 256, 64, True, BF16, seed=1)
-    x, off = _normal(device, 24, 256, dtype=BF16, seed=2), _offsets([10, 0, 2, 12], device)
+@pytest.mark.parametrize("per, n, k", [(1, 128, 256), (9, 2700, 1088)])
+def test_graphs_streams_and_repeats(device, per, n, k):
+    w, scale, bias = _weights(device, (4,), n, k, 64, True, BF16, seed=1)
+    x, off = _normal(device, 24 * per, k, dtype=BF16, seed=2), _offsets([10 * per, 0, 2 * per, 12 * per], device)
 
     def call():
         return w4_gemm(x, w, scale, bias, off), w4_gated_gemm(x, w, scale, None, off), w4_gemm(x, w[0], scale[0])
@@ -159,13 +174,13 @@ def test_graphs_streams_and_repeats(device):
     with torch.cuda.graph(graph):
         out = call()
     for i, counts in enumerate([[10, 0, 2, 12], [24, 0, 0, 0], [1, 1, 1, 1], [0, 0, 0, 0]]):
-        off.copy_(_offsets(counts, device))
-        x.copy_(_normal(device, 24, 256, dtype=BF16, seed=5 + i))
+        off.copy_(_offsets([c * per for c in counts], device))
+        x.copy_(_normal(device, 24 * per, k, dtype=BF16, seed=5 + i))
         graph.replay()
         torch.cuda.synchronize()
         want = call()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
-    off.copy_(_offsets([10, 0, 2, 12], device))
+    off.copy_(_offsets([10 * per, 0, 2 * per, 12 * per], device))
     want = call()
     streams = [torch.cuda.Stream(device) for _ in range(3)]
     got = []
