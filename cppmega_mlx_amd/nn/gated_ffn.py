@@ -116,4 +116,6 @@ def gated_gemm_apply(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | N
 
     ``pre_dtype``: what the two products are kept in for the backward pass, float32 (unrounded) or x's type (half the memory; the
     gradients' error grows by a fifth, as one more rounding of theirs)."""
+    if not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
+        return gated_gemm(x, w, offsets, activation=activation)      # (nothing to keep)
     return _GatedGemmFunction.apply(x, w, offsets, activation, pre_dtype)

@@ -337,6 +337,19 @@ def test_autograd(device):
         g.sum().backward()
 
 
+def test_nothing_is_kept_without_gradients(device):
+    x, w = _normal(device, 70, 64, dtype=BF16, seed=1), (_normal(device, 96, 64, seed=2) * 0.2).to(BF16).requires_grad_()
+    want = gated_gemm(x, w.detach())
+    base = torch.cuda.memory_allocated(device)
+    with torch.no_grad():
+        y = gated_gemm_apply(x, w)
+    z = gated_gemm_apply(x, w.detach())
+    assert torch.equal(y, want) and torch.equal(z, want) and not y.requires_grad and not z.requires_grad
+    kept = torch.cuda.memory_allocated(device) - base
+    assert kept <= 2 * 70 * 48 * 2 + 2 * 512                       # (two results, in units of 512 bytes)
+    assert torch.equal(gated_gemm_apply(x, w), want) and gated_gemm_apply(x, w).requires_grad
+
+
 def test_one_matrix_is_one_expert(device):
     x, w, dy = _normal(device, 200, 64, dtype=BF16, seed=1), (_normal(device, 96, 64, seed=2) * 0.2).to(BF16), _normal(device, 200, 48, dtype=BF16, seed=3)
     offsets = _offsets([200], device)
