@@ -279,12 +279,14 @@ int launch(W4Params p, hipStream_t stream) {
   const long long tiles_m = !q.offsets ? (q.rows + 15) / 16 : q.rows / 16 + tails < q.rows ? q.rows / 16 + tails : q.rows;
   const long long work = tiles_m * ((q.n + 15) / 16) * (p.gated ? 2 : 1);         // tiles of rows of x and of the weight
   const int steps = q.k / 128;
-  // Tiles of a workgroup share x's way through LDS; few of them, so that all CUs have some.  Four wavefronts where there is plenty of work or
-  // little to divide.  Measured, us 1 / 2 / 4 tiles with 4 wavefronts, then with 8, rows x n x k, bfloat16: 1 x 2048 x 7168 10 / 15 / 25, 9.5 / 12 / 19; 4 x 16384 x 7168
-  // 24 / 22 / 26, 29 / 22 / 22; 8 x 2048 x 2048 7.8 / 8.4 / 11, 9.2 / 9.3 / 9.7; 16 x 8192 x 2048 13 / 11 / 12, 14 / 10 / 11; 16 x 16384 x 7168 50 / 31 / 31, 61 / 34 / 25;
-  // 64 x 8192 x 8192 105 / 58 / 41, 117 / 63 / 36; 1024 x 1024 x 512 41 / 23 / 14, 62 / 45 / 24; 256 x 61 experts gated, 2 and 4 tiles: 270 / 243, 312 / 263.
+  // Tiles of a workgroup share x's way through LDS: as few as leave a workgroup to a CU (with up to four rows of x, two).  Four wavefronts where
+  // there is plenty of work or little to divide.  Measured, us 1 / 2 / 4 tiles with 4 wavefronts, then with 8, rows x n x k, bfloat16: 1 x 2048 x
+  // 7168 10 / 15 / 25, 9.5 / 12 / 19; 4 x 16384 x 7168 24 / 22 / 26, 29 / 22 / 22; 48 x 2048 x 7168 27 / 26 / 31, 30 / 21 / 24; 48 x 4096 x 4096 26 /
+  // 20 / 20, 29 / 21 / 16; 8 x 2048 x 2048 7.8 / 8.4 / 11, 9.2 / 9.3 / 9.7; 16 x 8192 x 2048 13 / 11 / 12, 14 / 10 / 11; 16 x 16384 x 7168 50 / 31 /
+  // 31, 61 / 34 / 25; 64 x 8192 x 8192 105 / 58 / 41, 117 / 63 / 36; 1024 x 1024 x 512 41 / 23 / 14, 62 / 45 / 24; 256 x 61 experts gated, 2 and 4
+  // tiles: 270 / 243, 312 / 263.
   const bool thin = q.rows <= 4 && q.experts == 1;
-  const int tiles = work >= 1024 && !thin ? 4 : work >= 512 || p.gated ? 2 : 1;
+  const int tiles = work > 512 && !thin ? 4 : work > 256 || p.gated ? 2 : 1;
   const int waves = work >= 4096 || steps * tiles < 32 ? 4 : 8;
   p.log_split = __builtin_ctz(waves / tiles);
   const int out = 16 * (p.gated ? tiles / 2 : tiles), parts = (q.n + out - 1) / out;
