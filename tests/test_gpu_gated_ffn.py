@@ -533,3 +533,22 @@ def test_a_layer_runs_through(device):
     p, size = _products(wide, w8.view(torch.float8_e4m3fn).double() / 64, offsets)
     want, bound = _gated(p, size, k + 3 + DROPPED, "silu")
     _assert_within(y8, want, _rounded(want, bound, BF16))
+
+
+def test_products_beyond_32_bits(device):
+    """Kept products and gradients of more than 2^32 bytes: rows repeat, and their results with them."""
+    rows, n, k = 270336, 2048, 64
+    x, dy = _normal(device, 1024, k, dtype=BF16, seed=1), _normal(device, 1024, n, dtype=BF16, seed=2)
+    w = (_normal(device, 2 * n, k, seed=3) * 0.2).to(BF16)
+    pre = torch.empty(rows, 2 * n, device=device)
+    many = x.repeat(rows // 1024, 1)
+    y = gated_gemm(many, w, pre=pre)
+    p, size = _products(x, w, None)
+    want, bound = _gated(p, size, k, "silu")
+    _assert_within(y[:1024], want, _rounded(want, bound, BF16))
+    _assert_within(pre[:1024], p, _rounded(p, size * (k * U) * 1.01, F32))
+    dx, _ = gated_gemm_bwd(dy.repeat(rows // 1024, 1), pre, many, w, need_dw=False)
+    wx, ex, _, _ = _grads(dy, pre[:1024], x, w, None, "silu")
+    _assert_within(dx[:1024], wx, _rounded(wx, ex, BF16))
+    for t in (y, pre, dx):
+        assert all(torch.equal(t[at:at + 1024], t[:1024]) for at in range(1024, rows, 1024))

@@ -244,3 +244,24 @@ def test_a_decode_step_runs_through(device):
     _assert_within(mid, want, _rounded(want, bound, BF16))
     want, size = _products(mid, down, ds, None, off)
     _assert_within(out, want, _rounded(want, size * (f + 16) * U, BF16))
+
+
+@pytest.mark.parametrize("rows, n, k", [(65535 * 16 + 40, 17, 32), (65535 * 64 + 70, 33, 1024)])
+def test_more_tiles_of_rows_than_a_grid_is_high(device, rows, n, k):
+    w, scale, bias = _weights(device, (), n, k, 32, True, BF16, seed=1)
+    x = _normal(device, 1024, k, dtype=BF16, seed=2).repeat((rows + 1023) // 1024, 1)[:rows]
+    y = w4_gemm(x, w, scale, bias)
+    want, size = _products(x[:1024], w, scale, bias, None)
+    _assert_within(y[:1024], want, _rounded(want, size * (k + 16) * U, BF16))
+    last = (rows - 1024) // 1024 * 1024                            # (rows repeat, and their results with them)
+    assert torch.equal(y[:last].view(-1, 1024, n), y[:1024].expand(last // 1024, 1024, n)) and torch.equal(y[last:], y[:1024].repeat(2, 1)[:rows - last])
+
+
+@pytest.mark.parametrize("n", [64, 10300])
+def test_rows_far_apart(device, n):
+    rows, k, pitch = 64, 1024, 1 << 24
+    w, scale, bias = _weights(device, (), n, k, 64, True, F16, seed=1)
+    x = _normal(device, rows, k, dtype=F16, seed=2)
+    far = torch.empty(rows, pitch, dtype=F16, device=device)[:, pitch - k:]
+    far.copy_(x)
+    assert torch.equal(w4_gemm(far, w, scale, bias), w4_gemm(x, w, scale, bias))
