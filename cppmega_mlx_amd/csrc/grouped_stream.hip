@@ -5,7 +5,8 @@
 // contraction, and their sums meet in LDS once at the end, added in order.  A step is 128 bytes of every weight row (whole cache lines),
 // requested one step ahead; the activations' pieces come from the caches, a quarter of the traffic.  Which expert a workgroup has, every
 // wavefront finds by itself (a scan over the counts in registers: no table, no barrier in front of the first load).
-// Measured: 256 rows over 61 of 64 experts, e4m3, 4096 x 7168: 298 us = 6.0 TB/s; 8 rows of 8 experts, bf16, 4096 x 2048: 25 us = 5.3 TB/s.
+// Measured: 256 rows over 61 of 64 experts, e4m3, 4096 x 7168: 298 us = 6.0 TB/s; 8 rows of 8 experts, bf16, 4096 x 2048: 25 us = 5.3 TB/s;
+// the gated block of as many weight rows 300 and 26.
 // Non-temporal loads were 15 to 20 % slower, eight wavefronts 5 %, 32 or 64 rows to a workgroup 5 to 15 % at any number of rows.
 //
 // e4m3 codes become bfloat16 on the way, which is exact; a step is one 128-channel block, whose sum is scaled in float32.
