@@ -94,7 +94,9 @@ def fp8_gated_gemm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_sc
 
 class _GatedGemmFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets, activation, pre_dtype):
+    def forward(ctx, x, w, offsets, activation, pre_dtype, keep):
+        if not keep:
+            return gated_gemm(x, w, offsets, activation=activation)
         pre = torch.empty((x.shape[0], w.shape[-2]), dtype=pre_dtype, device=x.device)
         y = gated_gemm(x, w, offsets, activation=activation, pre=pre)
         ctx.save_for_backward(x, w, offsets, pre)
@@ -107,15 +109,14 @@ class _GatedGemmFunction(torch.autograd.Function):
         x, w, offsets, pre = ctx.saved_tensors
         dy = dy if dy.is_contiguous() else dy.contiguous()
         dx, dw = gated_gemm_bwd(dy, pre, x, w, offsets, activation=ctx.activation, need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
 def gated_gemm_apply(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None = None, *, activation: str = "silu",
                      pre_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """Differentiable ``gated_gemm``.
+    """Differentiable ``gated_gemm``: first derivatives, by the backward pass (a tangent of forward mode is refused).
 
     ``pre_dtype``: what the two products are kept in for the backward pass, float32 (unrounded) or x's type (half the memory; the
-    gradients' error grows by a fifth, as one more rounding of theirs)."""
-    if not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
-        return gated_gemm(x, w, offsets, activation=activation)      # (nothing to keep)
-    return _GatedGemmFunction.apply(x, w, offsets, activation, pre_dtype)
+    gradients' error grows by a fifth, as one more rounding of theirs).  They are not kept where no gradient is wanted."""
+    # (by the function in either case: it refuses the derivatives that it lacks, where the bare call would drop them)
+    return _GatedGemmFunction.apply(x, w, offsets, activation, pre_dtype, torch.is_grad_enabled() and (x.requires_grad or w.requires_grad))
