@@ -106,10 +106,34 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   return 0;
 }
 
+int check(const Plan& plan, int op) {
+  if (plan.kind == kTile) return grouped_tile_check(plan.p, op, plan.high, plan.gated);
+  if (plan.kind == kStream) return grouped_stream_check(plan.p, plan.gated);
+  return plan.kind == kGeneral ? grouped_general_check(plan.p, op, plan.gated) : 0;
+}
+
 int launch(const Plan& plan, int op, int dtype, hipStream_t stream) {
+  if (int rc = check(plan, op)) return rc;
   if (plan.kind == kTile) return grouped_tile_launch(plan.p, op, dtype, plan.high, plan.gated, stream);
   if (plan.kind == kStream) return grouped_stream_launch(plan.p, dtype, plan.gated, stream);
   return plan.kind == kGeneral ? grouped_general_launch(plan.p, op, dtype, plan.gated, stream) : 0;
+}
+
+// The gradients that are wanted, and whether one launch makes both; everything that may refuse either of them is asked here.
+int plan_grads(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights, Plan& r, Plan& w,
+               bool& together) {
+  if (rows.op != kRowsGrad || weights.op != kWeightsGrad)
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm_bwd: ops %d and %d are not the rows' and the weights' gradient", rows.op, weights.op);
+  int rc = need_rows ? plan_of(rows, r) : 0;
+  if (!rc && need_weights) rc = plan_of(weights, w);
+  if (rc) return rc;
+  together = need_rows && need_weights && r.kind == kTile && w.kind == kTile && rows.x_dtype == weights.x_dtype;
+  if (together) {
+    r.high = w.high = high_grads(r.p, w.p);
+    return grouped_tile_grads_check(r.p, w.p, r.high);
+  }
+  rc = need_rows ? check(r, kRowsGrad) : 0;
+  return !rc && need_weights ? check(w, kWeightsGrad) : rc;
 }
 
 }  // namespace
@@ -121,24 +145,19 @@ int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t 
 }
 
 int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream) {
-  if (rows.op != kRowsGrad || weights.op != kWeightsGrad)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm_bwd: ops %d and %d are not the rows' and the weights' gradient", rows.op, weights.op);
   Plan r, w;
-  int rc = plan_of(rows, r);
-  if (!rc) rc = plan_of(weights, w);
-  if (rc) return rc;
-  if (r.kind == kTile && w.kind == kTile && rows.x_dtype == weights.x_dtype)
-    return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, high_grads(r.p, w.p), stream);
-  rc = launch(r, kRowsGrad, rows.x_dtype, stream);
+  bool together;
+  if (int rc = plan_grads(rows, weights, true, true, r, w, together)) return rc;
+  if (together) return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, r.high, stream);
+  const int rc = launch(r, kRowsGrad, rows.x_dtype, stream);
   return rc ? rc : launch(w, kWeightsGrad, weights.x_dtype, stream);
 }
 
 // Whether the gradients that are wanted would be launched, with the reason if not.
 int grouped_gemm_check(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights) {
-  Plan plan;
-  int rc = need_rows ? plan_of(rows, plan) : 0;
-  if (!rc && need_weights) rc = plan_of(weights, plan);
-  return rc;
+  Plan r, w;
+  bool together;
+  return plan_grads(rows, weights, need_rows, need_weights, r, w, together);
 }
 
 // The gated block is a product of rows with 2 n rows of a weight, whose kernels pair them off; the same rules choose among them.

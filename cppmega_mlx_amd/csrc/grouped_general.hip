@@ -241,14 +241,18 @@ __global__ __launch_bounds__(256) void grouped_general_kernel(const GroupedParam
   }
 }
 
-}  // namespace
-
-int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream) {
+long long tiles_of(const GroupedParams& p, int op, bool gated) {
   const int across = gated ? BN / 2 : BN;
   const long long tiles_n = ((op == kRows ? p.n : p.k) + across - 1) / across;
-  const long long tiles_m = op == kWeightsGrad ? (long long)p.experts * ((p.n + BM - 1) / BM) : p.rows / BM + p.experts + 1;
-  if (int rc = check_tiles(tiles_m * tiles_n, 256)) return rc;
-  const dim3 grid((unsigned)(tiles_m * tiles_n)), block(256);
+  return tiles_n * (op == kWeightsGrad ? (long long)p.experts * ((p.n + BM - 1) / BM) : p.rows / BM + p.experts + 1);
+}
+
+}  // namespace
+
+int grouped_general_check(const GroupedParams& p, int op, bool gated) { return check_tiles(tiles_of(p, op, gated), 256); }
+
+int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream) {
+  const dim3 grid((unsigned)tiles_of(p, op, gated)), block(256);
 #define CM_GENERAL(op_, dt, gated_) hipLaunchKernelGGL((grouped_general_kernel<op_, dt, gated_>), grid, block, 0, stream, p)
 #define CM_GENERAL_OP(op_, gated_)                                              \
   do {                                                                          \

@@ -149,14 +149,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void grouped_stream_kernel(const Gr
   store(p.y, p.y_dtype, (size_t)(first + l16) * p.y_pitch + n, v);
 }
 
-template <int DT, bool GATED>
-int launch(const GroupedParams& p, hipStream_t stream) {
+// Workgroups of a call, and whether each has several tiles of outputs.
+long long tiles_of(const GroupedParams& p, bool gated, bool& wide) {
   const long long tails = p.experts + 1 < p.rows ? p.experts + 1 : p.rows;       // tiles of rows that are not full, at most
   const long long tiles_m = p.rows / 16 + tails < p.rows ? p.rows / 16 + tails : p.rows;
-  constexpr int kWide = GATED ? 32 : 64;                                         // outputs of a workgroup
-  const bool wide = tiles_m * ((p.n + kWide - 1) / kWide) >= 512;                // (two workgroups to a CU at least)
-  const long long tiles = tiles_m * (wide ? (p.n + kWide - 1) / kWide : (p.n + 15) / 16);
-  if (int rc = check_tiles(tiles, 64 * kWaves)) return rc;
+  const int most = gated ? 32 : 64;                                              // outputs of a workgroup
+  wide = tiles_m * ((p.n + most - 1) / most) >= 512;                             // (two workgroups to a CU at least)
+  return tiles_m * (wide ? (p.n + most - 1) / most : (p.n + 15) / 16);
+}
+
+template <int DT, bool GATED>
+int launch(const GroupedParams& p, hipStream_t stream) {
+  bool wide;
+  const long long tiles = tiles_of(p, GATED, wide);
   const dim3 grid((unsigned)tiles), block(64 * kWaves);
   if (wide) hipLaunchKernelGGL((grouped_stream_kernel<DT, 4, GATED>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((grouped_stream_kernel<DT, GATED ? 2 : 1, GATED>), grid, block, 0, stream, p);
@@ -165,6 +170,11 @@ int launch(const GroupedParams& p, hipStream_t stream) {
 }
 
 }  // namespace
+
+int grouped_stream_check(const GroupedParams& p, bool gated) {
+  bool wide;
+  return check_tiles(tiles_of(p, gated, wide), 64 * kWaves);
+}
 
 int grouped_stream_launch(const GroupedParams& p, int dtype, bool gated, hipStream_t stream) {
   if (dtype == CPPMEGA_MI355_E4M3) return gated ? launch<CPPMEGA_MI355_E4M3, true>(p, stream) : launch<CPPMEGA_MI355_E4M3, false>(p, stream);

@@ -591,9 +591,14 @@ long long blocks_of(const GroupedParams& p, int op, bool high, bool cut, bool ga
 
 }  // namespace
 
+int grouped_tile_check(const GroupedParams& p, int op, bool high, bool gated) { return check_tiles(blocks_of(p, op, high, true, gated), high ? 512 : 256); }
+
+int grouped_tile_grads_check(const GroupedParams& rows, const GroupedParams& weights, bool high) {
+  return check_tiles(blocks_of(rows, kRowsGrad, high, false, false) + blocks_of(weights, kWeightsGrad, high, false, false), high ? 512 : 256);
+}
+
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bool gated, hipStream_t stream) {
   const long long blocks = blocks_of(p, op, high, true, gated);
-  if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
   // The gated block in no more low tiles than there are CUs: no second workgroup covers a CU's waits, so its rings are twice as deep (and a
   // tile's parts are counted for one workgroup to a CU).  Measured, us deep / not, rows x n x k: bf16 512 x 4096 x 4096 46 / 66, 256 x 4096 x 4096 36 / 60,
@@ -639,7 +644,6 @@ int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bo
 
 int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream) {
   const long long first = blocks_of(rows, kRowsGrad, high, false, false), blocks = first + blocks_of(weights, kWeightsGrad, high, false, false);
-  if (int rc = check_tiles(blocks, high ? 512 : 256)) return rc;
   const dim3 grid((unsigned)blocks), block(high ? 512 : 256);
 #define CM_GRADS(dt)                                                                                                              \
   do {                                                                                                                            \

@@ -110,6 +110,35 @@ def test_w4_refusals(over, code):
     assert _call(a, "cppmega_mi355_w4_gemm", over) == code
 
 
+@pytest.mark.parametrize("over", [
+    dict(k=1 << 18, n=1 << 20), dict(k=1 << 18, n=1 << 20, dx=None), dict(k=(1 << 18) + 1, n=1 << 20), dict(k=1 << 20, n=33, rows=(1 << 29) - 1), dict(k=1 << 20, n=33, rows=(1 << 29) - 1, dw=None)],
+    ids=lambda o: " ".join(f"{k}={v}" for k, v in o.items()))
+def test_gradients_of_more_tiles_than_a_launch_has_are_refused_before_the_first_launch(over):
+    """(Where no GPU is there, a launch that were tried would give the code of a failed one.)"""
+    a = _lib.GatedGemmBwdArgs()
+    a.dy = a.pre = a.x = a.w = a.dx = a.dw = a.workspace = FAKE
+    a.dtype = a.pre_dtype = a.dx_dtype = a.dw_dtype = _lib.BF16
+    a.offsets_dtype = _lib.I32
+    a.rows, a.experts = 4, 1
+    for k, v in over.items():
+        setattr(a, k, v)
+    a.dy_pitch, a.pre_pitch, a.x_pitch, a.dx_pitch, a.workspace_bytes = a.n, 2 * a.n, a.k, a.k, 1 << 62
+    assert _call(a, "cppmega_mi355_gated_gemm_bwd", {}) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("n, k", [(1 << 21, 1 << 18), (1 << 21, (1 << 18) + 1), ((1 << 21) + 1, 1 << 18)])
+def test_grouped_gradients_of_more_tiles_than_a_launch_has_are_refused_before_the_first_launch(n, k):
+    rows, weights = _lib.GroupedGemmArgs(), _lib.GroupedGemmArgs()
+    for a, op in ((rows, _lib.GROUPED_ROWS_GRAD), (weights, _lib.GROUPED_WEIGHTS_GRAD)):
+        a.struct_size, a.op = C.sizeof(a), op
+        a.x = a.w = a.y = a.offsets = FAKE
+        a.x_dtype = a.y_dtype = _lib.BF16
+        a.offsets_dtype = _lib.I32
+        a.rows, a.experts, a.n, a.k = 4, 1, n, k
+    rows.x_pitch, rows.y_pitch, weights.x_pitch, weights.w_pitch = n, k, n, k
+    assert _lib.load().cppmega_mi355_grouped_gemm_bwd(C.byref(rows), C.byref(weights), C.sizeof(rows), None) == _lib.ERR_UNSUPPORTED
+
+
 def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
     x, w, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
     pre, dy, codes, scale = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=torch.bfloat16)
