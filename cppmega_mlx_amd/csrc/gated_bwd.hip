@@ -11,9 +11,9 @@
 
 namespace cm {
 
-int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream);
-int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream);
-int grouped_gemm_check(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights);
+int grouped_gemm_launch_as(const char* call, const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream);
+int grouped_gemm_bwd_launch_as(const char* call, const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream);
+int grouped_gemm_check(const char* call, const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights);
 
 namespace {
 
@@ -133,9 +133,9 @@ int gated_gemm_bwd_launch(const cppmega_mi355_gated_gemm_bwd_args_t& a, hipStrea
     int log_across = 0;
     while (log_across < 8 && (1 << log_across) < runs) ++log_across;
     const long long across = (runs + (1 << log_across) - 1) >> log_across, blocks = across * (((a.rows << log_across) + kThreads - 1) / kThreads);
-    if (int rc = check_tiles(blocks, kThreads)) return rc;
+    if (int rc = check_tiles("gated_gemm_bwd", blocks, kThreads)) return rc;
     // (what the products refuse is refused before the first launch)
-    if (int rc = grouped_gemm_check(r, w, a.dx != nullptr, a.dw != nullptr)) return rc;
+    if (int rc = grouped_gemm_check("gated_gemm_bwd", r, w, a.dx != nullptr, a.dw != nullptr)) return rc;
     GradParams p;
     p.dy = a.dy; p.pre = a.pre; p.grad = (unsigned short*)a.workspace; p.offsets = a.offsets;
     p.rows = a.rows; p.dy_pitch = a.dy_pitch; p.pre_pitch = a.pre_pitch; p.grad_pitch = grad_pitch(a.n);
@@ -144,8 +144,8 @@ int gated_gemm_bwd_launch(const cppmega_mi355_gated_gemm_bwd_args_t& a, hipStrea
     hipLaunchKernelGGL(gated_grad_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p, log_across, (unsigned)across);
     CM_HIP_CHECK(hipGetLastError());
   }
-  if (a.dx && a.dw) return grouped_gemm_bwd_launch(r, w, stream);
-  return grouped_gemm_launch(a.dx ? r : w, stream);
+  if (a.dx && a.dw) return grouped_gemm_bwd_launch_as("gated_gemm_bwd", r, w, stream);
+  return grouped_gemm_launch_as("gated_gemm_bwd", a.dx ? r : w, stream);
 }
 
 }  // namespace cm

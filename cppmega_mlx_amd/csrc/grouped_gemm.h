@@ -106,15 +106,15 @@ __device__ __forceinline__ bool rows_of_tile(const GroupedParams& p, int mt, int
 }
 
 // A launch has fewer than 2^32 threads.
-inline int check_tiles(long long tiles, int threads) {
-  return tiles * threads > 0xffffffffll ? fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %lld tiles in one call", tiles) : 0;
+inline int check_tiles(const char* call, long long tiles, int threads) {
+  return tiles * threads > 0xffffffffll ? fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "%s: %lld tiles in one call", call, tiles) : 0;
 }
 
 // Whether a kernel's launch has few enough tiles (asked before a call's first launch: one that is refused has written nothing), and the launch.
-int grouped_general_check(const GroupedParams& p, int op, bool gated);
-int grouped_tile_check(const GroupedParams& p, int op, bool high, bool gated);
-int grouped_tile_grads_check(const GroupedParams& rows, const GroupedParams& weights, bool high);
-int grouped_stream_check(const GroupedParams& p, bool gated);
+int grouped_general_check(const char* call, const GroupedParams& p, int op, bool gated);
+int grouped_tile_check(const char* call, const GroupedParams& p, int op, bool high, bool gated);
+int grouped_tile_grads_check(const char* call, const GroupedParams& rows, const GroupedParams& weights, bool high);
+int grouped_stream_check(const char* call, const GroupedParams& p, bool gated);
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream);
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bool gated, hipStream_t stream);
 int grouped_tile_grads_launch(const GroupedParams& rows, const GroupedParams& weights, int dtype, bool high, hipStream_t stream);

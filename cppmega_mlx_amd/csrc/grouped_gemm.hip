@@ -57,30 +57,30 @@ struct Plan {
   bool high, gated;
 };
 
-int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
+int plan_of(const char* call, const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   to.kind = kNothing;
   to.gated = false;
-  if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: unknown op %d", a.op);
+  if (a.op < kRows || a.op > kWeightsGrad) return fail(CPPMEGA_MI355_ERR_SHAPE, "%s: unknown op %d", call, a.op);
   if (a.rows < 0 || a.rows > 0x1fffffffll || a.experts < 1 || a.n < 1 || a.k < 1)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: rows=%lld experts=%d n=%d k=%d", (long long)a.rows, a.experts, a.n, a.k);
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "%s: rows=%lld experts=%d k=%d, weights of %d rows", call, (long long)a.rows, a.experts, a.k, a.n);
   // (columns and contraction are counted in 32 bits, a tile past the end)
   if (a.n > CPPMEGA_MI355_GROUPED_MAX_SIZE || a.k > CPPMEGA_MI355_GROUPED_MAX_SIZE)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: n=%d k=%d, at most 2^30 are served", a.n, a.k);
-  if (a.experts > kMaxExperts) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "grouped_gemm: %d experts, at most %d are served", a.experts, kMaxExperts);
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "%s: k=%d, weights of %d rows; at most 2^30 are served", call, a.k, a.n);
+  if (a.experts > kMaxExperts) return fail(CPPMEGA_MI355_ERR_UNSUPPORTED, "%s: %d experts, at most %d are served", call, a.experts, kMaxExperts);
   const bool fp8 = a.x_dtype == CPPMEGA_MI355_E4M3;
   if (!fp8 && a.x_dtype != CPPMEGA_MI355_F16 && a.x_dtype != CPPMEGA_MI355_BF16)
-    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: operands of dtype %d are not float16 / bfloat16 / e4m3", a.x_dtype);
-  if (fp8 && a.op != kRows) return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: gradients of e4m3 operands are not served");
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "%s: operands of dtype %d are not float16 / bfloat16 / e4m3", call, a.x_dtype);
+  if (fp8 && a.op != kRows) return fail(CPPMEGA_MI355_ERR_DTYPE, "%s: gradients of e4m3 operands are not served", call);
   if (fp8 ? a.y_dtype != CPPMEGA_MI355_F32 && a.y_dtype != CPPMEGA_MI355_F16 && a.y_dtype != CPPMEGA_MI355_BF16
           : a.y_dtype != CPPMEGA_MI355_F32 && a.y_dtype != a.x_dtype)
-    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: a result of dtype %d from operands of dtype %d", a.y_dtype, a.x_dtype);
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "%s: a result of dtype %d from operands of dtype %d", call, a.y_dtype, a.x_dtype);
   if (a.offsets_dtype != CPPMEGA_MI355_I32 && a.offsets_dtype != CPPMEGA_MI355_I64)
-    return fail(CPPMEGA_MI355_ERR_DTYPE, "grouped_gemm: offsets must be int32 or int64");
+    return fail(CPPMEGA_MI355_ERR_DTYPE, "%s: offsets must be int32 or int64", call);
   if (fp8 && a.x_scale_block != 0 && a.x_scale_block != 128)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm: x_scale_block must be 0 (per row) or 128, got %d", a.x_scale_block);
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "%s: x_scale_block must be 0 (per row) or 128, got %d", call, a.x_scale_block);
   if (a.rows == 0 && a.op != kWeightsGrad) return 0;
   if (!a.y || (!a.offsets && a.experts != 1) || (a.rows > 0 && (!a.x || !a.w)) || (fp8 && (!a.x_scale || !a.w_scale)))
-    return fail(CPPMEGA_MI355_ERR_NULL, "grouped_gemm: x / w / y / offsets / scales is NULL");
+    return fail(CPPMEGA_MI355_ERR_NULL, "%s: x / w / y / offsets / scales is NULL", call);
   GroupedParams& p = to.p;
   memset(&p, 0, sizeof(p));
   p.x = a.x; p.w = a.w; p.y = a.y; p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale;
@@ -106,58 +106,63 @@ int plan_of(const cppmega_mi355_grouped_gemm_args_t& a, Plan& to) {
   return 0;
 }
 
-int check(const Plan& plan, int op) {
-  if (plan.kind == kTile) return grouped_tile_check(plan.p, op, plan.high, plan.gated);
-  if (plan.kind == kStream) return grouped_stream_check(plan.p, plan.gated);
-  return plan.kind == kGeneral ? grouped_general_check(plan.p, op, plan.gated) : 0;
+int check(const char* call, const Plan& plan, int op) {
+  if (plan.kind == kTile) return grouped_tile_check(call, plan.p, op, plan.high, plan.gated);
+  if (plan.kind == kStream) return grouped_stream_check(call, plan.p, plan.gated);
+  return plan.kind == kGeneral ? grouped_general_check(call, plan.p, op, plan.gated) : 0;
 }
 
-int launch(const Plan& plan, int op, int dtype, hipStream_t stream) {
-  if (int rc = check(plan, op)) return rc;
+int launch(const char* call, const Plan& plan, int op, int dtype, hipStream_t stream) {
+  if (int rc = check(call, plan, op)) return rc;
   if (plan.kind == kTile) return grouped_tile_launch(plan.p, op, dtype, plan.high, plan.gated, stream);
   if (plan.kind == kStream) return grouped_stream_launch(plan.p, dtype, plan.gated, stream);
   return plan.kind == kGeneral ? grouped_general_launch(plan.p, op, dtype, plan.gated, stream) : 0;
 }
 
 // The gradients that are wanted, and whether one launch makes both; everything that may refuse either of them is asked here.
-int plan_grads(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights, Plan& r, Plan& w,
+int plan_grads(const char* call, const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights, Plan& r, Plan& w,
                bool& together) {
   if (rows.op != kRowsGrad || weights.op != kWeightsGrad)
-    return fail(CPPMEGA_MI355_ERR_SHAPE, "grouped_gemm_bwd: ops %d and %d are not the rows' and the weights' gradient", rows.op, weights.op);
-  int rc = need_rows ? plan_of(rows, r) : 0;
-  if (!rc && need_weights) rc = plan_of(weights, w);
+    return fail(CPPMEGA_MI355_ERR_SHAPE, "%s: ops %d and %d are not the rows' and the weights' gradient", call, rows.op, weights.op);
+  int rc = need_rows ? plan_of(call, rows, r) : 0;
+  if (!rc && need_weights) rc = plan_of(call, weights, w);
   if (rc) return rc;
   together = need_rows && need_weights && r.kind == kTile && w.kind == kTile && rows.x_dtype == weights.x_dtype;
   if (together) {
     r.high = w.high = high_grads(r.p, w.p);
-    return grouped_tile_grads_check(r.p, w.p, r.high);
+    return grouped_tile_grads_check(call, r.p, w.p, r.high);
   }
-  rc = need_rows ? check(r, kRowsGrad) : 0;
-  return !rc && need_weights ? check(w, kWeightsGrad) : rc;
+  rc = need_rows ? check(call, r, kRowsGrad) : 0;
+  return !rc && need_weights ? check(call, w, kWeightsGrad) : rc;
 }
 
 }  // namespace
 
-int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
+// (`call`: the entry point that a refusal names)
+int grouped_gemm_launch_as(const char* call, const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) {
   Plan plan;
-  if (int rc = plan_of(a, plan)) return rc;
-  return launch(plan, a.op, a.x_dtype, stream);
+  if (int rc = plan_of(call, a, plan)) return rc;
+  return launch(call, plan, a.op, a.x_dtype, stream);
 }
+int grouped_gemm_launch(const cppmega_mi355_grouped_gemm_args_t& a, hipStream_t stream) { return grouped_gemm_launch_as("grouped_gemm", a, stream); }
 
-int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream) {
+int grouped_gemm_bwd_launch_as(const char* call, const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream) {
   Plan r, w;
   bool together;
-  if (int rc = plan_grads(rows, weights, true, true, r, w, together)) return rc;
+  if (int rc = plan_grads(call, rows, weights, true, true, r, w, together)) return rc;
   if (together) return grouped_tile_grads_launch(r.p, w.p, rows.x_dtype, r.high, stream);
-  const int rc = launch(r, kRowsGrad, rows.x_dtype, stream);
-  return rc ? rc : launch(w, kWeightsGrad, weights.x_dtype, stream);
+  const int rc = launch(call, r, kRowsGrad, rows.x_dtype, stream);
+  return rc ? rc : launch(call, w, kWeightsGrad, weights.x_dtype, stream);
+}
+int grouped_gemm_bwd_launch(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, hipStream_t stream) {
+  return grouped_gemm_bwd_launch_as("grouped_gemm_bwd", rows, weights, stream);
 }
 
 // Whether the gradients that are wanted would be launched, with the reason if not.
-int grouped_gemm_check(const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights) {
+int grouped_gemm_check(const char* call, const cppmega_mi355_grouped_gemm_args_t& rows, const cppmega_mi355_grouped_gemm_args_t& weights, bool need_rows, bool need_weights) {
   Plan r, w;
   bool together;
-  return plan_grads(rows, weights, need_rows, need_weights, r, w, together);
+  return plan_grads(call, rows, weights, need_rows, need_weights, r, w, together);
 }
 
 // The gated block is a product of rows with 2 n rows of a weight, whose kernels pair them off; the same rules choose among them.
@@ -176,7 +181,7 @@ int gated_gemm_launch(const cppmega_mi355_gated_gemm_args_t& a, hipStream_t stre
   g.rows = a.rows; g.x_pitch = a.x_pitch; g.y_pitch = a.y_pitch;
   g.experts = a.experts; g.n = 2 * a.n; g.k = a.k; g.zero_tail = a.zero_tail;
   Plan plan;
-  if (int rc = plan_of(g, plan)) return rc;
+  if (int rc = plan_of("gated_gemm", g, plan)) return rc;
   plan.gated = true;
   plan.p.n = a.n;
   plan.p.activation = a.activation;
@@ -187,7 +192,7 @@ int gated_gemm_launch(const cppmega_mi355_gated_gemm_args_t& a, hipStream_t stre
   // 4096 16 / 19, 128 x 2048 x 4096 24 / 19; 512 x 8 experts x 512 x 2048 31 / 21.
   const double passes = a.experts > 1 ? a.rows / 16.0 + 0.5 * a.experts : (double)((a.rows + 15) / 16);
   if (plan.kind == kTile && passes * a.n <= 8192.0) plan.kind = kStream;
-  return launch(plan, kRows, a.x_dtype, stream);
+  return launch("gated_gemm", plan, kRows, a.x_dtype, stream);
 }
 
 }  // namespace cm

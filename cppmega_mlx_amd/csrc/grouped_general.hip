@@ -249,7 +249,7 @@ long long tiles_of(const GroupedParams& p, int op, bool gated) {
 
 }  // namespace
 
-int grouped_general_check(const GroupedParams& p, int op, bool gated) { return check_tiles(tiles_of(p, op, gated), 256); }
+int grouped_general_check(const char* call, const GroupedParams& p, int op, bool gated) { return check_tiles(call, tiles_of(p, op, gated), 256); }
 
 int grouped_general_launch(const GroupedParams& p, int op, int dtype, bool gated, hipStream_t stream) {
   const dim3 grid((unsigned)tiles_of(p, op, gated)), block(256);

@@ -171,9 +171,9 @@ int launch(const GroupedParams& p, hipStream_t stream) {
 
 }  // namespace
 
-int grouped_stream_check(const GroupedParams& p, bool gated) {
+int grouped_stream_check(const char* call, const GroupedParams& p, bool gated) {
   bool wide;
-  return check_tiles(tiles_of(p, gated, wide), 64 * kWaves);
+  return check_tiles(call, tiles_of(p, gated, wide), 64 * kWaves);
 }
 
 int grouped_stream_launch(const GroupedParams& p, int dtype, bool gated, hipStream_t stream) {

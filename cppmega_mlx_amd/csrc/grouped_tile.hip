@@ -591,10 +591,10 @@ long long blocks_of(const GroupedParams& p, int op, bool high, bool cut, bool ga
 
 }  // namespace
 
-int grouped_tile_check(const GroupedParams& p, int op, bool high, bool gated) { return check_tiles(blocks_of(p, op, high, true, gated), high ? 512 : 256); }
+int grouped_tile_check(const char* call, const GroupedParams& p, int op, bool high, bool gated) { return check_tiles(call, blocks_of(p, op, high, true, gated), high ? 512 : 256); }
 
-int grouped_tile_grads_check(const GroupedParams& rows, const GroupedParams& weights, bool high) {
-  return check_tiles(blocks_of(rows, kRowsGrad, high, false, false) + blocks_of(weights, kWeightsGrad, high, false, false), high ? 512 : 256);
+int grouped_tile_grads_check(const char* call, const GroupedParams& rows, const GroupedParams& weights, bool high) {
+  return check_tiles(call, blocks_of(rows, kRowsGrad, high, false, false) + blocks_of(weights, kWeightsGrad, high, false, false), high ? 512 : 256);
 }
 
 int grouped_tile_launch(const GroupedParams& p, int op, int dtype, bool high, bool gated, hipStream_t stream) {

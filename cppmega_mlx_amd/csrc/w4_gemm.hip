@@ -290,7 +290,7 @@ int launch(W4Params p, hipStream_t stream) {
   const int waves = work >= 4096 || steps * tiles < 32 ? 4 : 8;
   p.log_split = __builtin_ctz(waves / tiles);
   const int out = 16 * (p.gated ? tiles / 2 : tiles), parts = (q.n + out - 1) / out;
-  if (int rc = check_tiles(parts, 64 * waves)) return rc;
+  if (int rc = check_tiles("w4_gemm", parts, 64 * waves)) return rc;
   constexpr long long kMostY = 65535;                            // (of a grid)
   for (long long t = 0; t < tiles_m; t += kMostY) {
     p.tile0 = (int)t;

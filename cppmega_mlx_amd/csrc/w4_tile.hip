@@ -238,7 +238,7 @@ int launch(W4Params p, hipStream_t stream) {
   const long long tails = q.experts + 1 < q.rows ? q.experts + 1 : q.rows;        // tiles of rows that are not full, at most
   const long long tiles_m = !q.offsets ? (q.rows + kBM - 1) / kBM : q.rows / kBM + tails;
   const int out = (p.gated ? 16 : 32) * (kWaves / SLICES), parts = (q.n + out - 1) / out;
-  if (int rc = check_tiles(parts, 64 * kWaves)) return rc;
+  if (int rc = check_tiles("w4_gemm", parts, 64 * kWaves)) return rc;
   constexpr long long kMostY = 65535;                            // (of a grid)
   for (long long t = 0; t < tiles_m; t += kMostY) {
     p.tile0 = (int)t;

@@ -139,6 +139,46 @@ def test_grouped_gradients_of_more_tiles_than_a_launch_has_are_refused_before_th
     assert _lib.load().cppmega_mi355_grouped_gemm_bwd(C.byref(rows), C.byref(weights), C.sizeof(rows), None) == _lib.ERR_UNSUPPORTED
 
 
+def _refused_by(fn, *args):
+    assert getattr(_lib.load(), fn)(*args) not in (_lib.OK, _lib.ERR_LAUNCH)
+    return _lib.load().cppmega_mi355_last_error().decode()
+
+
+def test_a_refusal_names_the_call():
+    """The gated block and the 4-bit products share checks with the grouped products: sizes, experts, tiles of a launch."""
+    g = _lib.GatedGemmArgs()
+    g.x = g.w = g.y = FAKE
+    g.x_dtype = g.y_dtype = _lib.BF16
+    g.offsets_dtype = _lib.I32
+    for over in (dict(rows=-1), dict(experts=513, offsets=FAKE), dict(k=0), dict(x_dtype=_lib.F32), dict(y_dtype=_lib.F16), dict(x=None), dict(rows=(1 << 29) - 1, n=1 << 22)):
+        a = _lib.GatedGemmArgs.from_buffer_copy(g)
+        a.rows, a.experts, a.n, a.k, a.x_pitch, a.y_pitch, a.struct_size = 4, 1, 64, 64, 64, 64, C.sizeof(a)
+        for k, v in over.items():
+            setattr(a, k, v)
+        assert _refused_by("cppmega_mi355_gated_gemm", C.byref(a), C.sizeof(a), None).startswith("gated_gemm: "), over
+    b = _lib.GatedGemmBwdArgs()
+    b.dy = b.pre = b.x = b.w = b.dx = b.dw = b.workspace = FAKE
+    b.dtype = b.pre_dtype = b.dx_dtype = b.dw_dtype = _lib.BF16
+    b.offsets_dtype = _lib.I32
+    for over in (dict(rows=-1), dict(experts=513, offsets=FAKE), dict(k=0), dict(dx_dtype=_lib.F16), dict(w=None), dict(n=1 << 20, k=1 << 18), dict(rows=(1 << 29) - 1, n=1 << 20)):
+        a = _lib.GatedGemmBwdArgs.from_buffer_copy(b)
+        a.rows, a.experts, a.n, a.k, a.struct_size, a.workspace_bytes = 4, 1, 64, 64, C.sizeof(a), 1 << 62
+        for k, v in over.items():
+            setattr(a, k, v)
+        a.dy_pitch, a.pre_pitch, a.x_pitch, a.dx_pitch = a.n, 2 * a.n, a.k, a.k
+        assert _refused_by("cppmega_mi355_gated_gemm_bwd", C.byref(a), C.sizeof(a), None).startswith("gated_gemm_bwd: "), over
+    w = _lib.W4GemmArgs()
+    w.x = w.w = w.scale = w.y = FAKE
+    w.x_dtype = w.y_dtype = w.scale_dtype = _lib.BF16
+    w.activation, w.offsets_dtype = _lib.GATE_NONE, _lib.I32
+    for n, k in ((1 << 30, 32), (1 << 30, 1024)):
+        w.rows, w.experts, w.n, w.k, w.group, w.x_pitch, w.y_pitch, w.struct_size = 64, 1, n, k, 32, k, n, C.sizeof(w)
+        assert _refused_by("cppmega_mi355_w4_gemm", C.byref(w), C.sizeof(w), None).startswith("w4_gemm: "), n
+    r = _lib.GroupedGemmArgs()
+    r.op, r.rows, r.struct_size = _lib.GROUPED_ROWS, -1, C.sizeof(r)
+    assert _refused_by("cppmega_mi355_grouped_gemm", C.byref(r), C.sizeof(r), None).startswith("grouped_gemm: ")
+
+
 def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
     x, w, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
     pre, dy, codes, scale = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=torch.bfloat16)
