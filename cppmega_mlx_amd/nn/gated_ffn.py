@@ -56,7 +56,8 @@ def gated_gemm_bwd(dy: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, w: torc
                    need_dw: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """``(dx [T, K], dw like w)`` in the operands' type (caller-owned ones may be float32); one that is not needed is None.
 
-    dg and du are rounded to the operands' type between the two launches."""
+    dg and du are rounded to the operands' type between the two launches.  In float16 they are infinite from 65520 on (dx of that row and dw of
+    that output are infinite or NaN then) and multiples of 2^-24 below 2^-14, whatever type the results have: scale the loss."""
     if dx is None and dw is None and need_dx and need_dw:
         done = ops.host.gated_gemm_bwd(dy, pre, x, w, offsets, ops.gate_code(activation))
         if done is not None:

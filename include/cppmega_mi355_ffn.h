@@ -57,6 +57,8 @@ int cppmega_mi355_gated_gemm(const cppmega_mi355_gated_gemm_args_t* args, size_t
 /* Gradients, s = sigmoid(z(g)):
  *   dg = dy u (s + g s (1 - s) z'(g)),  du = dy g s    (float32, rounded to `dtype` in the workspace)
  *   dx = dg w_gate + du w_up,  dw = (dg | du)^T x      (zeros for an expert without rows)
+ * F16: a dg or du of magnitude 65520 or more is an infinity (and dx of its row, dw of its output infinite or NaN), one
+ * below 2^-14 a multiple of 2^-24, whatever the results' types; scale the loss, as for any gradient in float16.
  * The workspace holds dg and du; it need not be initialised. */
 typedef struct cppmega_mi355_gated_gemm_bwd_args {
   uint32_t struct_size;
