@@ -13,7 +13,8 @@ group's sum of x comes off again: rows with infinities give NaN, and 32 times a 
 Made for the rows of a decode step: the codes are widened once for every 16 rows of an expert (64 where there are many), so long prompts
 cost as many passes.  By expert: a leading axis ``[E, ..]`` and ``offsets [E + 1]`` as
 in ``grouped_gemm``.  Rows behind the last expert's: zeros in an output made here, left as they were in a caller-owned one, which must not overlap
-the operands.  Fewer than 2^29 rows, up to 2^24 elements apart, N up to 2^30, K up to 2^24, up to 512 experts.
+the operands.  Fewer than 2^29 rows, up to 2^24 elements apart, N up to 2^30, K up to 2^24, up to 512 experts, and fewer than 2^32
+threads across the outputs (of up to four rows 2^29 outputs or, gated, 2^28 come to that, of more twice as many: they are refused).
 
 The 8-bit sibling is ``nn/_tilelang/fused_fp8_gemm.py``; the block over 16- and 8-bit weights ``gated_ffn.py``.
 """

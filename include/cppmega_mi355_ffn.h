@@ -10,6 +10,11 @@
  * non-decreasing, offsets[experts] <= rows, read on the device (offsets that break this give unspecified values, but no access outside
  * the operands).  offsets NULL: one expert has all rows.  Rows of an output from offsets[experts] on are left as they
  * were, or zeroed with zero_tail.
+ *
+ * A launch has fewer than 2^32 threads: a call whose sizes are within the limits below but whose tiles are more is refused
+ * (UNSUPPORTED) before anything is written.  The gated block has 256 threads for 16 rows of an expert and 32 outputs at the least, so
+ * up to 16 rows of one matrix reach that with 2^29 outputs; the 4-bit products have 256 for 32 outputs (gated: 16) of up to four rows of one matrix,
+ * for 64 (32) of more.
  */
 #ifndef CPPMEGA_MI355_FFN_H_
 #define CPPMEGA_MI355_FFN_H_

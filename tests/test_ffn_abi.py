@@ -179,6 +179,26 @@ def test_a_refusal_names_the_call():
     assert _refused_by("cppmega_mi355_grouped_gemm", C.byref(r), C.sizeof(r), None).startswith("grouped_gemm: ")
 
 
+@pytest.mark.parametrize("rows, n, gated", [(1, 1 << 29, False), (4, 1 << 28, True), (5, 1 << 30, False), (16, 1 << 29, True)])
+def test_w4_outputs_that_one_launch_has_no_threads_for_are_refused(rows, n, gated):
+    a = _lib.W4GemmArgs()
+    a.x = a.w = a.scale = a.y = FAKE
+    a.x_dtype = a.y_dtype = a.scale_dtype = _lib.BF16
+    a.activation, a.offsets_dtype = _lib.GATE_SILU if gated else _lib.GATE_NONE, _lib.I32
+    a.rows, a.experts, a.n, a.k, a.group, a.x_pitch, a.y_pitch = rows, 1, n, 32, 32, 32, n
+    assert _call(a, "cppmega_mi355_w4_gemm", {}) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("rows", [1, 16])
+def test_gated_outputs_that_one_launch_has_no_threads_for_are_refused(rows):
+    a = _lib.GatedGemmArgs()
+    a.x = a.w = a.y = FAKE
+    a.x_dtype = a.y_dtype = _lib.BF16
+    a.offsets_dtype = _lib.I32
+    a.rows, a.experts, a.n, a.k, a.x_pitch, a.y_pitch = rows, 1, 1 << 29, 8, 8, 1 << 29
+    assert _call(a, "cppmega_mi355_gated_gemm", {}) == _lib.ERR_UNSUPPORTED
+
+
 def test_python_entry_points_refuse_host_tensors_and_bad_arguments():
     x, w, off = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
     pre, dy, codes, scale = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1, dtype=torch.bfloat16)
