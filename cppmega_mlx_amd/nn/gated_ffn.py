@@ -12,8 +12,8 @@
 
 By expert: ``w [E, 2 F, K]`` and ``offsets [E + 1]``, an int32 or int64 device tensor as ``grouped_gemm`` takes it (rows sorted by expert; read on
 the stream, so that a captured call can be replayed with others; up to 512 experts).  Rows behind the last expert's: zeros in an output
-made here, left as they were in a caller-owned one, which must not overlap the operands (and makes a graph that has saved it refuse its backward
-pass).  Rows may have a pitch of their own; fewer than 2^29 rows, F up to 2^29, K up to 2^30, and a launch of fewer than 2^32 threads (few rows
+made here, left as they were in a caller-owned one, which must not overlap the operands or another output (and makes a graph that has saved it
+refuse its backward pass).  Rows may have a pitch of their own; fewer than 2^29 rows, F up to 2^29, K up to 2^30, and a launch of fewer than 2^32 threads (few rows
 to an expert have 256 for 16 of its rows, whether they are there or not, and 32 outputs: more are refused); rows that begin on 16 bytes take the faster kernels.
 
 The down projection behind the block is ``grouped_gemm`` (a dense one: ``grouped_gemm`` of one expert); for single tokens over 4-bit

@@ -1221,6 +1221,8 @@ def gated_gemm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | None, *
         _own_rows(pre, "pre", T, a.pre_pitch)
         a.pre_dtype = _dtype_or_raise(pre, "pre", (_lib.F32, a.x_dtype))
         a.pre = pre.data_ptr()
+        if T > 0 and pre.data_ptr() == out.data_ptr():
+            raise ValueError("out and pre are one place")
     if fp8:
         blocks_n, blocks_k = (n + 127) // 128, (k + 127) // 128
         want = (2, blocks_n, blocks_k) if offsets is None else (experts, 2, blocks_n, blocks_k)
@@ -1272,6 +1274,8 @@ def gated_gemm_backward(dy: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, w:
         if tuple(dw.shape) != tuple(w.shape):
             raise ValueError(f"dw must have shape {tuple(w.shape)}; got {tuple(dw.shape)}")
         a.dw_dtype = _dtype_or_raise(dw, "dw", (_lib.F32, a.dtype))
+        if dx is not None and T > 0 and dx.data_ptr() == dw.data_ptr():
+            raise ValueError("dx and dw are one place")
     a.dy, a.pre, a.x, a.w, a.dx, a.dw = dy.data_ptr(), pre.data_ptr(), x.data_ptr(), w.data_ptr(), _lib.ptr(dx), _lib.ptr(dw)
     a.zero_tail = int(bool(zero_tail))
     lib = _lib.load()
