@@ -8,10 +8,14 @@
 // rows of x, from the cache but behind weights, waited for memory.  x passes through LDS instead, as much of it at a time as there is room,
 // in the codes' order.
 //
-// Many experts are bound by memory: 61 experts of 4096 x 7168 codes, groups of 64, in 241 us, 4.2 TB/s.  One matrix is bound by the vector
-// instructions that widen its codes, by the start (arguments, x into LDS, the first weights: 4 to 5 us) and by the sums' way at the end: 16 x 16384 x
-// 7168 in 21 us, 2.9 TB/s; 1 x 2048 x 7168 in 9.  Tried at 1 x 16384 x 7168 with nothing gained (18 to 21 us): two or four tiles to a wavefront, x kept
-// in registers, 16 steps of weights on their way, 16 wavefronts, x read past LDS (as much of the first-level cache's time as the weights).
+// Times in this file: bfloat16, groups of 64, biases, and weights that come from memory (1.2 GB of them in turn), unless it says otherwise.
+// Many experts are bound by memory: 61 experts of 4096 x 7168 codes in 244 us.  They read 1378 MiB (counted) where codes, scales and
+// biases are 961, which fits lines of scales that come anew for every eight steps, 32 bytes of a row.  One matrix leaves a
+// CU one or two workgroups, whose wavefronts wait for half of their time (16 x 16384 x 7168, float16, groups of 128: waits 0.52 of the wavefronts' cycles, vector
+// instructions 0.26 and matrix ones 0.11 of the SIMDs'): for the start (arguments, x into LDS, the first weights: 4 to 5 us), for memory, and at
+// the end for each other's sums.  16 x 16384 x 7168 27.5 us (float16, groups of 128, no biases 25, and 21 where the weights are in the last-level
+// cache); 1 x 2048 x 7168 9.5.  Tried at 1 x 16384 x 7168 (float16, groups of 128, no biases: 19) with nothing gained, 18 to 21 us: two or four tiles to
+// a wavefront, x kept in registers, 16 steps of weights on their way, 16 wavefronts, x read past LDS (as much of the first-level cache's time as the weights).
 
 #include <string.h>
 
@@ -280,11 +284,11 @@ int launch(W4Params p, hipStream_t stream) {
   const long long work = tiles_m * ((q.n + 15) / 16) * (p.gated ? 2 : 1);         // tiles of rows of x and of the weight
   const int steps = q.k / 128;
   // Tiles of a workgroup share x's way through LDS: as few as leave a workgroup to a CU (with up to four rows of x, two).  Four wavefronts where
-  // there is plenty of work or little to divide.  Measured, us 1 / 2 / 4 tiles with 4 wavefronts, then with 8, rows x n x k, bfloat16: 1 x 2048 x
-  // 7168 10 / 15 / 25, 9.5 / 12 / 19; 4 x 16384 x 7168 24 / 22 / 26, 29 / 22 / 22; 48 x 2048 x 7168 27 / 26 / 31, 30 / 21 / 24; 48 x 4096 x 4096 26 /
-  // 20 / 20, 29 / 21 / 16; 8 x 2048 x 2048 7.8 / 8.4 / 11, 9.2 / 9.3 / 9.7; 16 x 8192 x 2048 13 / 11 / 12, 14 / 10 / 11; 16 x 16384 x 7168 50 / 31 /
-  // 31, 61 / 34 / 25; 64 x 8192 x 8192 105 / 58 / 41, 117 / 63 / 36; 1024 x 1024 x 512 41 / 23 / 14, 62 / 45 / 24; 256 x 61 experts gated, 2 and 4
-  // tiles: 270 / 243, 312 / 263.
+  // there is plenty of work or little to divide.  Measured, us 1 / 2 / 4 tiles with 4 wavefronts, then with 8, rows x n x k: 1 x 2048 x
+  // 7168 10 / 15 / 25, 9.6 / 12 / 19; 4 x 16384 x 7168 26 / 24 / 30, 30 / 23 / 23; 48 x 2048 x 7168 27 / 26 / 32, 30 / 21 / 24; 48 x 4096 x 4096 26 /
+  // 20 / 20, 30 / 21 / 15; 8 x 2048 x 2048 7.8 / 8.5 / 11, 9.2 / 9.3 / 9.9; 16 x 8192 x 2048 13 / 11 / 12, 14 / 10 / 11; 16 x 16384 x 7168 50 / 35 /
+  // 37, 60 / 33 / 28; 64 x 8192 x 8192 105 / 58 / 46, 117 / 64 / 39; 1024 x 1024 x 512 41 / 23 / 14, 61 / 44 / 24; 256 x 61 experts gated, 2 and 4
+  // tiles: 269 / 243, 306 / 263.
   const bool thin = q.rows <= 4 && q.experts == 1;
   const int tiles = work > 512 && !thin ? 4 : work > 256 || p.gated ? 2 : 1;
   const int waves = work >= 4096 || steps * tiles < 32 ? 4 : 8;
@@ -341,9 +345,10 @@ int w4_gemm_launch(const cppmega_mi355_w4_gemm_args_t& a, hipStream_t stream) {
   p.scale = a.scale; p.bias = a.bias; p.gated = is_gated;
   const bool f16 = a.x_dtype == CPPMEGA_MI355_F16, wide = a.scale_dtype == CPPMEGA_MI355_F32;
   // Weights widened once for 64 rows, or once for 16 with eight times the wavefronts: the former from 32 rows to an expert on, where there is as much
-  // work as makes up for its start, in tiles of 16 x 16 results.  Measured, us 64 / 16 rows, rows x n x k, bfloat16: 64 x 8192 x 8192 43 / 42, 64 x 16384 x
-  // 4096 24 / 37, 64 x 4096 x 4096 42 / 18, 128 x 4096 x 4096 22 / 21, 256 x 4096 x 4096 23 / 35, 32 x 32768 x 2048 21 / 23, 512 x 8192 x 8192 109 / 215, 1024 x 1024 x 512
-  // 18 / 14; gated 512 x 16 experts x 1024 x 2048 25 / 33, 256 x 16 experts x 1024 x 7168 62 / 60.
+  // work as makes up for its start, in tiles of 16 x 16 results.  Measured, us 64 / 16 rows, rows x n x k: 64 x 8192 x 8192 54 / 39, 64 x 16384 x
+  // 4096 31 / 40, 64 x 4096 x 4096 27 / 16, 128 x 4096 x 4096 28 / 23, 256 x 4096 x 4096 29 / 36, 32 x 32768 x 2048 25 / 24, 512 x 8192 x 8192 135 / 229, 4096 x
+  // 4096 x 4096 303 / 457; gated 512 x 16 experts x 1024 x 2048 25 / 32, 256 x 16 experts x 1024 x 7168 61 / 53.  Where the rule takes the slower one: 1024 x 1024
+  // x 512 11 / 14.
   const double tiles = ((a.rows + 15) / 16 + (a.experts > 1 ? a.experts / 2 : 0)) * (((double)a.n * (is_gated ? 2 : 1) + 15) / 16);
   if (a.rows >= 32ll * a.experts && a.k >= 1024 && tiles >= 2560.0) return w4_tile_launch(p, a.group, f16, wide, stream);
   return a.group == 32 ? launch_group<32>(p, f16, wide, stream) : a.group == 64 ? launch_group<64>(p, f16, wide, stream) : launch_group<128>(p, f16, wide, stream);

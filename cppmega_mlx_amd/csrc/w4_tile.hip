@@ -8,7 +8,8 @@
 //
 // Bound by the matrix cores, the vector instructions that widen and scale, and reads of x from LDS, a third of the time each, which the
 // two wavefronts of a SIMD overlap little (a set order of instructions changed nothing); a pass takes 4 us and more, the memory's answer to the
-// requests made a pass ahead.  512 x 8192 x 8192: 109 us, 0.63 PFLOP/s; 4096 x 4096 x 4096 242 us, 0.57.
+// requests made a pass ahead.  Bfloat16, groups of 128: 512 x 8192 x 8192 109 us, 0.63 PFLOP/s; 4096 x 4096 x 4096 242 us, 0.57; groups of 64, which
+// change places and are scaled twice as often: 135 and 303.
 
 #include "w4.h"
 
@@ -252,8 +253,9 @@ int launch(W4Params p, hipStream_t stream) {
 template <int G, bool F16, int S>
 int choose(const W4Params& p, hipStream_t stream) {
   const GroupedParams& q = p.g;
-  // Four slices while that leaves one workgroup to a CU.  Measured, us 2 / 4 slices, rows x n x k, bfloat16: 200 x 4096 x 4096 37 / 29, 48 x 16384 x 8192
-  // 53 / 43, 64 x 32768 x 1024 15 / 19, 512 x 8192 x 8192 109 / 159, 300 x 8 experts x 2048 x 4096 39 / 30.
+  // Four slices while that leaves one workgroup to a CU.  Measured, us 2 / 4 slices, rows x n x k, bfloat16, groups of 64, biases, weights from memory: 200 x
+  // 4096 x 4096 38 / 28, 48 x 16384 x 8192 67 / 52, 64 x 8192 x 8192 69 / 54, 64 x 32768 x 1024 18 / 24, 512 x 8192 x 8192 136 / 204; where the rule takes the slower
+  // one: 300 x 8 experts x 2048 x 4096 39 / 31.
   const long long work = ((q.rows + kBM - 1) / kBM + q.experts / 2) * (((long long)q.n * (p.gated ? 2 : 1) + 31) / 32);   // pairs, for 64 rows each
   return work <= 512 ? launch<G, F16, S, 4>(p, stream) : launch<G, F16, S, 2>(p, stream);
 }
