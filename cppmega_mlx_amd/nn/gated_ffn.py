@@ -119,6 +119,6 @@ def gated_gemm_apply(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor | N
     """Differentiable ``gated_gemm``: first derivatives, by the backward pass (a tangent of forward mode is refused).
 
     ``pre_dtype``: what the two products are kept in for the backward pass, float32 (unrounded) or x's type (half the memory; the
-    gradients' error grows by a fifth, as one more rounding of theirs).  They are not kept where no gradient is wanted."""
+    gradients' error grows by a fifth, as one more rounding of theirs, and products beyond 65504 are infinite in float16).  They are not kept where no gradient is wanted."""
     # (by the function in either case: it refuses the derivatives that it lacks, where the bare call would drop them)
     return _GatedGemmFunction.apply(x, w, offsets, activation, pre_dtype, torch.is_grad_enabled() and (x.requires_grad or w.requires_grad))
